@@ -291,6 +291,71 @@ int     sdh_ffn_stack_forward(sdh_ffn_stack * s, int act, const float * x, float
 int     sdh_ffn_stack_status(sdh_ffn_stack * s, int64_t * nonfinite, int64_t * timeouts);
 int64_t sdh_ffn_stack_payload_bytes(const sdh_ffn_stack * s);
 
+/* ---- around the projections: norm, 8-bit activations, dense Q8_0 projection, adapters ----------------------------
+ * What a layer runs next to its SeedDelta nodes: the norm that feeds them (build_norm before build_ffn), the tensors of
+ * the same layer that have no payload and stay dense, and the adapters that build_lora_mm adds to every projection
+ * (src/llama-graph.cpp:672-746). All calls below take device pointers, run on `stream` (NULL = the legacy default stream),
+ * allocate nothing, keep nothing between calls and may be recorded into a HIP graph from the first call on. The current
+ * device must be the one sdh_init() bound. n_tokens == 0 is a no-op (whatever the pointers). Rows may be strided (ld* in elements); every output is
+ * written for its n_tokens rows and nowhere else. Unless an entry says otherwise, outputs must not overlap inputs. */
+
+/* Activations in 8 bits: q int8 [n, n_tokens] with column stride ldq, d F32 [n/32, n_tokens] with column stride ldd; the
+ * value at i is q[i] * d[i / 32]: Q8_0's blocks of 32 (ggml/src/ggml-quants.c:199), quants and scales in planes of their own,
+ * scales in F32 (a block of small or large activations does not leave F16's range). */
+typedef struct sdh_q8 {
+    int8_t * q;
+    int64_t  ldq;
+    float *  d;
+    int64_t  ldd;
+} sdh_q8;
+
+/* sdh_rms_norm — residual addition, root-mean-square norm and weight in one pass (ggml_add, ggml_rms_norm, ggml_mul:
+ * ggml/src/ggml-cpu/ops.cpp), for each token
+ *   s = x + res                          (res NULL: s = x)
+ *   z = s * weight / sqrt(mean(s^2) + eps)   (weight NULL: 1)
+ * sum (may be NULL; may be x or res with the same stride): s, the residual stream after the addition.
+ * y (may be NULL; may be x or res with the same stride, if `sum` is not): z in F32.
+ * out8 (may be NULL): z in 8 bits, per block of 32: d = max|z| / 127, q = z / d rounded to the nearest integer, ties to even.
+ * s is rounded to F32; the mean, z and the division are formed in 64 bits and each output is rounded once: a value next to the
+ * border of two 8-bit steps goes to the right one. The bits of an output do not depend on which others are asked for. A block
+ * that holds a value that is not finite gets a scale that is not finite and quants of zero (all 32 values stand for NaN); a
+ * block of zeros gets d = 0.
+ * n >= 1; with out8 n % 32 == 0. */
+int sdh_rms_norm(const float * x, int64_t ldx, const float * res, int64_t ldr, const float * weight, float eps,
+                 int64_t n, int64_t n_tokens, float * sum, int64_t lds, float * y, int64_t ldy, const sdh_q8 * out8,
+                 void * stream);
+
+/* sdh_q8_quantize — x in 8 bits by the rule above (what a dense ffn_down reads: act(g) * u has no norm before it). */
+int sdh_q8_quantize(const float * x, int64_t ldx, int64_t n, int64_t n_tokens, const sdh_q8 * out8, void * stream);
+
+/* sdh_lora_* — low-rank adapters of many requests beside one projection [n_in -> n_out] (SeedDelta or dense):
+ *   y[:,t] = base[:,t] + scale_a * B_a (A_a x[:,t]),  a = ids[t]
+ * the graph of build_lora_mm (ggml_mul_mat(b, ggml_mul_mat(a, x)), ggml_scale, ggml_add) with the adapter chosen per token.
+ * A set holds 1 .. SDH_LORA_MAX_ADAPTERS adapters of ranks 1 .. SDH_LORA_MAX_RANK, each of its own rank and type (F16 or F32). */
+#define SDH_LORA_MAX_ADAPTERS 4096
+#define SDH_LORA_MAX_RANK     512
+typedef struct sdh_lora sdh_lora;    /* opaque: the device-resident adapters of one projection */
+typedef struct sdh_lora_desc {
+    sdh_tensor a;       /* [n_in, r]   F16/F32: <name>.lora_a */
+    sdh_tensor b;       /* [r, n_out]  F16/F32: <name>.lora_b */
+    float      scale;   /* alpha / r times the user's scale (llama_adapter_lora_weight::get_scale, src/llama-adapter.h) */
+    int32_t    reserved;
+} sdh_lora_desc;
+/* Upload a set once; the host tensors (views honoured) are not referenced after the call returns. */
+int     sdh_lora_create(int64_t n_in, int64_t n_out, const sdh_lora_desc * adapters, int n_adapters, sdh_lora ** out);
+void    sdh_lora_destroy(sdh_lora * l);                       /* waits for the device */
+int64_t sdh_lora_bytes(const sdh_lora * l);                   /* the adapters' weights as stored */
+/* Bytes of the caller's workspace for sdh_lora_apply with n_tokens (16-byte aligned; contents need not be kept or cleared;
+ * calls that may overlap — two streams, two graphs in flight — take one each). */
+int64_t sdh_lora_workspace_bytes(const sdh_lora * l, int64_t n_tokens);
+/* ids: int32 [n_tokens] on the device, read by the kernels (a captured graph sees the ids of the replay); anything outside
+ * [0, n_adapters) means no adapter: that token's y is its base. ids NULL: every token has adapter 0. Tokens may have their
+ * adapters in any order. base: F32 [n_out, n_tokens]; may be y with the same stride (add in place) or NULL (the adapters'
+ * part alone; zero without one). A token's bits do not depend on which other tokens are in the call as long as n_tokens
+ * stays the same. Several adapters on one token: one call after the other, base = y. */
+int     sdh_lora_apply(const sdh_lora * l, const int32_t * ids, const float * x, int64_t ldx, int64_t n_tokens,
+                       const float * base, int64_t ldb, float * y, int64_t ldy, void * ws, int64_t ws_bytes, void * stream);
+
 /* Regenerate a tile of the dense base W0 (bit-exact integer XOR indexing into the per-block
  * table G_b = FWHT(d2_b)): out[(o-o0) + (i-i0)*(o1-o0)] = W0[o,i] for o in [o0,o1), i in [i0,i1).
  * `out` is a device or host pointer according to `flags` (SDH_FWD_HOST_IO). Used by the
@@ -315,6 +380,13 @@ typedef struct sdh_scan  sdh_scan;    /* opaque: RNG stream + the last candidate
 int     sdh_dense_create(const sdh_tensor * W, sdh_dense ** out);
 void    sdh_dense_destroy(sdh_dense * W);
 int64_t sdh_dense_bytes(const sdh_dense * W);      /* bytes as stored (the scan's algorithmic bytes) */
+/* sdh_dense_forward_q8 — a dense Q8_0 weight times 8-bit activations, for the projections of a layer that have no payload:
+ *   y[o,t] = sum_b d_w[b,o] * d[b,t] * sum_{i in block b} q_w[i,o] * q[i,t]
+ * the arithmetic of ggml's Q8_0 mul_mat (ggml_vec_dot_q8_0_q8_0, ggml/src/ggml-cpu/quants.c): integer sums inside a block
+ * of 32, F32 across blocks. x: [n_in, n_tokens] as sdh_rms_norm / sdh_q8_quantize write it, x->q 16-byte aligned with ldq a
+ * multiple of 16. y: F32 [n_out, n_tokens] with column stride ldy. Same rules as the calls around the projections above.
+ * F16 / F32 weights: SDH_ERR_UNSUPPORTED. */
+int     sdh_dense_forward_q8(const sdh_dense * W, const sdh_q8 * x, int64_t n_tokens, float * y, int64_t ldy, void * stream);
 
 typedef struct sdh_scan_params {
     int32_t scheme;             /* 0 = COO, 1 = block                     (--scheme)                    */

@@ -117,6 +117,16 @@ static std::vector<float> pack_f32(const sdh_tensor & t) {     // F16/F32 -> F32
     return out;
 }
 
+std::vector<float> tensor_f32(const sdh_tensor & t) { return pack_f32(t); }
+
+int ready_on_device(const char * who) {
+    if (!lib().inited) { set_error("sdh_init not called"); return SDH_ERR_NO_DEVICE; }
+    int dev = -1;
+    SDH_HIP_CHECK(hipGetDevice(&dev));
+    if (dev != lib().device) { set_error("%s: the current device is %d, the library is bound to %d", who, dev, lib().device); return SDH_ERR_INVALID; }
+    return SDH_OK;
+}
+
 static std::vector<int32_t> pack_i32(const sdh_tensor & t) {   // I16/I32 -> I32
     const int64_t n0 = t.ne[0], n1 = t.ne[1];
     std::vector<int32_t> out((size_t) (n0 * n1));

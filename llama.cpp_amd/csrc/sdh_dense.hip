@@ -1,0 +1,182 @@
+// sdh_dense.hip — dense Q8_0 weight x 8-bit activations: y[t][o] = sum_b dw[o][b] dx[t][b] sum_{k in b} qw[o][k] qx[t][k].
+//
+// The integer sum of a block of 32 is exact (at most 32 * 127 * 128 < 2^20); the two scales multiply it once in F32 and the
+// blocks are summed in F32.
+//
+//   dense_few_kernel   few tokens: bound by the stream of the weight. A wave owns R rows, a lane a block of 32 per step (two
+//                      16-byte loads per row), v_dot4_i32_i8, the tokens' blocks from the cache; no LDS, no barrier.
+//   dense_tile_kernel  many tokens: v_mfma_i32_32x32x32_i8, whose K is exactly one block.
+#include "sdh_internal.h"
+
+#include <hip/hip_fp16.h>
+
+namespace sdh {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v16i __attribute__((ext_vector_type(16)));
+
+struct DenseArgs {
+    const int8_t * wq; const __half * wd;      // [n_out][n_in], [n_out][nblk]
+    const int8_t * xq; int64_t ldq;
+    const float * xd; int64_t ldd;
+    int n_out, nblk;                           // n_in = 32 * nblk
+    int64_t T;
+    float * y; int64_t ldy;
+};
+
+template <int TT, int R>
+__global__ __launch_bounds__(256) void dense_few_kernel(const DenseArgs a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int o0 = ((int) blockIdx.x * 4 + wave) * R;
+    const int64_t t0 = (int64_t) blockIdx.y * TT;
+    if (o0 >= a.n_out) return;
+    const int64_t n_in = (int64_t) a.nblk * 32;
+    float acc[TT][R];
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[t][r] = 0.0f;
+    int64_t row[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) row[r] = o0 + r < a.n_out ? o0 + r : a.n_out - 1;        // rows past the end: the last one, not stored
+    for (int b = lane; b < a.nblk; b += 64) {
+        v4i w[R][2];
+        float dw[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const v4i * p = reinterpret_cast<const v4i *>(a.wq + row[r] * n_in + (int64_t) b * 32);
+            w[r][0] = __builtin_nontemporal_load(p);
+            w[r][1] = __builtin_nontemporal_load(p + 1);
+            dw[r] = __half2float(a.wd[row[r] * a.nblk + b]);
+        }
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            const int64_t tt = t0 + t < a.T ? t0 + t : a.T - 1;
+            const v4i * p = reinterpret_cast<const v4i *>(a.xq + tt * a.ldq + (int64_t) b * 32);
+            const v4i x0 = p[0], x1 = p[1];
+            const float dx = a.xd[tt * a.ldd + b];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                int s = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s = __builtin_amdgcn_sdot4(w[r][0][k], x0[k], s, false);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s = __builtin_amdgcn_sdot4(w[r][1][k], x1[k], s, false);
+                acc[t][r] = fmaf((float) s, dw[r] * dx, acc[t][r]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float v = acc[t][r];
+            for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m, 64);
+            if (lane == 0 && t0 + t < a.T && o0 + r < a.n_out) a.y[(t0 + t) * a.ldy + o0 + r] = v;
+        }
+}
+
+// 32 tokens x 32 rows per workgroup, K split over its four waves, joined in LDS. Fragments straight from memory: lane = row (or
+// token) lane & 31, the 16 bytes of half lane >> 5 of the block; the result has token 8 (i / 4) + 4 (lane >> 5) + i % 4 in
+// register i and row lane & 31. The tokens' scales go through LDS once per four blocks.
+__global__ __launch_bounds__(256) void dense_tile_kernel(const DenseArgs a) {
+    __shared__ __align__(16) float dxs[4][4][32];
+    __shared__ float part[4][32][33];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int m = lane & 31, h = lane >> 5;
+    const int o = (int) blockIdx.x * 32 + m;
+    const int64_t t0 = (int64_t) blockIdx.y * 32;
+    const int64_t n_in = (int64_t) a.nblk * 32;
+    const int64_t orow = o < a.n_out ? o : a.n_out - 1, trow = t0 + m < a.T ? t0 + m : a.T - 1;
+    const int8_t * wp = a.wq + orow * n_in + 16 * h;
+    const int8_t * xp = a.xq + trow * a.ldq + 16 * h;
+    const __half * dwp = a.wd + orow * a.nblk;
+    const float * dxp = a.xd + trow * a.ldd;
+    float acc[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+    for (int b0 = wave * 4; b0 < a.nblk; b0 += 16) {
+        v4i wf[4], xf[4];
+        float dw[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int b = b0 + k < a.nblk ? b0 + k : a.nblk - 1;
+            wf[k] = *reinterpret_cast<const v4i *>(wp + (int64_t) b * 32);
+            xf[k] = *reinterpret_cast<const v4i *>(xp + (int64_t) b * 32);
+            dw[k] = b0 + k < a.nblk ? __half2float(dwp[b]) : 0.0f;
+        }
+#pragma unroll
+        for (int k = 2 * h; k < 2 * h + 2; ++k) dxs[wave][k][m] = b0 + k < a.nblk ? dxp[b0 + k] : 0.0f;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // this wave's own rows of dxs only
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v16i z = {};
+            z = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf[k], wf[k], z, 0, 0, 0);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 dx = *reinterpret_cast<const float4 *>(&dxs[wave][k][8 * g + 4 * h]);
+                acc[4 * g + 0] = fmaf((float) z[4 * g + 0], dx.x * dw[k], acc[4 * g + 0]);
+                acc[4 * g + 1] = fmaf((float) z[4 * g + 1], dx.y * dw[k], acc[4 * g + 1]);
+                acc[4 * g + 2] = fmaf((float) z[4 * g + 2], dx.z * dw[k], acc[4 * g + 2]);
+                acc[4 * g + 3] = fmaf((float) z[4 * g + 3], dx.w * dw[k], acc[4 * g + 3]);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) part[wave][8 * (i / 4) + 4 * h + (i & 3)][m] = acc[i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 1024; e += 256) {
+        const int t = e >> 5, c = e & 31;
+        if (t0 + t < a.T && (int) blockIdx.x * 32 + c < a.n_out)
+            a.y[(t0 + t) * a.ldy + (int) blockIdx.x * 32 + c] = (part[0][t][c] + part[1][t][c]) + (part[2][t][c] + part[3][t][c]);
+    }
+}
+
+template <int TT, int R>
+static void launch_few(const DenseArgs & a, hipStream_t s) {
+    hipLaunchKernelGGL((dense_few_kernel<TT, R>), dim3((unsigned) ((a.n_out + 4 * R - 1) / (4 * R)), (unsigned) ((a.T + TT - 1) / TT)), dim3(256), 0, s, a);
+}
+
+static int launch_dense(const DenseArgs & a, hipStream_t s) {
+    if (a.T == 1) launch_few<1, 4>(a, s);
+    else if (a.T == 2) launch_few<2, 4>(a, s);
+    else if (a.T <= 8) launch_few<4, 2>(a, s);
+    else {
+        constexpr int64_t CHUNK = 65535ll * 32;             // the grid's second dimension
+        for (int64_t t0 = 0; t0 < a.T; t0 += CHUNK) {
+            DenseArgs c = a;
+            c.T = a.T - t0 < CHUNK ? a.T - t0 : CHUNK;
+            c.xq += t0 * a.ldq; c.xd += t0 * a.ldd; c.y += t0 * a.ldy;
+            hipLaunchKernelGGL(dense_tile_kernel, dim3((unsigned) ((a.n_out + 31) / 32), (unsigned) ((c.T + 31) / 32)), dim3(256), 0, s, c);
+        }
+    }
+    SDH_HIP_CHECK(hipGetLastError());
+    return SDH_OK;
+}
+
+} // namespace sdh
+
+using namespace sdh;
+
+static int sdh_dense_forward_q8_impl(const sdh_dense * W, const sdh_q8 * x, int64_t T, float * y, int64_t ldy, void * stream) {
+    static const char * who = "sdh_dense_forward_q8";
+    if (T == 0) return ready_on_device(who);
+    if (!W || !x || !x->q || !x->d || !y) { set_error("%s: null argument", who); return SDH_ERR_INVALID; }
+    const DenseQ8 w = dense_q8(W);
+    if (w.type != SDH_TYPE_Q8_0) { set_error("%s: the weight is not Q8_0 (type %d)", who, w.type); return SDH_ERR_UNSUPPORTED; }
+    if (T < 0 || ldy < w.n_out || x->ldq < w.n_in || x->ldd < w.n_in / 32) {
+        set_error("%s: bad shape: T=%lld ldq=%lld ldd=%lld (n_in=%lld) ldy=%lld (n_out=%lld)", who, (long long) T, (long long) x->ldq, (long long) x->ldd, (long long) w.n_in, (long long) ldy, (long long) w.n_out);
+        return SDH_ERR_INVALID;
+    }
+    if (!aligned(x->q, 16) || x->ldq % 16 || !aligned(x->d, 4) || !aligned(y, 4)) { set_error("%s: x->q needs 16-byte aligned rows, x->d and y 4-byte ones", who); return SDH_ERR_INVALID; }
+    const int rc = ready_on_device(who);
+    if (rc != SDH_OK) return rc;
+    const DenseArgs a{w.q, (const __half *) w.d, x->q, x->ldq, x->d, x->ldd, (int) w.n_out, (int) (w.n_in / 32), T, y, ldy};
+    return launch_dense(a, (hipStream_t) stream);
+}
+
+extern "C" int sdh_dense_forward_q8(const sdh_dense * W, const sdh_q8 * x, int64_t n_tokens, float * y, int64_t ldy, void * stream) {
+    SDH_NO_THROW(sdh_dense_forward_q8_impl(W, x, n_tokens, y, ldy, stream));
+}

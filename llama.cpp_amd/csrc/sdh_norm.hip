@@ -1,0 +1,220 @@
+// sdh_norm.hip — residual addition + root-mean-square norm + weight, outputs in F32 and / or 8 bits with scales, and the
+// 8-bit conversion alone. Per token
+//   s = x + res,  z = s * w / sqrt(mean(s^2) + eps),  per 32 values d = max|z| / 127, q = rint(z / d).
+//
+// One workgroup per token, the row in registers between the sum of squares and the outputs: every input is read once. A lane
+// holds 4 consecutive values per step, so eight neighbouring lanes hold a block of 32 and its maximum is three lane exchanges.
+//
+// Arithmetic: s is rounded to F32 (the next layer reads it); from there on everything is in double and rounded once per output.
+// gfx950 issues double multiplies and adds at the F32 rate, the kernel waits for memory, and q then does not depend on how the
+// sum of squares was split (in F32 about one value in 40,000 lands on the other side of a rounding border).
+#include "sdh_internal.h"
+
+namespace sdh {
+
+struct NormArgs {
+    const float * x; int64_t ldx;
+    const float * res; int64_t ldr;      // or null
+    const float * w;                     // or null
+    double eps;
+    int n;
+    float * sum; int64_t lds;            // or null
+    float * y; int64_t ldy;              // or null
+    int8_t * q; int64_t ldq;             // or null
+    float * d; int64_t ldd;
+};
+
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const float * p, int i, int n) {
+    if constexpr (VEC) return *reinterpret_cast<const float4 *>(p + i);
+    float4 v;
+    v.x = p[i];
+    v.y = i + 1 < n ? p[i + 1] : 0.0f; v.z = i + 2 < n ? p[i + 2] : 0.0f; v.w = i + 3 < n ? p[i + 3] : 0.0f;
+    return v;
+}
+template <bool VEC>
+__device__ __forceinline__ void store4(float * p, int i, int n, float4 v) {
+    if constexpr (VEC) { *reinterpret_cast<float4 *>(p + i) = v; return; }
+    p[i] = v.x;
+    if (i + 1 < n) p[i + 1] = v.y;
+    if (i + 2 < n) p[i + 2] = v.z;
+    if (i + 3 < n) p[i + 3] = v.w;
+}
+
+// magnitude bits of a double: ordered as unsigned integers, every NaN above infinity, so a maximum keeps a NaN
+__device__ __forceinline__ unsigned long long mag(double z) { return (unsigned long long) __double_as_longlong(z) & 0x7fffffffffffffffull; }
+__device__ __forceinline__ unsigned long long umax64(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
+
+__device__ __forceinline__ double block_sum(double v, double * red) {
+    for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m, 64);
+    const int nw = (int) blockDim.x >> 6;
+    if (nw == 1) return v;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double t = 0.0;
+    for (int i = 0; i < nw; ++i) t += red[i];
+    return t;
+}
+
+// outputs of four consecutive values i .. i + 3 of one row; live: i < n. All lanes of the wave come here (lane exchanges).
+template <bool VEC, bool NORM>
+__device__ __forceinline__ void emit4(const NormArgs & a, int64_t t, int i, bool live, float4 s, double r) {
+    double z[4] = {(double) s.x, (double) s.y, (double) s.z, (double) s.w};
+    if constexpr (NORM) {
+        float4 w = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+        if (a.w && live) w = load4<VEC>(a.w, i, a.n);
+        z[0] = z[0] * r * (double) w.x; z[1] = z[1] * r * (double) w.y; z[2] = z[2] * r * (double) w.z; z[3] = z[3] * r * (double) w.w;
+        if (a.y && live) store4<VEC>(a.y + t * a.ldy, i, a.n, make_float4((float) z[0], (float) z[1], (float) z[2], (float) z[3]));
+    }
+    if (a.q) {                                              // n % 32 == 0: the eight lanes of a block are live together
+        unsigned long long m = live ? umax64(umax64(mag(z[0]), mag(z[1])), umax64(mag(z[2]), mag(z[3]))) : 0;
+        m = umax64(m, __shfl_xor(m, 1, 64)); m = umax64(m, __shfl_xor(m, 2, 64)); m = umax64(m, __shfl_xor(m, 4, 64));
+        const double amax = __longlong_as_double((long long) m);
+        const float d = (float) (amax / 127.0);
+        const bool fine = d > 0.0f && m < 0x7ff0000000000000ull;     // zeros, and blocks that are not finite: quants of 0
+        const double inv = fine ? 127.0 / amax : 0.0;
+        unsigned b = 0;
+        if (fine)
+            for (int k = 0; k < 4; ++k) b |= ((unsigned) (int) rint(z[k] * inv) & 0xffu) << (8 * k);
+        if (live) {
+            *reinterpret_cast<unsigned *>(a.q + t * a.ldq + i) = b;
+            if ((i & 31) == 0) a.d[t * a.ldd + (i >> 5)] = d;
+        }
+    }
+}
+
+// NV: steps of 4 values per thread, n <= 4 * NV * blockDim.x
+template <int NV, bool VEC, bool NORM>
+__global__ __launch_bounds__(1024) void norm_rows_kernel(const NormArgs a) {
+    __shared__ double red[16];
+    const int64_t t = blockIdx.x;
+    const float * x = a.x + t * a.ldx;
+    float4 s[NV];
+    double ss = 0.0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const int i = 4 * ((int) threadIdx.x + v * (int) blockDim.x);
+        s[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (i < a.n) {
+            s[v] = load4<VEC>(x, i, a.n);
+            if (NORM && a.res) { const float4 r = load4<VEC>(a.res + t * a.ldr, i, a.n); s[v].x += r.x; s[v].y += r.y; s[v].z += r.z; s[v].w += r.w; }
+        }
+    }
+    double r = 1.0;
+    if constexpr (NORM) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int i = 4 * ((int) threadIdx.x + v * (int) blockDim.x);
+            ss += (double) s[v].x * s[v].x + (double) s[v].y * s[v].y + ((double) s[v].z * s[v].z + (double) s[v].w * s[v].w);
+            if (a.sum && i < a.n) store4<VEC>(a.sum + t * a.lds, i, a.n, s[v]);
+        }
+        r = 1.0 / sqrt(block_sum(ss, red) / a.n + a.eps);
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const int i = 4 * ((int) threadIdx.x + v * (int) blockDim.x);
+        emit4<VEC, NORM>(a, t, i, i < a.n, s[v], r);
+    }
+}
+
+// rows that do not fit the registers of a workgroup: two passes; the second reads s where the first one stored it
+template <bool VEC, bool NORM>
+__global__ __launch_bounds__(1024) void norm_long_kernel(const NormArgs a) {
+    __shared__ double red[16];
+    const int64_t t = blockIdx.x;
+    const float * x = a.x + t * a.ldx;
+    double ss = 0.0, r = 1.0;
+    const int end = (a.n + 4095) / 4096 * 4096;             // every lane takes part in the exchanges of the last step
+    if constexpr (NORM) {
+        for (int i = 4 * (int) threadIdx.x; i < a.n; i += 4096) {
+            float4 s = load4<VEC>(x, i, a.n);
+            if (a.res) { const float4 q = load4<VEC>(a.res + t * a.ldr, i, a.n); s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w; }
+            ss += (double) s.x * s.x + (double) s.y * s.y + ((double) s.z * s.z + (double) s.w * s.w);
+            if (a.sum) store4<VEC>(a.sum + t * a.lds, i, a.n, s);
+        }
+        r = 1.0 / sqrt(block_sum(ss, red) / a.n + a.eps);
+    }
+    for (int i = 4 * (int) threadIdx.x; i < end; i += 4096) {
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (i < a.n) {
+            if (NORM && a.sum) s = load4<VEC>(a.sum + t * a.lds, i, a.n);      // this thread's own stores
+            else {
+                s = load4<VEC>(x, i, a.n);
+                if (NORM && a.res) { const float4 q = load4<VEC>(a.res + t * a.ldr, i, a.n); s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w; }
+            }
+        }
+        emit4<VEC, NORM>(a, t, i, i < a.n, s, r);
+    }
+}
+
+template <bool VEC, bool NORM>
+static void launch_norm_v(const NormArgs & a, int64_t T, hipStream_t s) {
+    const dim3 grid((unsigned) T);
+    const int q4 = (a.n + 3) / 4;
+    auto threads = [&](int nv) { return dim3((unsigned) (((q4 + nv - 1) / nv + 63) / 64 * 64)); };
+    if (q4 <= 1024) hipLaunchKernelGGL((norm_rows_kernel<1, VEC, NORM>), grid, threads(1), 0, s, a);
+    else if (q4 <= 2048) hipLaunchKernelGGL((norm_rows_kernel<2, VEC, NORM>), grid, threads(2), 0, s, a);
+    else if (q4 <= 4096) hipLaunchKernelGGL((norm_rows_kernel<4, VEC, NORM>), grid, threads(4), 0, s, a);
+    else hipLaunchKernelGGL((norm_long_kernel<VEC, NORM>), grid, dim3(1024), 0, s, a);
+}
+
+template <bool NORM>
+static int launch_norm(const NormArgs & a, int64_t T, hipStream_t s) {
+    // 16-byte accesses where every row of every tensor starts on 16 bytes and the row length is a multiple of 4
+    auto ok = [](const float * p, int64_t ld) { return !p || (aligned(p, 16) && ld % 4 == 0); };
+    const bool vec = a.n % 4 == 0 && ok(a.x, a.ldx) && ok(a.res, a.ldr) && ok(a.sum, a.lds) && ok(a.y, a.ldy) && ok(a.w, 0);
+    if (vec) launch_norm_v<true, NORM>(a, T, s); else launch_norm_v<false, NORM>(a, T, s);
+    SDH_HIP_CHECK(hipGetLastError());
+    return SDH_OK;
+}
+
+static int check_q8(const char * who, const sdh_q8 * o, int64_t n) {
+    if (!o->q || !o->d) { set_error("%s: null plane of the 8-bit output", who); return SDH_ERR_INVALID; }
+    if (n % 32) { set_error("%s: 8-bit outputs need n %% 32 == 0 (n=%lld)", who, (long long) n); return SDH_ERR_INVALID; }
+    if (o->ldq < n || o->ldd < n / 32) { set_error("%s: ldq=%lld ldd=%lld are too short for n=%lld", who, (long long) o->ldq, (long long) o->ldd, (long long) n); return SDH_ERR_INVALID; }
+    if (!aligned(o->q, 4) || o->ldq % 4 || !aligned(o->d, 4)) { set_error("%s: the 8-bit plane needs 4-byte aligned rows", who); return SDH_ERR_INVALID; }
+    return SDH_OK;
+}
+
+} // namespace sdh
+
+using namespace sdh;
+
+static int sdh_rms_norm_impl(const float * x, int64_t ldx, const float * res, int64_t ldr, const float * weight, float eps,
+                             int64_t n, int64_t T, float * sum, int64_t lds, float * y, int64_t ldy, const sdh_q8 * o8, void * stream) {
+    static const char * who = "sdh_rms_norm";
+    if (T == 0) return ready_on_device(who);
+    int rc;
+    if (!x || (!sum && !y && !o8)) { set_error("%s: null argument (x, or every output)", who); return SDH_ERR_INVALID; }
+    if (n < 1 || n > INT32_MAX / 2 || T < 0 || T > INT32_MAX || !(eps >= 0.0f)) { set_error("%s: bad shape or eps: n=%lld T=%lld eps=%g", who, (long long) n, (long long) T, (double) eps); return SDH_ERR_INVALID; }
+    if (ldx < n || (res && ldr < n) || (sum && lds < n) || (y && ldy < n)) { set_error("%s: a row stride is shorter than n=%lld", who, (long long) n); return SDH_ERR_INVALID; }
+    if (!aligned(x, 4) || !aligned(res, 4) || !aligned(weight, 4) || !aligned(sum, 4) || !aligned(y, 4)) { set_error("%s: a pointer is not 4-byte aligned", who); return SDH_ERR_INVALID; }
+    if (o8 && (rc = check_q8(who, o8, n)) != SDH_OK) return rc;
+    auto in_place = [&](const float * o, int64_t ldo) { return !o || ((o != x || ldo == ldx) && (o != res || ldo == ldr)); };
+    if (!in_place(sum, lds) || !in_place(y, ldy) || (y && y == sum)) { set_error("%s: outputs overlap (sum or y may be x or res with the same stride, and not each other)", who); return SDH_ERR_INVALID; }
+    if ((rc = ready_on_device(who)) != SDH_OK) return rc;
+    NormArgs a{x, ldx, res, ldr, weight, (double) eps, (int) n, sum, lds, y, ldy, nullptr, 0, nullptr, 0};
+    if (o8) { a.q = o8->q; a.ldq = o8->ldq; a.d = o8->d; a.ldd = o8->ldd; }
+    return launch_norm<true>(a, T, (hipStream_t) stream);
+}
+
+static int sdh_q8_quantize_impl(const float * x, int64_t ldx, int64_t n, int64_t T, const sdh_q8 * o8, void * stream) {
+    static const char * who = "sdh_q8_quantize";
+    if (T == 0) return ready_on_device(who);
+    int rc;
+    if (!x || !o8) { set_error("%s: null argument", who); return SDH_ERR_INVALID; }
+    if (n < 1 || n > INT32_MAX / 2 || T < 0 || T > INT32_MAX || ldx < n || !aligned(x, 4)) { set_error("%s: bad shape: n=%lld T=%lld ldx=%lld", who, (long long) n, (long long) T, (long long) ldx); return SDH_ERR_INVALID; }
+    if ((rc = check_q8(who, o8, n)) != SDH_OK) return rc;
+    if ((rc = ready_on_device(who)) != SDH_OK) return rc;
+    NormArgs a{x, ldx, nullptr, 0, nullptr, 0.0, (int) n, nullptr, 0, nullptr, 0, o8->q, o8->ldq, o8->d, o8->ldd};
+    return launch_norm<false>(a, T, (hipStream_t) stream);
+}
+
+extern "C" int sdh_rms_norm(const float * x, int64_t ldx, const float * res, int64_t ldr, const float * weight, float eps,
+                            int64_t n, int64_t n_tokens, float * sum, int64_t lds, float * y, int64_t ldy, const sdh_q8 * out8, void * stream) {
+    SDH_NO_THROW(sdh_rms_norm_impl(x, ldx, res, ldr, weight, eps, n, n_tokens, sum, lds, y, ldy, out8, stream));
+}
+
+extern "C" int sdh_q8_quantize(const float * x, int64_t ldx, int64_t n, int64_t n_tokens, const sdh_q8 * out8, void * stream) {
+    SDH_NO_THROW(sdh_q8_quantize_impl(x, ldx, n, n_tokens, out8, stream));
+}

@@ -1439,6 +1439,11 @@ static std::shared_ptr<const FitPlan> plan_fit(std::mt19937 & rng, int64_t n_in,
     });
 }
 
+DenseQ8 dense_q8(const sdh_dense * W) {
+    const DenseView & v = ((const DeviceDense *) W)->v;
+    return DenseQ8{v.q, (const uint16_t *) v.d, v.n_in, v.n_out, v.type};
+}
+
 static DenseView view_or_null(const sdh_dense * d) {
     return d ? ((const DeviceDense *) d)->v : DenseView{};
 }

@@ -38,7 +38,9 @@ ABI_SYMBOLS = [
     "sdh_forward", "sdh_forward_noalloc", "sdh_noalloc_scratch_bytes", "sdh_debug_alloc_calls", "sdh_debug_fold_layout", "sdh_debug_last_decode_kind", "sdh_probe_stream_floor", "sdh_nonfinite_count", "sdh_w0_tile", "sdh_ffn_forward", "sdh_ffn_gate_up", "sdh_ffn_last_fused", "sdh_glu",
     "sdh_ffn_stack_create", "sdh_ffn_stack_destroy", "sdh_ffn_stack_forward", "sdh_ffn_stack_status", "sdh_ffn_stack_payload_bytes",
     "sdh_profile_enable", "sdh_profile_read", "sdh_profile_span_begin", "sdh_profile_span_end",
-    "sdh_dense_create", "sdh_dense_destroy", "sdh_dense_bytes",
+    "sdh_dense_create", "sdh_dense_destroy", "sdh_dense_bytes", "sdh_dense_forward_q8",
+    "sdh_rms_norm", "sdh_q8_quantize",
+    "sdh_lora_create", "sdh_lora_destroy", "sdh_lora_bytes", "sdh_lora_workspace_bytes", "sdh_lora_apply",
     "sdh_scan_create", "sdh_scan_destroy", "sdh_scan_reseed", "sdh_scan_tensor", "sdh_scan_tensor_kgrid", "sdh_scan_pick", "sdh_scan_rewind", "sdh_scan_skip", "sdh_scan_fetch", "sdh_scan_fetch_packed", "sdh_scan_memo_clear", "sdh_imatrix_scale",
 ]
 
@@ -68,6 +70,14 @@ class SdhScanResult(C.Structure):
                 ("em_x", C.c_double * 5), ("cost", C.c_double * 8), ("proxy", C.c_double * 8),
                 ("gpu_ms", C.c_double), ("has_w", C.c_int32), ("reserved", C.c_int32),
                 ("em_w", C.c_double * 5), ("em_x_w", C.c_double * 5), ("delta_clamp_scale", C.c_double)]
+
+
+class SdhQ8(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("ldq", C.c_int64), ("d", C.c_void_p), ("ldd", C.c_int64)]
+
+
+class SdhLoraDesc(C.Structure):
+    _fields_ = [("a", SdhTensor), ("b", SdhTensor), ("scale", C.c_float), ("reserved", C.c_int32)]
 
 
 class SeedDeltaError(RuntimeError):
@@ -155,6 +165,18 @@ def load_library(path: str = LIB_PATH):
     lib.sdh_dense_destroy.restype = None
     lib.sdh_dense_bytes.argtypes = [C.c_void_p]
     lib.sdh_dense_bytes.restype = C.c_int64
+    p, i64 = C.c_void_p, C.c_int64
+    lib.sdh_dense_forward_q8.argtypes = [p, p, i64, p, i64, p]
+    lib.sdh_rms_norm.argtypes = [p, i64, p, i64, p, C.c_float, i64, i64, p, i64, p, i64, p, p]
+    lib.sdh_q8_quantize.argtypes = [p, i64, i64, i64, p, p]
+    lib.sdh_lora_create.argtypes = [i64, i64, C.POINTER(SdhLoraDesc), C.c_int, C.POINTER(p)]
+    lib.sdh_lora_destroy.argtypes = [p]
+    lib.sdh_lora_destroy.restype = None
+    lib.sdh_lora_bytes.argtypes = [p]
+    lib.sdh_lora_bytes.restype = i64
+    lib.sdh_lora_workspace_bytes.argtypes = [p, i64]
+    lib.sdh_lora_workspace_bytes.restype = i64
+    lib.sdh_lora_apply.argtypes = [p, p, p, i64, i64, p, i64, p, i64, p, i64, p]
     lib.sdh_scan_create.argtypes = [C.c_uint32, C.POINTER(C.c_void_p)]
     lib.sdh_scan_reseed.argtypes = [C.c_void_p, C.c_uint32]
     lib.sdh_scan_destroy.argtypes = [C.c_void_p]
