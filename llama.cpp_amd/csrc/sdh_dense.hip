@@ -134,6 +134,128 @@ __global__ __launch_bounds__(256) void dense_tile_kernel(const DenseArgs a) {
     }
 }
 
+// Many tokens: BM tokens x 128 rows per workgroup of four waves, both operands through LDS in steps of four blocks (128 bytes a
+// row), two stages. A wave owns 64 tokens x 16 BM / 32 rows as 32x32 tiles.
+//
+// What bounds it is the vector pipe: a 32x32x32 MFMA takes 32 cycles and leaves 16 integers per lane, each of which costs a
+// conversion, the product of its two scales and a fused multiply-add (48 instructions of 4 cycles, packed F32 being off).
+//   LDS        16-byte chunks of a row at chunk ^ ((row >> 1) & 7): the 16 rows of a fragment read hit all 64 banks once.
+//   scales     [block][row] as F32: a lane reads the four tokens of a register group as one broadcast.
+//   workgroups XCD k (round-robin dispatch) takes the row panels k, k + 8, ... with all their token tiles: a panel of the weight
+//              comes from memory once and stays in that XCD's L2.
+template <int BM>
+__global__ __launch_bounds__(256, 2) void dense_mfma_kernel(const DenseArgs a, int n_tt) {
+    constexpr int BN = 128, NM = 2, NN = BM / 64;                   // 32x32 tiles per wave: tokens, rows
+    constexpr int XL = BM / 32, WL = BN / 32;                       // 16-byte loads per thread and stage
+    __shared__ __align__(16) int8_t xs[2][BM * 128];
+    __shared__ __align__(16) int8_t ws[2][BN * 128];
+    __shared__ __align__(16) float dxs[2][4][BM];
+    __shared__ float dws[2][4][BN];
+    const int id = (int) blockIdx.x, seq = id >> 3;
+    const int o_tile = ((seq / n_tt) * 8 + (id & 7)) * BN;
+    const int64_t t_tile = (int64_t) (seq % n_tt) * BM;
+    if (o_tile >= a.n_out) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 31, h = lane >> 5;
+    const int wt = BM == 128 ? (wave & 1) * 64 : 0, wo = BM == 128 ? (wave >> 1) * 64 : wave * 32;
+    const int64_t n_in = (int64_t) a.nblk * 32;
+    const int lr = tid >> 3, lc = tid & 7;                          // staging: rows lr + 32 i, chunk lc
+    const int8_t * xp[XL], * wp[WL];
+#pragma unroll
+    for (int i = 0; i < XL; ++i) xp[i] = a.xq + min(t_tile + lr + 32 * i, a.T - 1) * a.ldq;
+#pragma unroll
+    for (int i = 0; i < WL; ++i) wp[i] = a.wq + (int64_t) min(o_tile + lr + 32 * i, a.n_out - 1) * n_in;
+    const int sr = tid & 127, sb = (tid >> 7) * 2;                  // scales: row sr, blocks sb, sb + 1
+    const float * dxp = a.xd + min(t_tile + (sr < BM ? sr : 0), a.T - 1) * a.ldd;
+    const __half * dwp = a.wd + (int64_t) min(o_tile + sr, a.n_out - 1) * a.nblk;
+    const int st_off = lr * 128 + ((lc ^ ((lr >> 1) & 7)) << 4);    // rows 32 apart have the same key
+
+    v4i xr[XL], wr[WL];
+    float dxr[2], dwr[2];
+    auto load = [&](int b0) {
+        const int cb = min(b0 + (lc >> 1), a.nblk - 1);             // blocks past the end: the last one, with scales of zero
+        const int64_t off = (int64_t) cb * 32 + (lc & 1) * 16;
+#pragma unroll
+        for (int i = 0; i < XL; ++i) xr[i] = *reinterpret_cast<const v4i *>(xp[i] + off);
+#pragma unroll
+        for (int i = 0; i < WL; ++i) wr[i] = *reinterpret_cast<const v4i *>(wp[i] + off);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int b = min(b0 + sb + k, a.nblk - 1);
+            const bool in = b0 + sb + k < a.nblk;
+            dxr[k] = dxp[b]; dwr[k] = __half2float(dwp[b]);
+            if (!in) { dxr[k] = 0.0f; dwr[k] = 0.0f; }
+        }
+    };
+    auto store = [&](int st) {
+#pragma unroll
+        for (int i = 0; i < XL; ++i) *reinterpret_cast<v4i *>(&xs[st][st_off + i * 4096]) = xr[i];
+#pragma unroll
+        for (int i = 0; i < WL; ++i) *reinterpret_cast<v4i *>(&ws[st][st_off + i * 4096]) = wr[i];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (sr < BM) dxs[st][sb + k][sr] = dxr[k];
+            dws[st][sb + k][sr] = dwr[k];
+        }
+    };
+    float acc[NM][NN][16];
+#pragma unroll
+    for (int i = 0; i < NM; ++i)
+#pragma unroll
+        for (int j = 0; j < NN; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+    load(0);
+    store(0);
+    const int n_step = (a.nblk + 3) / 4, key = (m >> 1) & 7;        // tiles start at multiples of 32 rows: the key is the lane's
+    for (int s = 0; s < n_step; ++s) {
+        __syncthreads();
+        const int st = s & 1;
+        if (s + 1 < n_step) load(4 * (s + 1));
+#pragma unroll 1                                                    // or every MFMA of the step is started first, and registers spill
+        for (int k = 0; k < 4; ++k) {
+            const int ch = ((2 * k + h) ^ key) << 4;
+            v4i xf[NM], wf[NN];
+            float dw[NN];
+#pragma unroll
+            for (int i = 0; i < NM; ++i) xf[i] = *reinterpret_cast<const v4i *>(&xs[st][(wt + 32 * i + m) * 128 + ch]);
+#pragma unroll
+            for (int j = 0; j < NN; ++j) { wf[j] = *reinterpret_cast<const v4i *>(&ws[st][(wo + 32 * j + m) * 128 + ch]); dw[j] = dws[st][k][wo + 32 * j + m]; }
+#pragma unroll
+            for (int i = 0; i < NM; ++i) {
+                v16i z[NN];
+#pragma unroll
+                for (int j = 0; j < NN; ++j) {
+                    v16i zero = {};
+                    z[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf[i], wf[j], zero, 0, 0, 0);
+                }
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const float4 d4 = *reinterpret_cast<const float4 *>(&dxs[st][k][wt + 32 * i + 8 * g + 4 * h]);
+                    const float d[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+                    for (int j = 0; j < NN; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) acc[i][j][4 * g + q] = fmaf((float) z[j][4 * g + q], d[q] * dw[j], acc[i][j][4 * g + q]);
+                }
+            }
+        }
+        if (s + 1 < n_step) store(st ^ 1);
+    }
+#pragma unroll
+    for (int i = 0; i < NM; ++i)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            const int64_t t = t_tile + wt + 32 * i + 8 * (q / 4) + 4 * h + (q & 3);
+            if (t < a.T) {
+#pragma unroll
+                for (int j = 0; j < NN; ++j) {
+                    const int o = o_tile + wo + 32 * j + m;
+                    if (o < a.n_out) a.y[t * a.ldy + o] = acc[i][j][q];
+                }
+            }
+        }
+}
+
 template <int TT, int R>
 static void launch_few(const DenseArgs & a, hipStream_t s) {
     hipLaunchKernelGGL((dense_few_kernel<TT, R>), dim3((unsigned) ((a.n_out + 4 * R - 1) / (4 * R)), (unsigned) ((a.T + TT - 1) / TT)), dim3(256), 0, s, a);
@@ -143,7 +265,10 @@ static int launch_dense(const DenseArgs & a, hipStream_t s) {
     if (a.T == 1) launch_few<1, 4>(a, s);
     else if (a.T == 2) launch_few<2, 4>(a, s);
     else if (a.T <= 8) launch_few<4, 2>(a, s);
-    else {
+    else if (a.T > 64) {
+        const int n_tt = (int) ((a.T + 127) / 128), n_pan = (a.n_out + 127) / 128;
+        hipLaunchKernelGGL((dense_mfma_kernel<128>), dim3((unsigned) ((n_pan + 7) / 8 * 8 * n_tt)), dim3(256), 0, s, a, n_tt);
+    } else {
         constexpr int64_t CHUNK = 65535ll * 32;             // the grid's second dimension
         for (int64_t t0 = 0; t0 < a.T; t0 += CHUNK) {
             DenseArgs c = a;
