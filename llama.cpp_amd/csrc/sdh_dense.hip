@@ -144,9 +144,9 @@ __global__ __launch_bounds__(256) void dense_tile_kernel(const DenseArgs a) {
 //   workgroups XCD k (round-robin dispatch) takes the row panels k, k + 8, ... with all their token tiles: a panel of the weight
 //              comes from memory once and stays in that XCD's L2.
 template <int BM>
-__global__ __launch_bounds__(256, 2) void dense_mfma_kernel(const DenseArgs a, int n_tt) {
-    constexpr int BN = 128, NM = 2, NN = BM / 64;                   // 32x32 tiles per wave: tokens, rows
-    constexpr int XL = BM / 32, WL = BN / 32;                       // 16-byte loads per thread and stage
+__global__ __launch_bounds__(512, 4) void dense_mfma_kernel(const DenseArgs a, int n_tt) {
+    constexpr int BN = 128, NM = 1, NN = BM / 64;                   // 32x32 tiles per wave: tokens, rows
+    constexpr int XL = BM / 64, WL = BN / 64;                       // 16-byte loads per thread and stage
     __shared__ __align__(16) int8_t xs[2][BM * 128];
     __shared__ __align__(16) int8_t ws[2][BN * 128];
     __shared__ __align__(16) float dxs[2][4][BM];
@@ -156,21 +156,21 @@ __global__ __launch_bounds__(256, 2) void dense_mfma_kernel(const DenseArgs a, i
     const int64_t t_tile = (int64_t) (seq % n_tt) * BM;
     if (o_tile >= a.n_out) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 31, h = lane >> 5;
-    const int wt = BM == 128 ? (wave & 1) * 64 : 0, wo = BM == 128 ? (wave >> 1) * 64 : wave * 32;
+    const int wt = (wave % (BM / 32)) * 32, wo = (wave / (BM / 32)) * 32 * NN;
     const int64_t n_in = (int64_t) a.nblk * 32;
-    const int lr = tid >> 3, lc = tid & 7;                          // staging: rows lr + 32 i, chunk lc
+    const int lr = tid >> 3, lc = tid & 7;                          // staging: rows lr + 64 i, chunk lc
     const int8_t * xp[XL], * wp[WL];
 #pragma unroll
-    for (int i = 0; i < XL; ++i) xp[i] = a.xq + min(t_tile + lr + 32 * i, a.T - 1) * a.ldq;
+    for (int i = 0; i < XL; ++i) xp[i] = a.xq + min(t_tile + lr + 64 * i, a.T - 1) * a.ldq;
 #pragma unroll
-    for (int i = 0; i < WL; ++i) wp[i] = a.wq + (int64_t) min(o_tile + lr + 32 * i, a.n_out - 1) * n_in;
-    const int sr = tid & 127, sb = (tid >> 7) * 2;                  // scales: row sr, blocks sb, sb + 1
+    for (int i = 0; i < WL; ++i) wp[i] = a.wq + (int64_t) min(o_tile + lr + 64 * i, a.n_out - 1) * n_in;
+    const int sr = tid & 127, sb = tid >> 7;                        // scales: row sr, block sb
     const float * dxp = a.xd + min(t_tile + (sr < BM ? sr : 0), a.T - 1) * a.ldd;
     const __half * dwp = a.wd + (int64_t) min(o_tile + sr, a.n_out - 1) * a.nblk;
-    const int st_off = lr * 128 + ((lc ^ ((lr >> 1) & 7)) << 4);    // rows 32 apart have the same key
+    const int st_off = lr * 128 + ((lc ^ ((lr >> 1) & 7)) << 4);    // rows 64 apart have the same key
 
     v4i xr[XL], wr[WL];
-    float dxr[2], dwr[2];
+    float dxr, dwr;
     auto load = [&](int b0) {
         const int cb = min(b0 + (lc >> 1), a.nblk - 1);             // blocks past the end: the last one, with scales of zero
         const int64_t off = (int64_t) cb * 32 + (lc & 1) * 16;
@@ -178,24 +178,17 @@ __global__ __launch_bounds__(256, 2) void dense_mfma_kernel(const DenseArgs a, i
         for (int i = 0; i < XL; ++i) xr[i] = *reinterpret_cast<const v4i *>(xp[i] + off);
 #pragma unroll
         for (int i = 0; i < WL; ++i) wr[i] = *reinterpret_cast<const v4i *>(wp[i] + off);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int b = min(b0 + sb + k, a.nblk - 1);
-            const bool in = b0 + sb + k < a.nblk;
-            dxr[k] = dxp[b]; dwr[k] = __half2float(dwp[b]);
-            if (!in) { dxr[k] = 0.0f; dwr[k] = 0.0f; }
-        }
+        const int b = min(b0 + sb, a.nblk - 1);
+        dxr = dxp[b]; dwr = __half2float(dwp[b]);
+        if (b0 + sb >= a.nblk) { dxr = 0.0f; dwr = 0.0f; }
     };
     auto store = [&](int st) {
 #pragma unroll
-        for (int i = 0; i < XL; ++i) *reinterpret_cast<v4i *>(&xs[st][st_off + i * 4096]) = xr[i];
+        for (int i = 0; i < XL; ++i) *reinterpret_cast<v4i *>(&xs[st][st_off + i * 8192]) = xr[i];
 #pragma unroll
-        for (int i = 0; i < WL; ++i) *reinterpret_cast<v4i *>(&ws[st][st_off + i * 4096]) = wr[i];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if (sr < BM) dxs[st][sb + k][sr] = dxr[k];
-            dws[st][sb + k][sr] = dwr[k];
-        }
+        for (int i = 0; i < WL; ++i) *reinterpret_cast<v4i *>(&ws[st][st_off + i * 8192]) = wr[i];
+        if (sr < BM) dxs[st][sb][sr] = dxr;
+        dws[st][sb][sr] = dwr;
     };
     float acc[NM][NN][16];
 #pragma unroll
@@ -267,7 +260,7 @@ static int launch_dense(const DenseArgs & a, hipStream_t s) {
     else if (a.T <= 8) launch_few<4, 2>(a, s);
     else if (a.T > 64) {
         const int n_tt = (int) ((a.T + 127) / 128), n_pan = (a.n_out + 127) / 128;
-        hipLaunchKernelGGL((dense_mfma_kernel<128>), dim3((unsigned) ((n_pan + 7) / 8 * 8 * n_tt)), dim3(256), 0, s, a, n_tt);
+        hipLaunchKernelGGL((dense_mfma_kernel<128>), dim3((unsigned) ((n_pan + 7) / 8 * 8 * n_tt)), dim3(512), 0, s, a, n_tt);
     } else {
         constexpr int64_t CHUNK = 65535ll * 32;             // the grid's second dimension
         for (int64_t t0 = 0; t0 < a.T; t0 += CHUNK) {
