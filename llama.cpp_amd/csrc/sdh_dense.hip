@@ -144,13 +144,13 @@ __global__ __launch_bounds__(256) void dense_tile_kernel(const DenseArgs a) {
 //   workgroups XCD k (round-robin dispatch) takes the row panels k, k + 8, ... with all their token tiles: a panel of the weight
 //              comes from memory once and stays in that XCD's L2.
 template <int BM>
-__global__ __launch_bounds__(512, 4) void dense_mfma_kernel(const DenseArgs a, int n_tt) {
-    constexpr int BN = 128, NM = 1, NN = BM / 64;                   // 32x32 tiles per wave: tokens, rows
-    constexpr int XL = BM / 64, WL = BN / 64;                       // 16-byte loads per thread and stage
+__global__ __launch_bounds__(4 * BM, BM == 128 ? 4 : 3) void dense_mfma_kernel(const DenseArgs a, int n_tt) {
+    constexpr int BN = 128, NM = 1, NN = 2;                         // 32x32 tiles per wave: tokens, rows
+    constexpr int NT = 4 * BM, XL = 2, WL = 256 / BM, SL = 512 / NT;                       // 16-byte loads per thread and stage
     __shared__ __align__(16) int8_t xs[2][BM * 128];
     __shared__ __align__(16) int8_t ws[2][BN * 128];
     __shared__ __align__(16) float dxs[2][4][BM];
-    __shared__ float dws[2][4][BN];
+    __shared__ __half dws[2][4][BN];
     const int id = (int) blockIdx.x, seq = id >> 3;
     const int o_tile = ((seq / n_tt) * 8 + (id & 7)) * BN;
     const int64_t t_tile = (int64_t) (seq % n_tt) * BM;
@@ -158,19 +158,20 @@ __global__ __launch_bounds__(512, 4) void dense_mfma_kernel(const DenseArgs a, i
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 31, h = lane >> 5;
     const int wt = (wave % (BM / 32)) * 32, wo = (wave / (BM / 32)) * 32 * NN;
     const int64_t n_in = (int64_t) a.nblk * 32;
-    const int lr = tid >> 3, lc = tid & 7;                          // staging: rows lr + 64 i, chunk lc
+    const int lr = tid >> 3, lc = tid & 7;                          // staging: rows lr + NT / 8 i, chunk lc
     const int8_t * xp[XL], * wp[WL];
 #pragma unroll
-    for (int i = 0; i < XL; ++i) xp[i] = a.xq + min(t_tile + lr + 64 * i, a.T - 1) * a.ldq;
+    for (int i = 0; i < XL; ++i) xp[i] = a.xq + min(t_tile + lr + NT / 8 * i, a.T - 1) * a.ldq;
 #pragma unroll
-    for (int i = 0; i < WL; ++i) wp[i] = a.wq + (int64_t) min(o_tile + lr + 64 * i, a.n_out - 1) * n_in;
-    const int sr = tid & 127, sb = tid >> 7;                        // scales: row sr, block sb
+    for (int i = 0; i < WL; ++i) wp[i] = a.wq + (int64_t) min(o_tile + lr + NT / 8 * i, a.n_out - 1) * n_in;
+    const int sr = tid & 127, sb = (tid >> 7) * SL;                 // scales: row sr, blocks sb .. sb + SL - 1
     const float * dxp = a.xd + min(t_tile + (sr < BM ? sr : 0), a.T - 1) * a.ldd;
     const __half * dwp = a.wd + (int64_t) min(o_tile + sr, a.n_out - 1) * a.nblk;
-    const int st_off = lr * 128 + ((lc ^ ((lr >> 1) & 7)) << 4);    // rows 64 apart have the same key
+    const int st_off = lr * 128 + ((lc ^ ((lr >> 1) & 7)) << 4);    // rows 16 apart have the same key
 
     v4i xr[XL], wr[WL];
-    float dxr, dwr;
+    float dxr[SL];
+    __half dwr[SL];
     auto load = [&](int b0) {
         const int cb = min(b0 + (lc >> 1), a.nblk - 1);             // blocks past the end: the last one, with scales of zero
         const int64_t off = (int64_t) cb * 32 + (lc & 1) * 16;
@@ -178,17 +179,23 @@ __global__ __launch_bounds__(512, 4) void dense_mfma_kernel(const DenseArgs a, i
         for (int i = 0; i < XL; ++i) xr[i] = *reinterpret_cast<const v4i *>(xp[i] + off);
 #pragma unroll
         for (int i = 0; i < WL; ++i) wr[i] = *reinterpret_cast<const v4i *>(wp[i] + off);
-        const int b = min(b0 + sb, a.nblk - 1);
-        dxr = dxp[b]; dwr = __half2float(dwp[b]);
-        if (b0 + sb >= a.nblk) { dxr = 0.0f; dwr = 0.0f; }
+#pragma unroll
+        for (int k = 0; k < SL; ++k) {
+            const int b = min(b0 + sb + k, a.nblk - 1);
+            dxr[k] = dxp[b]; dwr[k] = dwp[b];
+            if (b0 + sb + k >= a.nblk) { dxr[k] = 0.0f; dwr[k] = __half(0.0f); }
+        }
     };
     auto store = [&](int st) {
 #pragma unroll
-        for (int i = 0; i < XL; ++i) *reinterpret_cast<v4i *>(&xs[st][st_off + i * 8192]) = xr[i];
+        for (int i = 0; i < XL; ++i) *reinterpret_cast<v4i *>(&xs[st][st_off + i * 16 * NT]) = xr[i];
 #pragma unroll
-        for (int i = 0; i < WL; ++i) *reinterpret_cast<v4i *>(&ws[st][st_off + i * 8192]) = wr[i];
-        if (sr < BM) dxs[st][sb][sr] = dxr;
-        dws[st][sb][sr] = dwr;
+        for (int i = 0; i < WL; ++i) *reinterpret_cast<v4i *>(&ws[st][st_off + i * 16 * NT]) = wr[i];
+#pragma unroll
+        for (int k = 0; k < SL; ++k) {
+            if (sr < BM) dxs[st][sb + k][sr] = dxr[k];
+            dws[st][sb + k][sr] = dwr[k];
+        }
     };
     float acc[NM][NN][16];
 #pragma unroll
@@ -212,7 +219,7 @@ __global__ __launch_bounds__(512, 4) void dense_mfma_kernel(const DenseArgs a, i
 #pragma unroll
             for (int i = 0; i < NM; ++i) xf[i] = *reinterpret_cast<const v4i *>(&xs[st][(wt + 32 * i + m) * 128 + ch]);
 #pragma unroll
-            for (int j = 0; j < NN; ++j) { wf[j] = *reinterpret_cast<const v4i *>(&ws[st][(wo + 32 * j + m) * 128 + ch]); dw[j] = dws[st][k][wo + 32 * j + m]; }
+            for (int j = 0; j < NN; ++j) { wf[j] = *reinterpret_cast<const v4i *>(&ws[st][(wo + 32 * j + m) * 128 + ch]); dw[j] = __half2float(dws[st][k][wo + 32 * j + m]); }
 #pragma unroll
             for (int i = 0; i < NM; ++i) {
                 v16i z[NN];
@@ -259,8 +266,12 @@ static int launch_dense(const DenseArgs & a, hipStream_t s) {
     else if (a.T == 2) launch_few<2, 4>(a, s);
     else if (a.T <= 8) launch_few<4, 2>(a, s);
     else if (a.T > 64) {
-        const int n_tt = (int) ((a.T + 127) / 128), n_pan = (a.n_out + 127) / 128;
-        hipLaunchKernelGGL((dense_mfma_kernel<128>), dim3((unsigned) ((n_pan + 7) / 8 * 8 * n_tt)), dim3(512), 0, s, a, n_tt);
+        const int64_t n_pan = (a.n_out + 127) / 128;
+        const bool half = n_pan * ((a.T + 127) / 128) < 4 * lib().num_cu;
+        const int n_tt = (int) (half ? (a.T + 63) / 64 : (a.T + 127) / 128);
+        const dim3 grid((unsigned) ((n_pan + 7) / 8 * 8 * n_tt));
+        if (half) hipLaunchKernelGGL((dense_mfma_kernel<64>), grid, dim3(256), 0, s, a, n_tt);
+        else      hipLaunchKernelGGL((dense_mfma_kernel<128>), grid, dim3(512), 0, s, a, n_tt);
     } else {
         constexpr int64_t CHUNK = 65535ll * 32;             // the grid's second dimension
         for (int64_t t0 = 0; t0 < a.T; t0 += CHUNK) {
