@@ -8,6 +8,7 @@
 //   dense_tile_kernel  many tokens: v_mfma_i32_32x32x32_i8, whose K is exactly one block.
 #include "sdh_internal.h"
 
+#include <algorithm>
 #include <hip/hip_fp16.h>
 
 namespace sdh {
@@ -24,45 +25,56 @@ struct DenseArgs {
     float * y; int64_t ldy;
 };
 
-template <int TT, int R>
+// U chunks of 16 bytes (half a block) per lane and row in flight; chunk c of a row belongs to lane c & 63.
+template <int TT, int R, int U>
 __global__ __launch_bounds__(256) void dense_few_kernel(const DenseArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int o0 = ((int) blockIdx.x * 4 + wave) * R;
     const int64_t t0 = (int64_t) blockIdx.y * TT;
     if (o0 >= a.n_out) return;
     const int64_t n_in = (int64_t) a.nblk * 32;
+    const int n_ch = 2 * a.nblk;
     float acc[TT][R];
 #pragma unroll
     for (int t = 0; t < TT; ++t)
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[t][r] = 0.0f;
-    int64_t row[R];
+    const int8_t * wp[R];
+    const __half * dp[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) row[r] = o0 + r < a.n_out ? o0 + r : a.n_out - 1;        // rows past the end: the last one, not stored
-    for (int b = lane; b < a.nblk; b += 64) {
-        v4i w[R][2];
-        float dw[R];
+    for (int r = 0; r < R; ++r) {                             // rows past the end: the last one, not stored
+        const int64_t row = min(o0 + r, a.n_out - 1);
+        wp[r] = a.wq + row * n_in;
+        dp[r] = a.wd + row * a.nblk;
+    }
+    for (int c0 = lane; c0 < n_ch; c0 += 64 * U) {
+        v4i w[U][R];
+        float dw[U][R];
+        int c[U];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const v4i * p = reinterpret_cast<const v4i *>(a.wq + row[r] * n_in + (int64_t) b * 32);
-            w[r][0] = __builtin_nontemporal_load(p);
-            w[r][1] = __builtin_nontemporal_load(p + 1);
-            dw[r] = __half2float(a.wd[row[r] * a.nblk + b]);
+        for (int u = 0; u < U; ++u) {                         // chunks past the end: the last one, with a scale of zero
+            c[u] = min(c0 + 64 * u, n_ch - 1);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                w[u][r] = __builtin_nontemporal_load(reinterpret_cast<const v4i *>(wp[r] + (int64_t) c[u] * 16));
+                dw[u][r] = __half2float(dp[r][c[u] >> 1]);
+            }
         }
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
-            const int64_t tt = t0 + t < a.T ? t0 + t : a.T - 1;
-            const v4i * p = reinterpret_cast<const v4i *>(a.xq + tt * a.ldq + (int64_t) b * 32);
-            const v4i x0 = p[0], x1 = p[1];
-            const float dx = a.xd[tt * a.ldd + b];
+            const int64_t tt = min(t0 + t, a.T - 1);
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                int s = 0;
+            for (int u = 0; u < U; ++u) {
+                const v4i x = *reinterpret_cast<const v4i *>(a.xq + tt * a.ldq + (int64_t) c[u] * 16);
+                const float dx = c0 + 64 * u < n_ch && !(lane & 1) ? a.xd[tt * a.ldd + (c[u] >> 1)] : 0.0f;     // even lanes count
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s = __builtin_amdgcn_sdot4(w[r][0][k], x0[k], s, false);
+                for (int r = 0; r < R; ++r) {
+                    int s = 0;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s = __builtin_amdgcn_sdot4(w[r][1][k], x1[k], s, false);
-                acc[t][r] = fmaf((float) s, dw[r] * dx, acc[t][r]);
+                    for (int k = 0; k < 4; ++k) s = __builtin_amdgcn_sdot4(w[u][r][k], x[k], s, false);
+                    s += __builtin_amdgcn_update_dpp(0, s, 0xB1, 0xF, 0xF, true);      // the neighbour's half of the block
+                    acc[t][r] = fmaf((float) s, dw[u][r] * dx, acc[t][r]);
+                }
             }
         }
     }
@@ -76,61 +88,100 @@ __global__ __launch_bounds__(256) void dense_few_kernel(const DenseArgs a) {
         }
 }
 
-// 32 tokens x 32 rows per workgroup, K split over its four waves, joined in LDS. Fragments straight from memory: lane = row (or
-// token) lane & 31, the 16 bytes of half lane >> 5 of the block; the result has token 8 (i / 4) + 4 (lane >> 5) + i % 4 in
-// register i and row lane & 31. The tokens' scales go through LDS once per four blocks.
-__global__ __launch_bounds__(256) void dense_tile_kernel(const DenseArgs a) {
-    __shared__ __align__(16) float dxs[4][4][32];
-    __shared__ float part[4][32][33];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int m = lane & 31, h = lane >> 5;
+// 32 NT tokens x 32 rows per workgroup: the stream of the weight again. The waves split K in groups of four blocks (128 bytes, a
+// whole line of a row) and are joined in LDS at the end; every fragment goes from memory to registers, the next group's before the
+// present one is multiplied, so that a CU has 64 KB in flight without a barrier anywhere in the loop.
+//   fragments  v_mfma_i32_32x32x32_i8: lane = row (or token) lane & 31, the 16 bytes of half lane >> 5 of the block; the result has
+//              token 8 (i / 4) + 4 (lane >> 5) + i % 4 in register i and row lane & 31.
+//   scales     four of a row as one 8-byte load (whatever its alignment); the tokens' are transposed through LDS (each wave its own
+//              corner; LDS works in order within a wave).
+//   tail       the last group of a row is its last four blocks, with scales of zero for those that an earlier group has taken.
+template <int NT, int NW>
+__global__ __launch_bounds__(64 * NW, NT == 1 ? 4 : 2) void dense_mid_kernel(const DenseArgs a) {
+    __shared__ __align__(16) float dxs[NW][NT][4][32];
+    __shared__ float part[NW][32][33];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 31, h = lane >> 5;
     const int o = (int) blockIdx.x * 32 + m;
-    const int64_t t0 = (int64_t) blockIdx.y * 32;
-    const int64_t n_in = (int64_t) a.nblk * 32;
-    const int64_t orow = o < a.n_out ? o : a.n_out - 1, trow = t0 + m < a.T ? t0 + m : a.T - 1;
-    const int8_t * wp = a.wq + orow * n_in + 16 * h;
-    const int8_t * xp = a.xq + trow * a.ldq + 16 * h;
+    const int64_t t0 = (int64_t) blockIdx.y * (32 * NT), orow = min(o, a.n_out - 1);
+    const int8_t * wp = a.wq + orow * a.nblk * 32 + 16 * h;
     const __half * dwp = a.wd + orow * a.nblk;
-    const float * dxp = a.xd + trow * a.ldd;
-    float acc[16];
+    const int8_t * xp[NT];
+    const float * dxp[NT];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-    for (int b0 = wave * 4; b0 < a.nblk; b0 += 16) {
-        v4i wf[4], xf[4];
-        float dw[4];
+    for (int n = 0; n < NT; ++n) {
+        const int64_t t = min(t0 + 32 * n + m, a.T - 1);
+        xp[n] = a.xq + t * a.ldq + 16 * h;
+        dxp[n] = a.xd + t * a.ldd + 2 * h;
+    }
+    float acc[NT][16];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int b = b0 + k < a.nblk ? b0 + k : a.nblk - 1;
-            wf[k] = *reinterpret_cast<const v4i *>(wp + (int64_t) b * 32);
-            xf[k] = *reinterpret_cast<const v4i *>(xp + (int64_t) b * 32);
-            dw[k] = b0 + k < a.nblk ? __half2float(dwp[b]) : 0.0f;
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[n][i] = 0.0f;
+    v4i wf[4], xf[NT][4];
+    __half dw[4];
+    float dx[NT][2];
+    auto load = [&](int b0) {
+        const int bs = min(b0, a.nblk - 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) wf[k] = *reinterpret_cast<const v4i *>(wp + (int64_t) (bs + k) * 32);
+        __builtin_memcpy(dw, dwp + bs, 8);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) xf[n][k] = *reinterpret_cast<const v4i *>(xp[n] + (int64_t) (bs + k) * 32);
+            __builtin_memcpy(dx[n], dxp[n] + bs, 8);
         }
+    };
+    load(4 * wave);
+    for (int b0 = 4 * wave; b0 < a.nblk; b0 += 4 * NW) {
+        const int bs = min(b0, a.nblk - 4);
+        v4i wc[4], xc[NT][4];
+        float dc[4];
 #pragma unroll
-        for (int k = 2 * h; k < 2 * h + 2; ++k) dxs[wave][k][m] = b0 + k < a.nblk ? dxp[b0 + k] : 0.0f;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // this wave's own rows of dxs only
+        for (int k = 0; k < 4; ++k) { wc[k] = wf[k]; dc[k] = bs + k >= b0 ? __half2float(dw[k]) : 0.0f; }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) xc[n][k] = xf[n][k];
+            dxs[wave][n][2 * h][m] = dx[n][0];
+            dxs[wave][n][2 * h + 1][m] = dx[n][1];
+        }
+        load(b0 + 4 * NW);
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            v16i z = {};
-            z = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf[k], wf[k], z, 0, 0, 0);
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4 dx = *reinterpret_cast<const float4 *>(&dxs[wave][k][8 * g + 4 * h]);
-                acc[4 * g + 0] = fmaf((float) z[4 * g + 0], dx.x * dw[k], acc[4 * g + 0]);
-                acc[4 * g + 1] = fmaf((float) z[4 * g + 1], dx.y * dw[k], acc[4 * g + 1]);
-                acc[4 * g + 2] = fmaf((float) z[4 * g + 2], dx.z * dw[k], acc[4 * g + 2]);
-                acc[4 * g + 3] = fmaf((float) z[4 * g + 3], dx.w * dw[k], acc[4 * g + 3]);
+            for (int n = 0; n < NT; ++n) {
+                v16i z = {};
+                z = __builtin_amdgcn_mfma_i32_32x32x32_i8(xc[n][k], wc[k], z, 0, 0, 0);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float4 d = *reinterpret_cast<const float4 *>(&dxs[wave][n][k][8 * q + 4 * h]);
+                    acc[n][4 * q + 0] = fmaf((float) z[4 * q + 0], d.x * dc[k], acc[n][4 * q + 0]);
+                    acc[n][4 * q + 1] = fmaf((float) z[4 * q + 1], d.y * dc[k], acc[n][4 * q + 1]);
+                    acc[n][4 * q + 2] = fmaf((float) z[4 * q + 2], d.z * dc[k], acc[n][4 * q + 2]);
+                    acc[n][4 * q + 3] = fmaf((float) z[4 * q + 3], d.w * dc[k], acc[n][4 * q + 3]);
+                }
             }
-        }
         __builtin_amdgcn_wave_barrier();
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) part[wave][8 * (i / 4) + 4 * h + (i & 3)][m] = acc[i];
-    __syncthreads();
-    for (int e = threadIdx.x; e < 1024; e += 256) {
-        const int t = e >> 5, c = e & 31;
-        if (t0 + t < a.T && (int) blockIdx.x * 32 + c < a.n_out)
-            a.y[(t0 + t) * a.ldy + (int) blockIdx.x * 32 + c] = (part[0][t][c] + part[1][t][c]) + (part[2][t][c] + part[3][t][c]);
+    for (int n = 0; n < NT; ++n) {
+        if (n) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[wave][8 * (i / 4) + 4 * h + (i & 3)][m] = acc[n][i];
+        __syncthreads();
+        for (int e = threadIdx.x; e < 1024; e += 64 * NW) {
+            const int t = e >> 5, c = e & 31;
+            const int64_t tt = t0 + 32 * n + t;
+            if (tt < a.T && (int) blockIdx.x * 32 + c < a.n_out) {
+                float v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) v += part[w][t][c];
+                a.y[tt * a.ldy + (int) blockIdx.x * 32 + c] = v;
+            }
+        }
     }
 }
 
@@ -143,10 +194,10 @@ __global__ __launch_bounds__(256) void dense_tile_kernel(const DenseArgs a) {
 //   scales     [block][row] as F32: a lane reads the four tokens of a register group as one broadcast.
 //   workgroups XCD k (round-robin dispatch) takes the row panels k, k + 8, ... with all their token tiles: a panel of the weight
 //              comes from memory once and stays in that XCD's L2.
-template <int BM>
-__global__ __launch_bounds__(4 * BM, BM == 128 ? 4 : 3) void dense_mfma_kernel(const DenseArgs a, int n_tt) {
-    constexpr int BN = 128, NM = 1, NN = 2;                         // 32x32 tiles per wave: tokens, rows
-    constexpr int NT = 4 * BM, XL = 2, WL = 256 / BM, SL = 512 / NT;                       // 16-byte loads per thread and stage
+template <int BM, int NN /* 32x32 tiles per wave, along the rows */>
+__global__ __launch_bounds__(8 * BM / NN, NN == 1 ? 4 : BM == 128 ? 4 : 3) void dense_mfma_kernel(const DenseArgs a, int n_tt) {
+    constexpr int BN = 128, NM = 1;
+    constexpr int NT = 8 * BM / NN, XL = NN, WL = 128 * NN / BM, SL = 512 / NT;                      // 16-byte loads per thread and stage
     __shared__ __align__(16) int8_t xs[2][BM * 128];
     __shared__ __align__(16) int8_t ws[2][BN * 128];
     __shared__ __align__(16) float dxs[2][4][BM];
@@ -169,32 +220,32 @@ __global__ __launch_bounds__(4 * BM, BM == 128 ? 4 : 3) void dense_mfma_kernel(c
     const __half * dwp = a.wd + (int64_t) min(o_tile + sr, a.n_out - 1) * a.nblk;
     const int st_off = lr * 128 + ((lc ^ ((lr >> 1) & 7)) << 4);    // rows 16 apart have the same key
 
-    v4i xr[XL], wr[WL];
-    float dxr[SL];
-    __half dwr[SL];
-    auto load = [&](int b0) {
+    // stages asked for ahead of the one in use: with one workgroup per CU a step's arithmetic (0.8 us) does not cover a load
+    constexpr int D = BM == 128 ? 1 : 2;
+    struct Stage { v4i x[XL], w[WL]; float dx[SL]; __half dw[SL]; } pre[D];
+    auto load = [&](int b0, Stage & r) {
         const int cb = min(b0 + (lc >> 1), a.nblk - 1);             // blocks past the end: the last one, with scales of zero
         const int64_t off = (int64_t) cb * 32 + (lc & 1) * 16;
 #pragma unroll
-        for (int i = 0; i < XL; ++i) xr[i] = *reinterpret_cast<const v4i *>(xp[i] + off);
+        for (int i = 0; i < XL; ++i) r.x[i] = *reinterpret_cast<const v4i *>(xp[i] + off);
 #pragma unroll
-        for (int i = 0; i < WL; ++i) wr[i] = *reinterpret_cast<const v4i *>(wp[i] + off);
+        for (int i = 0; i < WL; ++i) r.w[i] = *reinterpret_cast<const v4i *>(wp[i] + off);
 #pragma unroll
         for (int k = 0; k < SL; ++k) {
             const int b = min(b0 + sb + k, a.nblk - 1);
-            dxr[k] = dxp[b]; dwr[k] = dwp[b];
-            if (b0 + sb + k >= a.nblk) { dxr[k] = 0.0f; dwr[k] = __half(0.0f); }
+            r.dx[k] = dxp[b]; r.dw[k] = dwp[b];
+            if (b0 + sb + k >= a.nblk) { r.dx[k] = 0.0f; r.dw[k] = __half(0.0f); }
         }
     };
-    auto store = [&](int st) {
+    auto store = [&](int st, const Stage & r) {
 #pragma unroll
-        for (int i = 0; i < XL; ++i) *reinterpret_cast<v4i *>(&xs[st][st_off + i * 16 * NT]) = xr[i];
+        for (int i = 0; i < XL; ++i) *reinterpret_cast<v4i *>(&xs[st][st_off + i * 16 * NT]) = r.x[i];
 #pragma unroll
-        for (int i = 0; i < WL; ++i) *reinterpret_cast<v4i *>(&ws[st][st_off + i * 16 * NT]) = wr[i];
+        for (int i = 0; i < WL; ++i) *reinterpret_cast<v4i *>(&ws[st][st_off + i * 16 * NT]) = r.w[i];
 #pragma unroll
         for (int k = 0; k < SL; ++k) {
-            if (sr < BM) dxs[st][sb + k][sr] = dxr[k];
-            dws[st][sb + k][sr] = dwr[k];
+            if (sr < BM) dxs[st][sb + k][sr] = r.dx[k];
+            dws[st][sb + k][sr] = r.dw[k];
         }
     };
     float acc[NM][NN][16];
@@ -204,13 +255,19 @@ __global__ __launch_bounds__(4 * BM, BM == 128 ? 4 : 3) void dense_mfma_kernel(c
         for (int j = 0; j < NN; ++j)
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
-    load(0);
-    store(0);
     const int n_step = (a.nblk + 3) / 4, key = (m >> 1) & 7;        // tiles start at multiples of 32 rows: the key is the lane's
-    for (int s = 0; s < n_step; ++s) {
+    load(0, pre[0]);
+    store(0, pre[0]);
+#pragma unroll
+    for (int d = 1; d < D; ++d) load(4 * d, pre[d - 1]);
+    for (int s0 = 0; s0 < n_step; s0 += D)
+#pragma unroll
+    for (int d = 0; d < D; ++d) {                                   // stage s + 1 is in pre[d], stage s + D goes to pre[(d + D - 1) % D]
+        const int s = s0 + d;
+        if (s >= n_step) break;
         __syncthreads();
         const int st = s & 1;
-        if (s + 1 < n_step) load(4 * (s + 1));
+        load(4 * (s + D), pre[(d + D - 1) % D]);                    // past the end: in bounds, with scales of zero, and not stored
 #pragma unroll 1                                                    // or every MFMA of the step is started first, and registers spill
         for (int k = 0; k < 4; ++k) {
             const int ch = ((2 * k + h) ^ key) << 4;
@@ -239,7 +296,7 @@ __global__ __launch_bounds__(4 * BM, BM == 128 ? 4 : 3) void dense_mfma_kernel(c
                 }
             }
         }
-        if (s + 1 < n_step) store(st ^ 1);
+        if (s + 1 < n_step) store(st ^ 1, pre[d]);
     }
 #pragma unroll
     for (int i = 0; i < NM; ++i)
@@ -256,29 +313,33 @@ __global__ __launch_bounds__(4 * BM, BM == 128 ? 4 : 3) void dense_mfma_kernel(c
         }
 }
 
-template <int TT, int R>
+template <int TT, int R, int U>
 static void launch_few(const DenseArgs & a, hipStream_t s) {
-    hipLaunchKernelGGL((dense_few_kernel<TT, R>), dim3((unsigned) ((a.n_out + 4 * R - 1) / (4 * R)), (unsigned) ((a.T + TT - 1) / TT)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((dense_few_kernel<TT, R, U>), dim3((unsigned) ((a.n_out + 4 * R - 1) / (4 * R)), (unsigned) ((a.T + TT - 1) / TT)), dim3(256), 0, s, a);
 }
 
-static int launch_dense(const DenseArgs & a, hipStream_t s) {
-    if (a.T == 1) launch_few<1, 4>(a, s);
-    else if (a.T == 2) launch_few<2, 4>(a, s);
-    else if (a.T <= 8) launch_few<4, 2>(a, s);
-    else if (a.T > 64) {
-        const int64_t n_pan = (a.n_out + 127) / 128;
-        const bool half = n_pan * ((a.T + 127) / 128) < 4 * lib().num_cu;
-        const int n_tt = (int) (half ? (a.T + 63) / 64 : (a.T + 127) / 128);
-        const dim3 grid((unsigned) ((n_pan + 7) / 8 * 8 * n_tt));
-        if (half) hipLaunchKernelGGL((dense_mfma_kernel<64>), grid, dim3(256), 0, s, a, n_tt);
-        else      hipLaunchKernelGGL((dense_mfma_kernel<128>), grid, dim3(512), 0, s, a, n_tt);
-    } else {
-        constexpr int64_t CHUNK = 65535ll * 32;             // the grid's second dimension
-        for (int64_t t0 = 0; t0 < a.T; t0 += CHUNK) {
-            DenseArgs c = a;
-            c.T = a.T - t0 < CHUNK ? a.T - t0 : CHUNK;
-            c.xq += t0 * a.ldq; c.xd += t0 * a.ldd; c.y += t0 * a.ldy;
-            hipLaunchKernelGGL(dense_tile_kernel, dim3((unsigned) ((a.n_out + 31) / 32), (unsigned) ((c.T + 31) / 32)), dim3(256), 0, s, c);
+template <int NT, int NW>
+static void launch_mid(const DenseArgs & a, hipStream_t s) {
+    hipLaunchKernelGGL((dense_mid_kernel<NT, NW>), dim3((unsigned) ((a.n_out + 31) / 32), (unsigned) ((a.T + 32 * NT - 1) / (32 * NT))), dim3(64 * NW), 0, s, a);
+}
+
+static int launch_dense(const DenseArgs & all, hipStream_t s) {
+    // a launch has fewer than 2^32 threads: tokens in chunks for very many of them
+    const int64_t n_pan = (all.n_out + 127) / 128, chunk = std::max<int64_t>(1, std::min<int64_t>(8192, (1 << 22) / n_pan)) * 128;
+    for (int64_t t0 = 0; t0 < all.T; t0 += chunk) {
+        DenseArgs a = all;
+        a.T = std::min(chunk, all.T - t0);
+        a.xq += t0 * a.ldq; a.xd += t0 * a.ldd; a.y += t0 * a.ldy;
+        if (all.T == 1)       { if (a.nblk >= 96) launch_few<1, 2, 4>(a, s); else launch_few<1, 2, 2>(a, s); }
+        else if (all.T == 2 || a.nblk < 4) launch_few<2, 2, 4>(a, s);
+        else if (all.T <= 32) launch_mid<1, 8>(a, s);
+        else if (all.T <= 64) launch_mid<2, 8>(a, s);
+        else {
+            const bool half = n_pan * ((all.T + 127) / 128) < 4 * lib().num_cu;
+            const int n_tt = (int) (half ? (a.T + 63) / 64 : (a.T + 127) / 128);
+            const dim3 grid((unsigned) ((n_pan + 7) / 8 * 8 * n_tt));
+            if (half) hipLaunchKernelGGL((dense_mfma_kernel<64, 1>), grid, dim3(512), 0, s, a, n_tt);
+            else      hipLaunchKernelGGL((dense_mfma_kernel<128, 2>), grid, dim3(512), 0, s, a, n_tt);
         }
     }
     SDH_HIP_CHECK(hipGetLastError());
@@ -295,6 +356,7 @@ static int sdh_dense_forward_q8_impl(const sdh_dense * W, const sdh_q8 * x, int6
     if (!W || !x || !x->q || !x->d || !y) { set_error("%s: null argument", who); return SDH_ERR_INVALID; }
     const DenseQ8 w = dense_q8(W);
     if (w.type != SDH_TYPE_Q8_0) { set_error("%s: the weight is not Q8_0 (type %d)", who, w.type); return SDH_ERR_UNSUPPORTED; }
+    if (w.n_out > (1 << 26)) { set_error("%s: %lld rows, more than a launch has threads for", who, (long long) w.n_out); return SDH_ERR_UNSUPPORTED; }
     if (T < 0 || ldy < w.n_out || x->ldq < w.n_in || x->ldd < w.n_in / 32) {
         set_error("%s: bad shape: T=%lld ldq=%lld ldd=%lld (n_in=%lld) ldy=%lld (n_out=%lld)", who, (long long) T, (long long) x->ldq, (long long) x->ldd, (long long) w.n_in, (long long) ldy, (long long) w.n_out);
         return SDH_ERR_INVALID;
