@@ -3,9 +3,9 @@
 // The integer sum of a block of 32 is exact (at most 32 * 127 * 128 < 2^20); the two scales multiply it once in F32 and the
 // blocks are summed in F32.
 //
-//   dense_few_kernel   few tokens: bound by the stream of the weight. A wave owns R rows, a lane a block of 32 per step (two
-//                      16-byte loads per row), v_dot4_i32_i8, the tokens' blocks from the cache; no LDS, no barrier.
-//   dense_tile_kernel  many tokens: v_mfma_i32_32x32x32_i8, whose K is exactly one block.
+//   dense_few_kernel   one or two tokens: bound by the stream of the weight; v_dot4_i32_i8.
+//   dense_mid_kernel   a batch: 32 x 32 tiles of v_mfma_i32_32x32x32_i8, whose K is exactly one block, straight from memory.
+//   dense_mfma_kernel  a prompt: tiles of 64 x 64 to 128 x 128 through LDS, bound by the vector pipe (the scales).
 #include "sdh_internal.h"
 
 #include <algorithm>
@@ -25,7 +25,11 @@ struct DenseArgs {
     float * y; int64_t ldy;
 };
 
-// U chunks of 16 bytes (half a block) per lane and row in flight; chunk c of a row belongs to lane c & 63.
+// A wave owns R rows; chunk c of 16 bytes (half a block) of a row belongs to lane c & 63, so a load instruction takes 1 KB of
+// consecutive bytes, U of them per row in flight; neighbouring lanes join their halves of a block as integers. The tokens' chunks
+// come from the cache; no LDS, no barrier. One token x 4096 -> 14336: 12.1 us, 5.2 TB/s (58.7 MB, a large copy moves 4.9 TB/s);
+// a block per lane, two loads 32 bytes apart, took 22.8 us, four rows per wave 13.3 to 13.9 us, one row 10.5 us without the
+// exchange of halves against 10.6 for two.
 template <int TT, int R, int U>
 __global__ __launch_bounds__(256) void dense_few_kernel(const DenseArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -88,126 +92,111 @@ __global__ __launch_bounds__(256) void dense_few_kernel(const DenseArgs a) {
         }
 }
 
-// 32 NT tokens x 32 rows per workgroup: the stream of the weight again. The waves split K in groups of four blocks (128 bytes, a
-// whole line of a row) and are joined in LDS at the end; every fragment goes from memory to registers, the next group's before the
-// present one is multiplied, so that a CU has 64 KB in flight without a barrier anywhere in the loop.
+// 32 tokens x 32 rows per workgroup: still the stream of the weight. The waves split K in groups of four blocks (128 bytes, a whole
+// line of a row) and are joined in LDS at the end; every fragment goes from memory to registers, the next group's before the present
+// one is multiplied, so that a CU has 64 KB in flight without a barrier anywhere in the loop.
 //   fragments  v_mfma_i32_32x32x32_i8: lane = row (or token) lane & 31, the 16 bytes of half lane >> 5 of the block; the result has
 //              token 8 (i / 4) + 4 (lane >> 5) + i % 4 in register i and row lane & 31.
-//   scales     four of a row as one 8-byte load (whatever its alignment); the tokens' are transposed through LDS (each wave its own
-//              corner; LDS works in order within a wave).
+//   scales     four of a row as one 8-byte load (whatever its alignment; one by one they took as long as the weight); the tokens' are
+//              transposed through LDS (each wave its own corner; LDS works in order within a wave).
 //   tail       the last group of a row is its last four blocks, with scales of zero for those that an earlier group has taken.
-template <int NT, int NW>
-__global__ __launch_bounds__(64 * NW, NT == 1 ? 4 : 2) void dense_mid_kernel(const DenseArgs a) {
-    __shared__ __align__(16) float dxs[NW][NT][4][32];
+// 11 tokens x 14336 -> 4096: 28 us (2.2 TB/s); 16-row tiles with 8-byte fragments took 43 us, 16 waves 31 us, 64 tokens per workgroup
+// 35 us (60 against 38 us at 64 tokens).
+__global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
+    constexpr int NW = 8;
+    __shared__ __align__(16) float dxs[NW][4][32];
     __shared__ float part[NW][32][33];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 31, h = lane >> 5;
-    const int o = (int) blockIdx.x * 32 + m;
-    const int64_t t0 = (int64_t) blockIdx.y * (32 * NT), orow = min(o, a.n_out - 1);
+    const int o0 = (int) blockIdx.x * 32;
+    const int64_t t0 = (int64_t) blockIdx.y * 32, orow = min(o0 + m, a.n_out - 1), trow = min(t0 + m, a.T - 1);
     const int8_t * wp = a.wq + orow * a.nblk * 32 + 16 * h;
     const __half * dwp = a.wd + orow * a.nblk;
-    const int8_t * xp[NT];
-    const float * dxp[NT];
+    const int8_t * xp = a.xq + trow * a.ldq + 16 * h;
+    const float * dxp = a.xd + trow * a.ldd + 2 * h;
+    float acc[16];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int64_t t = min(t0 + 32 * n + m, a.T - 1);
-        xp[n] = a.xq + t * a.ldq + 16 * h;
-        dxp[n] = a.xd + t * a.ldd + 2 * h;
-    }
-    float acc[NT][16];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[n][i] = 0.0f;
-    v4i wf[4], xf[NT][4];
+    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+    v4i wf[4], xf[4];
     __half dw[4];
-    float dx[NT][2];
+    float dx[2];
     auto load = [&](int b0) {
         const int bs = min(b0, a.nblk - 4);
 #pragma unroll
         for (int k = 0; k < 4; ++k) wf[k] = *reinterpret_cast<const v4i *>(wp + (int64_t) (bs + k) * 32);
         __builtin_memcpy(dw, dwp + bs, 8);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) xf[n][k] = *reinterpret_cast<const v4i *>(xp[n] + (int64_t) (bs + k) * 32);
-            __builtin_memcpy(dx[n], dxp[n] + bs, 8);
-        }
+        for (int k = 0; k < 4; ++k) xf[k] = *reinterpret_cast<const v4i *>(xp + (int64_t) (bs + k) * 32);
+        __builtin_memcpy(dx, dxp + bs, 8);
     };
     load(4 * wave);
     for (int b0 = 4 * wave; b0 < a.nblk; b0 += 4 * NW) {
         const int bs = min(b0, a.nblk - 4);
-        v4i wc[4], xc[NT][4];
+        v4i wc[4], xc[4];
         float dc[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { wc[k] = wf[k]; dc[k] = bs + k >= b0 ? __half2float(dw[k]) : 0.0f; }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) xc[n][k] = xf[n][k];
-            dxs[wave][n][2 * h][m] = dx[n][0];
-            dxs[wave][n][2 * h + 1][m] = dx[n][1];
-        }
-        load(b0 + 4 * NW);
+        for (int k = 0; k < 4; ++k) { wc[k] = wf[k]; xc[k] = xf[k]; dc[k] = bs + k >= b0 ? __half2float(dw[k]) : 0.0f; }
+        dxs[wave][2 * h][m] = dx[0];
+        dxs[wave][2 * h + 1][m] = dx[1];
+        load(b0 + 4 * NW);                                       // past the end: in bounds and not used
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 4; ++k) {
+            v16i z = {};
+            z = __builtin_amdgcn_mfma_i32_32x32x32_i8(xc[k], wc[k], z, 0, 0, 0);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                v16i z = {};
-                z = __builtin_amdgcn_mfma_i32_32x32x32_i8(xc[n][k], wc[k], z, 0, 0, 0);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float4 d = *reinterpret_cast<const float4 *>(&dxs[wave][n][k][8 * q + 4 * h]);
-                    acc[n][4 * q + 0] = fmaf((float) z[4 * q + 0], d.x * dc[k], acc[n][4 * q + 0]);
-                    acc[n][4 * q + 1] = fmaf((float) z[4 * q + 1], d.y * dc[k], acc[n][4 * q + 1]);
-                    acc[n][4 * q + 2] = fmaf((float) z[4 * q + 2], d.z * dc[k], acc[n][4 * q + 2]);
-                    acc[n][4 * q + 3] = fmaf((float) z[4 * q + 3], d.w * dc[k], acc[n][4 * q + 3]);
-                }
+            for (int q = 0; q < 4; ++q) {
+                const float4 d = *reinterpret_cast<const float4 *>(&dxs[wave][k][8 * q + 4 * h]);
+                acc[4 * q + 0] = fmaf((float) z[4 * q + 0], d.x * dc[k], acc[4 * q + 0]);
+                acc[4 * q + 1] = fmaf((float) z[4 * q + 1], d.y * dc[k], acc[4 * q + 1]);
+                acc[4 * q + 2] = fmaf((float) z[4 * q + 2], d.z * dc[k], acc[4 * q + 2]);
+                acc[4 * q + 3] = fmaf((float) z[4 * q + 3], d.w * dc[k], acc[4 * q + 3]);
             }
+        }
         __builtin_amdgcn_wave_barrier();
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        if (n) __syncthreads();
+    for (int i = 0; i < 16; ++i) part[wave][8 * (i / 4) + 4 * h + (i & 3)][m] = acc[i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 1024; e += 64 * NW) {
+        const int t = e >> 5, c = e & 31;
+        if (t0 + t < a.T && o0 + c < a.n_out) {
+            float v = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) part[wave][8 * (i / 4) + 4 * h + (i & 3)][m] = acc[n][i];
-        __syncthreads();
-        for (int e = threadIdx.x; e < 1024; e += 64 * NW) {
-            const int t = e >> 5, c = e & 31;
-            const int64_t tt = t0 + 32 * n + t;
-            if (tt < a.T && (int) blockIdx.x * 32 + c < a.n_out) {
-                float v = 0.0f;
-#pragma unroll
-                for (int w = 0; w < NW; ++w) v += part[w][t][c];
-                a.y[tt * a.ldy + (int) blockIdx.x * 32 + c] = v;
-            }
+            for (int w = 0; w < NW; ++w) v += part[w][t][c];
+            a.y[(t0 + t) * a.ldy + o0 + c] = v;
         }
     }
 }
 
-// Many tokens: BM tokens x 128 rows per workgroup of four waves, both operands through LDS in steps of four blocks (128 bytes a
-// row), two stages. A wave owns 64 tokens x 16 BM / 32 rows as 32x32 tiles.
+// Many tokens: BM tokens x BN rows per workgroup, both operands through LDS in steps of four blocks (128 bytes a row), two stages. A
+// wave owns 32 tokens x 32 NN rows; with KS = 2 two waves share them, each with every other block, joined at the end.
 //
 // What bounds it is the vector pipe: a 32x32x32 MFMA takes 32 cycles and leaves 16 integers per lane, each of which costs a
-// conversion, the product of its two scales and a fused multiply-add (48 instructions of 4 cycles, packed F32 being off).
+// conversion, the product of its two scales and a fused multiply-add (48 instructions of 4 cycles, packed F32 being off). At 2048
+// tokens x 4096 -> 14336 the vector pipe issues in 85 % of the cycles, the matrix pipe in 11 %, without LDS conflicts.
+//   waves      four per SIMD: a wave waits for LDS, MFMA and conversions in turn (four waves of 64 x 64 in the place of eight of 32 x 64:
+//              559 us against 463).
 //   LDS        16-byte chunks of a row at chunk ^ ((row >> 1) & 7): the 16 rows of a fragment read hit all 64 banks once.
-//   scales     [block][row] as F32: a lane reads the four tokens of a register group as one broadcast.
+//   scales     [block][row]: a lane reads the four tokens of a register group as one broadcast.
 //   workgroups XCD k (round-robin dispatch) takes the row panels k, k + 8, ... with all their token tiles: a panel of the weight
 //              comes from memory once and stays in that XCD's L2.
-template <int BM, int NN /* 32x32 tiles per wave, along the rows */>
-__global__ __launch_bounds__(8 * BM / NN, NN == 1 ? 4 : BM == 128 ? 4 : 3) void dense_mfma_kernel(const DenseArgs a, int n_tt) {
-    constexpr int BN = 128, NM = 1;
-    constexpr int NT = 8 * BM / NN, XL = NN, WL = 128 * NN / BM, SL = 512 / NT;                      // 16-byte loads per thread and stage
+template <int BM, int BN, int NN, int KS>
+__global__ __launch_bounds__(BM * BN / 16 / NN * KS, 4) void dense_mfma_kernel(const DenseArgs a, int n_tt) {
+    constexpr int NT = BM * BN / 16 / NN * KS;                      // threads
+    constexpr int XL = BM * 8 / NT, WL = BN * 8 / NT;               // 16-byte loads per thread and stage
+    constexpr int XS = (4 * BM + NT - 1) / NT, WS = (4 * BN + NT - 1) / NT;      // scales per thread and stage
+    constexpr int D = BM == 128 ? 1 : 2;                            // stages asked for ahead of the one in use (128: no registers for two)
+    static_assert(NT * XL == BM * 8 && NT * WL == BN * 8, "whole loads");
     __shared__ __align__(16) int8_t xs[2][BM * 128];
     __shared__ __align__(16) int8_t ws[2][BN * 128];
-    __shared__ __align__(16) float dxs[2][4][BM];
-    __shared__ __half dws[2][4][BN];
+    __shared__ __align__(16) float dxs[2][4 * BM];
+    __shared__ __half dws[2][4 * BN];
     const int id = (int) blockIdx.x, seq = id >> 3;
     const int o_tile = ((seq / n_tt) * 8 + (id & 7)) * BN;
     const int64_t t_tile = (int64_t) (seq % n_tt) * BM;
     if (o_tile >= a.n_out) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 31, h = lane >> 5;
-    const int wt = (wave % (BM / 32)) * 32, wo = (wave / (BM / 32)) * 32 * NN;
+    const int wt = (wave % (BM / 32)) * 32, wo = (wave / (BM / 32)) % (BN / 32 / NN) * 32 * NN, ks = KS == 1 ? 0 : wave / (BM * BN / 1024 / NN);
     const int64_t n_in = (int64_t) a.nblk * 32;
     const int lr = tid >> 3, lc = tid & 7;                          // staging: rows lr + NT / 8 i, chunk lc
     const int8_t * xp[XL], * wp[WL];
@@ -215,14 +204,11 @@ __global__ __launch_bounds__(8 * BM / NN, NN == 1 ? 4 : BM == 128 ? 4 : 3) void 
     for (int i = 0; i < XL; ++i) xp[i] = a.xq + min(t_tile + lr + NT / 8 * i, a.T - 1) * a.ldq;
 #pragma unroll
     for (int i = 0; i < WL; ++i) wp[i] = a.wq + (int64_t) min(o_tile + lr + NT / 8 * i, a.n_out - 1) * n_in;
-    const int sr = tid & 127, sb = (tid >> 7) * SL;                 // scales: row sr, blocks sb .. sb + SL - 1
-    const float * dxp = a.xd + min(t_tile + (sr < BM ? sr : 0), a.T - 1) * a.ldd;
-    const __half * dwp = a.wd + (int64_t) min(o_tile + sr, a.n_out - 1) * a.nblk;
+    const float * dxp = a.xd + min(t_tile + tid % BM, a.T - 1) * a.ldd;               // scale e of a stage: row e % BM (BN), block e / BM (BN)
+    const __half * dwp = a.wd + (int64_t) min(o_tile + tid % BN, a.n_out - 1) * a.nblk;
     const int st_off = lr * 128 + ((lc ^ ((lr >> 1) & 7)) << 4);    // rows 16 apart have the same key
 
-    // stages asked for ahead of the one in use: with one workgroup per CU a step's arithmetic (0.8 us) does not cover a load
-    constexpr int D = BM == 128 ? 1 : 2;
-    struct Stage { v4i x[XL], w[WL]; float dx[SL]; __half dw[SL]; } pre[D];
+    struct Stage { v4i x[XL], w[WL]; float dx[XS]; __half dw[WS]; } pre[D];
     auto load = [&](int b0, Stage & r) {
         const int cb = min(b0 + (lc >> 1), a.nblk - 1);             // blocks past the end: the last one, with scales of zero
         const int64_t off = (int64_t) cb * 32 + (lc & 1) * 16;
@@ -231,11 +217,9 @@ __global__ __launch_bounds__(8 * BM / NN, NN == 1 ? 4 : BM == 128 ? 4 : 3) void 
 #pragma unroll
         for (int i = 0; i < WL; ++i) r.w[i] = *reinterpret_cast<const v4i *>(wp[i] + off);
 #pragma unroll
-        for (int k = 0; k < SL; ++k) {
-            const int b = min(b0 + sb + k, a.nblk - 1);
-            r.dx[k] = dxp[b]; r.dw[k] = dwp[b];
-            if (b0 + sb + k >= a.nblk) { r.dx[k] = 0.0f; r.dw[k] = __half(0.0f); }
-        }
+        for (int k = 0; k < XS; ++k) { const int b = b0 + ((tid + NT * k) / BM & 3); r.dx[k] = dxp[min(b, a.nblk - 1)]; if (b >= a.nblk) r.dx[k] = 0.0f; }
+#pragma unroll
+        for (int k = 0; k < WS; ++k) { const int b = b0 + ((tid + NT * k) / BN & 3); r.dw[k] = dwp[min(b, a.nblk - 1)]; if (b >= a.nblk) r.dw[k] = __half(0.0f); }
     };
     auto store = [&](int st, const Stage & r) {
 #pragma unroll
@@ -243,18 +227,15 @@ __global__ __launch_bounds__(8 * BM / NN, NN == 1 ? 4 : BM == 128 ? 4 : 3) void 
 #pragma unroll
         for (int i = 0; i < WL; ++i) *reinterpret_cast<v4i *>(&ws[st][st_off + i * 16 * NT]) = r.w[i];
 #pragma unroll
-        for (int k = 0; k < SL; ++k) {
-            if (sr < BM) dxs[st][sb + k][sr] = r.dx[k];
-            dws[st][sb + k][sr] = r.dw[k];
-        }
+        for (int k = 0; k < XS; ++k) if (tid + NT * k < 4 * BM) dxs[st][tid + NT * k] = r.dx[k];
+#pragma unroll
+        for (int k = 0; k < WS; ++k) if (tid + NT * k < 4 * BN) dws[st][tid + NT * k] = r.dw[k];
     };
-    float acc[NM][NN][16];
+    float acc[NN][16];
 #pragma unroll
-    for (int i = 0; i < NM; ++i)
+    for (int j = 0; j < NN; ++j)
 #pragma unroll
-        for (int j = 0; j < NN; ++j)
-#pragma unroll
-            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+        for (int q = 0; q < 16; ++q) acc[j][q] = 0.0f;
     const int n_step = (a.nblk + 3) / 4, key = (m >> 1) & 7;        // tiles start at multiples of 32 rows: the key is the lane's
     load(0, pre[0]);
     store(0, pre[0]);
@@ -267,50 +248,56 @@ __global__ __launch_bounds__(8 * BM / NN, NN == 1 ? 4 : BM == 128 ? 4 : 3) void 
         if (s >= n_step) break;
         __syncthreads();
         const int st = s & 1;
-        load(4 * (s + D), pre[(d + D - 1) % D]);                    // past the end: in bounds, with scales of zero, and not stored
+        load(4 * (s + D), pre[(d + D - 1) % D]);                    // past the end: in bounds and not stored
 #pragma unroll 1                                                    // or every MFMA of the step is started first, and registers spill
-        for (int k = 0; k < 4; ++k) {
+        for (int k = ks; k < 4; k += KS) {
             const int ch = ((2 * k + h) ^ key) << 4;
-            v4i xf[NM], wf[NN];
+            const v4i xf = *reinterpret_cast<const v4i *>(&xs[st][(wt + m) * 128 + ch]);
+            v4i wf[NN];
             float dw[NN];
+            v16i z[NN];
 #pragma unroll
-            for (int i = 0; i < NM; ++i) xf[i] = *reinterpret_cast<const v4i *>(&xs[st][(wt + 32 * i + m) * 128 + ch]);
+            for (int j = 0; j < NN; ++j) { wf[j] = *reinterpret_cast<const v4i *>(&ws[st][(wo + 32 * j + m) * 128 + ch]); dw[j] = __half2float(dws[st][k * BN + wo + 32 * j + m]); }
 #pragma unroll
-            for (int j = 0; j < NN; ++j) { wf[j] = *reinterpret_cast<const v4i *>(&ws[st][(wo + 32 * j + m) * 128 + ch]); dw[j] = __half2float(dws[st][k][wo + 32 * j + m]); }
+            for (int j = 0; j < NN; ++j) {
+                const v16i zero = {};
+                z[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf, wf[j], zero, 0, 0, 0);
+            }
 #pragma unroll
-            for (int i = 0; i < NM; ++i) {
-                v16i z[NN];
+            for (int g = 0; g < 4; ++g) {
+                const float4 d4 = *reinterpret_cast<const float4 *>(&dxs[st][k * BM + wt + 8 * g + 4 * h]);
+                const float dx[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
-                for (int j = 0; j < NN; ++j) {
-                    v16i zero = {};
-                    z[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf[i], wf[j], zero, 0, 0, 0);
-                }
+                for (int j = 0; j < NN; ++j)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const float4 d4 = *reinterpret_cast<const float4 *>(&dxs[st][k][wt + 32 * i + 8 * g + 4 * h]);
-                    const float d[4] = {d4.x, d4.y, d4.z, d4.w};
-#pragma unroll
-                    for (int j = 0; j < NN; ++j)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) acc[i][j][4 * g + q] = fmaf((float) z[j][4 * g + q], d[q] * dw[j], acc[i][j][4 * g + q]);
-                }
+                    for (int q = 0; q < 4; ++q) acc[j][4 * g + q] = fmaf((float) z[j][4 * g + q], dx[q] * dw[j], acc[j][4 * g + q]);
             }
         }
         if (s + 1 < n_step) store(st ^ 1, pre[d]);
     }
+    if constexpr (KS == 2) {                                        // 4 KB per pair of waves: as much as the stages of x hold
+        static_assert(KS == 1 || (NN == 1 && BM * BN * 4 <= 2 * BM * 128), "room for the second halves");
+        float * red = reinterpret_cast<float *>(xs) + (wave % (NT / 128)) * 1024 + lane;
+        __syncthreads();
+        if (ks)
 #pragma unroll
-    for (int i = 0; i < NM; ++i)
+            for (int q = 0; q < 16; ++q) red[64 * q] = acc[0][q];
+        __syncthreads();
+        if (ks) return;
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-            const int64_t t = t_tile + wt + 32 * i + 8 * (q / 4) + 4 * h + (q & 3);
-            if (t < a.T) {
+        for (int q = 0; q < 16; ++q) acc[0][q] += red[64 * q];
+    }
 #pragma unroll
-                for (int j = 0; j < NN; ++j) {
-                    const int o = o_tile + wo + 32 * j + m;
-                    if (o < a.n_out) a.y[t * a.ldy + o] = acc[i][j][q];
-                }
+    for (int q = 0; q < 16; ++q) {
+        const int64_t t = t_tile + wt + 8 * (q / 4) + 4 * h + (q & 3);
+        if (t < a.T) {
+#pragma unroll
+            for (int j = 0; j < NN; ++j) {
+                const int o = o_tile + wo + 32 * j + m;
+                if (o < a.n_out) a.y[t * a.ldy + o] = acc[j][q];
             }
         }
+    }
 }
 
 template <int TT, int R, int U>
@@ -318,29 +305,40 @@ static void launch_few(const DenseArgs & a, hipStream_t s) {
     hipLaunchKernelGGL((dense_few_kernel<TT, R, U>), dim3((unsigned) ((a.n_out + 4 * R - 1) / (4 * R)), (unsigned) ((a.T + TT - 1) / TT)), dim3(256), 0, s, a);
 }
 
-template <int NT, int NW>
-static void launch_mid(const DenseArgs & a, hipStream_t s) {
-    hipLaunchKernelGGL((dense_mid_kernel<NT, NW>), dim3((unsigned) ((a.n_out + 31) / 32), (unsigned) ((a.T + 32 * NT - 1) / (32 * NT))), dim3(64 * NW), 0, s, a);
+template <int BM, int BN, int NN, int KS>
+static void launch_mfma(const DenseArgs & a, hipStream_t s) {
+    const int n_tt = (int) ((a.T + BM - 1) / BM), n_pan = (a.n_out + BN - 1) / BN;
+    hipLaunchKernelGGL((dense_mfma_kernel<BM, BN, NN, KS>), dim3((unsigned) ((n_pan + 7) / 8 * 8 * n_tt)), dim3(BM * BN / 16 / NN * KS), 0, s, a, n_tt);
 }
 
 static int launch_dense(const DenseArgs & all, hipStream_t s) {
-    // a launch has fewer than 2^32 threads: tokens in chunks for very many of them
-    const int64_t n_pan = (all.n_out + 127) / 128, chunk = std::max<int64_t>(1, std::min<int64_t>(8192, (1 << 22) / n_pan)) * 128;
+    // Which form, from 3 tokens on: us per 128 bytes of K, by the rounds in which the workgroups fill the CUs (r = workgroups per CU,
+    // rounded up), fitted to nine shapes between 1152 and 14336 at 33 to 2048 tokens:
+    //   32 x 32 (mid) 0.34 r + 0.1;  64 x 64, two waves per tile 0.66 r + 0.16;  64 x 128 1.0 r + 0.2;  128 x 128 1.85 r - 0.2, 2.35 at least
+    // 14336 -> 4096, us at 64 / 128 / 256 / 512 / 2048 tokens: mid 38 / 73 / 143 / 283 / 1122, 64 x 64 94 / 93 / 93 / 151 / 655,
+    // 64 x 128 134 / 133 / 133 / 134 / 467, 128 x 128 249 / 263 / 261 / 259 / 403; 4096 -> 14336: 50 / 86 / 165 / 327 / 1304,
+    // 30 / 44 / 83 / 145 / 649, 41 / 41 / 65 / 124 / 485, 73 / 76 / 77 / 112 / 421.
+    auto rounds = [&](int bm, int bn) {
+        const int64_t wg = ((all.T + bm - 1) / bm) * ((all.n_out + bn - 1) / bn), cu = lib().num_cu;
+        return (double) ((wg + cu - 1) / cu);
+    };
+    const double cost[4] = {0.34 * rounds(32, 32) + 0.1, 0.66 * rounds(64, 64) + 0.16, 1.0 * rounds(64, 128) + 0.2, std::max(2.35, 1.85 * rounds(128, 128) - 0.2)};
+    const int form = (int) (std::min_element(cost, cost + 4) - cost);
+    // a launch has fewer than 2^32 threads, 65536 token tiles in its second dimension: tokens in chunks for very many of them
+    const int64_t n_pan = (all.n_out + 63) / 64, chunk = std::max<int64_t>(1, std::min<int64_t>(1024, (1 << 21) / n_pan)) * 128;
     for (int64_t t0 = 0; t0 < all.T; t0 += chunk) {
         DenseArgs a = all;
         a.T = std::min(chunk, all.T - t0);
         a.xq += t0 * a.ldq; a.xd += t0 * a.ldd; a.y += t0 * a.ldy;
+        // one and two tokens: 12.1 / 15.2 us for 4096 -> 14336 (mid 19); up to 8 where mid would have less than a workgroup for every
+        // fourth CU and long rows (6912 -> 1152, 3 / 8 tokens: 7.3 / 8.6 us, mid 12.7 / 13.6); fewer than four blocks: no group for mid
+        const bool narrow = all.T <= 8 && a.nblk >= 128 && a.n_out <= 8 * lib().num_cu;
         if (all.T == 1)       { if (a.nblk >= 96) launch_few<1, 2, 4>(a, s); else launch_few<1, 2, 2>(a, s); }
-        else if (all.T == 2 || a.nblk < 4) launch_few<2, 2, 4>(a, s);
-        else if (all.T <= 32) launch_mid<1, 8>(a, s);
-        else if (all.T <= 64) launch_mid<2, 8>(a, s);
-        else {
-            const bool half = n_pan * ((all.T + 127) / 128) < 4 * lib().num_cu;
-            const int n_tt = (int) (half ? (a.T + 63) / 64 : (a.T + 127) / 128);
-            const dim3 grid((unsigned) ((n_pan + 7) / 8 * 8 * n_tt));
-            if (half) hipLaunchKernelGGL((dense_mfma_kernel<64, 1>), grid, dim3(512), 0, s, a, n_tt);
-            else      hipLaunchKernelGGL((dense_mfma_kernel<128, 2>), grid, dim3(512), 0, s, a, n_tt);
-        }
+        else if (all.T == 2 || narrow || a.nblk < 4) launch_few<2, 2, 4>(a, s);
+        else if (form == 0) hipLaunchKernelGGL(dense_mid_kernel, dim3((unsigned) ((a.n_out + 31) / 32), (unsigned) ((a.T + 31) / 32)), dim3(512), 0, s, a);
+        else if (form == 1) launch_mfma<64, 64, 1, 2>(a, s);
+        else if (form == 2) launch_mfma<64, 128, 1, 1>(a, s);
+        else                launch_mfma<128, 128, 2, 1>(a, s);
     }
     SDH_HIP_CHECK(hipGetLastError());
     return SDH_OK;
