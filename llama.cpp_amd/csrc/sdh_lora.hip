@@ -1,11 +1,15 @@
 // sdh_lora.hip — low-rank adapters of many requests beside one projection: y[t] = base[t] + scale_a B_a (A_a x[t]), a = ids[t].
 //
-// Three steps: the tokens are sorted by adapter and cut into tiles of 32 of one adapter each (lora_plan_kernel; ids live on the
-// device, so a captured graph sees the ids of the replay), u = A x for every tile (lora_shrink_kernel), y = base + scale B u
-// (lora_expand_kernel). An adapter is then read once per tile of its tokens, whatever the order of the tokens.
+// Two steps: u = A x for the tokens of an adapter (lora_shrink_kernel, K = n_in, split over workgroups), y = base + B (scale u)
+// (lora_expand_kernel, K = rank). Tokens are taken by adapter, 32 at a time, so an adapter is read once per 32 of its tokens in
+// whatever order they stand. ids live on the device (a captured graph sees the ids of the replay), so the sorting does too:
+//   up to 64 tokens   a wave sees all ids at once: the first token of an adapter does the work of all of them (no launch for it);
+//   more              lora_plan_kernel sorts the tokens by adapter and cuts them into tiles.
+// One to four tokens of small adapters take one launch (lora_fused_kernel) in which every workgroup forms u for itself.
 //
-// Everything is F32: v_mfma_f32_16x16x4_f32 for u, whose K is long (n_in), fused multiply-adds for y, whose K is the rank: that
-// step moves 8 bytes per output for 2 * rank operations.
+// Everything is F32: v_mfma_f32_16x16x4_f32 does 2048 operations in 32 cycles, and both steps move far more bytes than that costs
+// (8 bytes of y per 2 * rank operations, 4 of x per 2 * rank). Which k an MFMA takes is free as long as both operands agree: lane
+// group g = lane >> 4 holds consecutive columns and MFMA j multiplies its j-th, so every operand load is a vector.
 #include "sdh_internal.h"
 
 #include <algorithm>
@@ -16,41 +20,56 @@ namespace sdh {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 
+// A: [rank][a_ld], columns past n_in zero. B in the order of the expand kernel's fragments: per 16 output rows, per 16 ranks,
+// [lane][4] with row lane & 15 and ranks 4 (lane >> 4) ..; up to rank 8 one [lane][2] with ranks 2 (lane >> 4) ..; rows past n_out
+// and ranks past `rank` zero.
 struct LoraAdapter {
-    const void * a;        // [rank][a_ld]   f16 / f32, columns past n_in zero
-    const void * b;        // [n_out][r_ld]  f16 / f32, columns past rank zero
+    const void * a;
+    const void * b;
     float scale;
-    int rank, r_ld, f32;
+    int rank, r_ld, f32;   // r_ld: 8, or rank rounded up to 16
 };
+
+__host__ __device__ inline int64_t lora_b_at(int64_t o, int r, int r_ld) {
+    const int64_t tile = (o >> 4) * 16 * r_ld;
+    const int row = (int) (o & 15);
+    if (r_ld == 8) return tile + (((r >> 1) * 16 + row) << 1) + (r & 1);
+    return tile + (r >> 4) * 256 + ((((r & 15) >> 2) * 16 + row) << 2) + (r & 3);
+}
 
 struct LoraSet {
     int64_t n_in = 0, n_out = 0, a_ld = 0;
     int n = 0, u_ld = 0;                   // adapters; row pitch of u: the largest r_ld
+    bool any_f32 = false;
     uint8_t * dev = nullptr;               // the LoraAdapter table, then the matrices
     int64_t stored_bytes = 0;
 };
 
-constexpr int LT = 32;                     // tokens per tile
-constexpr int LORA_RC = 64;                // ranks per pass of the shrink kernel
+constexpr int LT = 32;                     // tokens per tile of the shrink kernel
+constexpr int ET = 128;                    // ... of the expand kernel, where there are many (else 32)
+constexpr int LORA_RC = 32;                // ranks per workgroup of the shrink kernel
 
 struct LoraTile { int adapter, start, count, pad; };       // adapter -1: none
 
 // the caller's workspace
 struct LoraWs {
-    int * perm; LoraTile * tiles; int * n_tiles; float * u;
-    int64_t max_tiles; int splits; int64_t bytes;
+    int * perm; LoraTile * tiles; LoraTile * etiles; int * n_tiles; float * u;
+    int64_t max_tiles, max_etiles; int splits, et; int64_t bytes;
 };
 
 static LoraWs lora_ws(const LoraSet & l, int64_t T, uint8_t * base) {
     LoraWs w{};
     auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+    w.et = T >= 2048 && l.u_ld <= 64 ? ET : LT;
     w.max_tiles = (T + LT - 1) / LT + std::min<int64_t>(T, l.n + 1);
-    // K splits of the shrink step: about two workgroups per CU, at least 128 columns each
+    w.max_etiles = (T + w.et - 1) / w.et + std::min<int64_t>(T, l.n + 1);
+    // K splits of the shrink step: about four workgroups per CU, at least 128 columns each
     const int64_t tiles = (T + LT - 1) / LT, most = std::max<int64_t>(1, l.n_in / 128);
-    w.splits = (int) std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, most), 512 / tiles));
+    w.splits = (int) std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, most), 1024 / tiles));
     int64_t at = 0;
     w.perm = (int *) (base + at);         at += up(T * 4);
     w.tiles = (LoraTile *) (base + at);   at += up(w.max_tiles * (int64_t) sizeof(LoraTile));
+    w.etiles = (LoraTile *) (base + at);  at += up(w.max_etiles * (int64_t) sizeof(LoraTile));
     w.n_tiles = (int *) (base + at);      at += 256;
     w.u = (float *) (base + at);          at += up((int64_t) w.splits * T * l.u_ld * 4);
     w.bytes = at;
@@ -61,37 +80,67 @@ static LoraWs lora_ws(const LoraSet & l, int64_t T, uint8_t * base) {
 // One workgroup: count, scan, scatter. The place of a token inside its adapter's run depends on the order of the atomics; no
 // result depends on the place.
 __global__ __launch_bounds__(1024)
-void lora_plan_kernel(const int * __restrict__ ids, int64_t T, int n, int * __restrict__ perm, LoraTile * __restrict__ tiles, int * __restrict__ n_tiles) {
+void lora_plan_kernel(const int * __restrict__ ids, int64_t T, int n, int * __restrict__ perm, LoraTile * __restrict__ tiles, LoraTile * __restrict__ etiles, int et, int * __restrict__ n_tiles) {
     extern __shared__ int lds[];
-    int * cnt = lds, * off = lds + (n + 1), * toff = lds + 2 * (n + 1);      // bin n: no adapter
-    __shared__ int wsum[2][16];
+    int * cnt = lds, * off = lds + (n + 1);                  // bin n: no adapter
+    __shared__ int wsum[3][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int b = tid; b <= n; b += 1024) cnt[b] = 0;
     __syncthreads();
-    auto bin = [&](int64_t t) { const int a = ids ? ids[t] : 0; return (unsigned) a < (unsigned) n ? a : n; };
-    for (int64_t t = tid; t < T; t += 1024) atomicAdd(&cnt[bin(t)], 1);
-    __syncthreads();
-    // exclusive sums of the counts and of the tile counts, a contiguous share of the bins per thread
-    const int per = (n + 1 + 1023) / 1024, b0 = tid * per, b1 = min(n + 1, b0 + per);
-    int c = 0, k = 0;
-    for (int b = b0; b < b1; ++b) { c += cnt[b]; k += (cnt[b] + LT - 1) / LT; }
-    int ci = c, ki = k;
-    for (int m = 1; m < 64; m <<= 1) {
-        const int cu = __shfl_up(ci, m, 64), ku = __shfl_up(ki, m, 64);
-        if (lane >= m) { ci += cu; ki += ku; }
+    auto bin = [&](int64_t t) { const int a = t < T && ids ? ids[t] : 0; return t >= T ? -1 : (unsigned) a < (unsigned) n ? a : n; };
+    // adds the wave's tokens to the counters of their adapters, one LDS atomic per adapter -> this lane's place
+    auto count_in = [&](int b, int * counter) {
+        int place = 0;
+        for (unsigned long long left = __ballot(b >= 0); left;) {
+            const int first = __ffsll(left) - 1, one = __shfl(b, first, 64);
+            const unsigned long long m = __ballot(b == one);
+            int at = 0;
+            if (lane == first) at = atomicAdd(&counter[one], __popcll(m));
+            at = __shfl(at, first, 64);
+            if (b == one) place = at + __popcll(m & ((1ull << lane) - 1));
+            left &= ~m;
+        }
+        return place;
+    };
+    const int64_t t_end = (T + 4095) / 4096 * 4096;         // four ids in flight per thread; all lanes take part
+    for (int64_t t = tid; t < t_end; t += 4096) {
+        const int b[4] = {bin(t), bin(t + 1024), bin(t + 2048), bin(t + 3072)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) count_in(b[i], cnt);
     }
-    if (lane == 63) { wsum[0][wave] = ci; wsum[1][wave] = ki; }
     __syncthreads();
-    int cb = ci - c, kb = ki - k;
-    for (int w = 0; w < wave; ++w) { cb += wsum[0][w]; kb += wsum[1][w]; }
+    // exclusive sums of the counts and of both tile counts, a contiguous share of the bins per thread
+    const int per = (n + 1 + 1023) / 1024, b0 = min(n + 1, tid * per), b1 = min(n + 1, b0 + per);
+    int v[3] = {0, 0, 0}, in[3];
+    for (int b = b0; b < b1; ++b) { v[0] += cnt[b]; v[1] += (cnt[b] + LT - 1) / LT; v[2] += (cnt[b] + et - 1) / et; }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        in[i] = v[i];
+        for (int m = 1; m < 64; m <<= 1) { const int up = __shfl_up(in[i], m, 64); if (lane >= m) in[i] += up; }
+        if (lane == 63) wsum[i][wave] = in[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        v[i] = in[i] - v[i];
+        for (int w = 0; w < wave; ++w) v[i] += wsum[i][w];
+    }
     for (int b = b0; b < b1; ++b) {
-        off[b] = cb; toff[b] = kb;
-        for (int j = 0; j * LT < cnt[b]; ++j) tiles[kb + j] = LoraTile{b < n ? b : -1, cb + j * LT, min(LT, cnt[b] - j * LT), 0};
-        cb += cnt[b]; kb += (cnt[b] + LT - 1) / LT;
+        off[b] = v[0];
+        for (int j = 0; j < cnt[b]; j += LT) tiles[v[1]++] = LoraTile{b < n ? b : -1, v[0] + j, min(LT, cnt[b] - j), 0};
+        for (int j = 0; j < cnt[b]; j += et) etiles[v[2]++] = LoraTile{b < n ? b : -1, v[0] + j, min(et, cnt[b] - j), 0};
+        v[0] += cnt[b];
     }
-    if (tid == 1023) *n_tiles = kb;
+    if (tid == 1023) { n_tiles[0] = v[1]; n_tiles[1] = v[2]; }
     __syncthreads();
-    for (int64_t t = tid; t < T; t += 1024) perm[atomicAdd(&off[bin(t)], 1)] = (int) t;
+    for (int64_t t = tid; t < t_end; t += 4096) {
+        const int b[4] = {bin(t), bin(t + 1024), bin(t + 2048), bin(t + 3072)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int place = count_in(b[i], off);
+            if (b[i] >= 0) perm[place] = (int) (t + 1024 * i);
+        }
+    }
 }
 
 // eight consecutive weights as F32
@@ -108,6 +157,14 @@ __device__ __forceinline__ void load8(const float * p, float (&v)[8]) {
     const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
+template <int N> __device__ __forceinline__ void load_n(const __half * p, float (&v)[N]) {
+    __half h[N];
+    __builtin_memcpy(h, __builtin_assume_aligned(p, 2 * N), 2 * N);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __half2float(h[i]);
+}
+template <int N> __device__ __forceinline__ void load_n(const float * p, float (&v)[N]) { __builtin_memcpy(v, __builtin_assume_aligned(p, 4 * N), 4 * N); }
+
 // eight consecutive activations; past n: zero
 template <bool VEC>
 __device__ __forceinline__ void load8x(const float * p, int64_t k, int64_t n, float (&v)[8]) {
@@ -116,160 +173,338 @@ __device__ __forceinline__ void load8x(const float * p, int64_t k, int64_t n, fl
     for (int i = 0; i < 8; ++i) v[i] = k + i < n ? p[k + i] : 0.0f;
 }
 
-// ---- u[split][place][r] = sum over the split's columns of A[r][k] x[token][k] -----------------------------------------
-// 16x16x4 operands: row / column lane & 15, k = lane >> 4. Which k an MFMA takes is free as long as both operands agree: lane
-// group g holds columns 8 g .. 8 g + 7 of a 32-column step and MFMA j multiplies column 8 g + j, so every load is 16 bytes.
+template <bool VEC>
+__device__ __forceinline__ void load4x(const float * p, int64_t k, int64_t n, float (&v)[4]) {
+    if (VEC && k + 4 <= n) { load_n<4>(p + k, v); return; }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = k + i < n ? p[k + i] : 0.0f;
+}
+
+// ---- the tokens of a workgroup --------------------------------------------------------------------------------------
+// PLAN: tile `at` of the plan. Otherwise all tokens of the adapter of token `at`, if that is the first of them. -> the tokens in `list` (a row of LDS of each wave's own: LDS works in order within a wave, no barrier), their number (0:
+// nothing to do here) and the adapter (-1: none)
+template <bool PLAN>
+__device__ __forceinline__ int lora_tokens(const LoraTile * tiles, const int * n_tiles, const int * perm, const int * ids, int T, int n, int at, int * list, int * adapter) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (PLAN) {
+        const LoraTile tile = tiles[at];
+        if (at >= *n_tiles) return 0;
+        for (int i = lane; i < tile.count; i += 64) list[i] = perm[tile.start + i];
+        *adapter = tile.adapter;
+        return tile.count;
+    }
+    const int t = at;
+    int a = lane < T ? (ids ? ids[lane] : 0) : -2;          // -2: no token
+    if (lane < T && (unsigned) a >= (unsigned) n) a = -1;
+    const int mine = __shfl(a, t, 64);
+    const unsigned long long m = __ballot(a == mine);
+    if (m & ((1ull << t) - 1)) return 0;
+    if (a == mine) list[__popcll(m & ((1ull << lane) - 1))] = lane;
+    *adapter = mine;
+    return __popcll(m);
+}
+
+// ---- u[split][token][r] = sum over the split's columns of A[r][k] x[token][k] -------------------------------------------
+// A workgroup: one tile, LORA_RC ranks, one split of the columns; its four waves take steps of 32 columns in turn and are joined in
+// LDS. 16x16x4 operands: row / column lane & 15, k = lane >> 4; in a step lane group g holds columns 4 g .. 4 g + 3 and 16 + 4 g ..,
+// so that a load instruction takes 64 consecutive bytes of 16 tokens.
 template <typename W, bool VEC>
-__device__ void shrink_body(const LoraAdapter & ad, const LoraTile & tile, const int * perm, const float * x, int64_t ldx, int64_t n_in, int64_t a_ld,
+__device__ void shrink_tile(const LoraAdapter & ad, const int * list, int count, int rc, const float * x, int64_t ldx, int64_t n_in, int64_t a_ld,
                             int64_t k_begin, int64_t k_end, float * u, int u_ld, float (*red)[LT][LORA_RC + 1]) {
+    constexpr int NJ = LORA_RC / 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
     const W * A = (const W *) ad.a;
     const float * xr[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) xr[i] = x + (int64_t) perm[tile.start + min(16 * i + m, tile.count - 1)] * ldx;
-    for (int rc = 0; rc < ad.rank; rc += LORA_RC) {
-        const int nj = min(4, (ad.rank - rc + 15) / 16);
-        const W * ar[4];
+    for (int i = 0; i < 2; ++i) xr[i] = x + (int64_t) list[min(16 * i + m, count - 1)] * ldx;
+    const bool two = count > 16;
+    const int nj = min(NJ, (ad.rank - rc + 15) / 16);
+    const W * ar[NJ];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ar[j] = A + (int64_t) min(rc + 16 * j + m, ad.rank - 1) * a_ld;
-        v4f acc[2][4];
+    for (int j = 0; j < NJ; ++j) ar[j] = A + (int64_t) min(rc + 16 * j + m, ad.rank - 1) * a_ld;
+    v4f acc[2][NJ];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int64_t k = k_begin + 32 * wave; k < k_end; k += 128) {
-            float xv[2][8];
+        for (int j = 0; j < NJ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t k = k_begin + 32 * wave; k < k_end; k += 128) {
+        float xv[2][2][4], av[NJ][2][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) load8x<VEC>(xr[i], k + 8 * g, n_in, xv[i]);
+        for (int h = 0; h < 2; ++h) {
+            const int64_t at = k + 16 * h + 4 * g;
+            load4x<VEC>(xr[0], at, n_in, xv[0][h]);
+            if (two) load4x<VEC>(xr[1], at, n_in, xv[1][h]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j < nj) {
-                    float av[8];
-                    load8(ar[j] + k + 8 * g, av);
+            for (int j = 0; j < NJ; ++j) if (j < nj) load_n<4>(ar[j] + at, av[j][h]);
+        }
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        acc[0][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[0][q], av[q], acc[0][j], 0, 0, 0);
-                        acc[1][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[1][q], av[q], acc[1][j], 0, 0, 0);
+        for (int j = 0; j < NJ; ++j) {
+            if (j < nj) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        acc[0][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[0][h][q], av[j][h][q], acc[0][j], 0, 0, 0);
+                        if (two) acc[1][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[1][h][q], av[j][h][q], acc[1][j], 0, 0, 0);
                     }
-                }
             }
         }
+    }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) red[wave][16 * i + 4 * g + q][16 * j + m] = acc[i][j][q];
-        __syncthreads();
-        const int nr = min(LORA_RC, ad.r_ld - rc);
-        for (int e = threadIdx.x; e < tile.count * LORA_RC; e += 256) {
-            const int t = e / LORA_RC, r = e % LORA_RC;
-            if (r < nr)                                     // columns between rank and r_ld are zero, whatever x holds
-                u[(int64_t) (tile.start + t) * u_ld + rc + r] = rc + r < ad.rank ? (red[0][t][r] + red[1][t][r]) + (red[2][t][r] + red[3][t][r]) : 0.0f;
-        }
-        __syncthreads();
+            for (int q = 0; q < 4; ++q) red[wave][16 * i + 4 * g + q][16 * j + m] = acc[i][j][q];
+    __syncthreads();
+    const int nr = min(LORA_RC, ad.r_ld - rc);
+    for (int e = threadIdx.x; e < count * LORA_RC; e += 256) {
+        const int t = e / LORA_RC, r = e % LORA_RC;
+        if (r < nr)                                         // columns between rank and r_ld are zero, whatever x holds
+            u[(int64_t) list[t] * u_ld + rc + r] = rc + r < ad.rank ? (red[0][t][r] + red[1][t][r]) + (red[2][t][r] + red[3][t][r]) : 0.0f;
+    }
+    __syncthreads();
+}
+
+template <bool PLAN, bool VEC>
+__global__ __launch_bounds__(256)
+void lora_shrink_kernel(const LoraAdapter * __restrict__ ads, int n, const int * __restrict__ ids, const LoraTile * __restrict__ tiles, const int * __restrict__ n_tiles,
+                        const int * __restrict__ perm, const float * __restrict__ x, int64_t ldx, int64_t n_in, int64_t a_ld, int64_t T, int64_t k_split,
+                        float * __restrict__ u, int u_ld) {
+    __shared__ float red[4][LT][LORA_RC + 1];
+    __shared__ int lists[4][64];
+    int * list = lists[threadIdx.x >> 6];
+    int a = -1;
+    const int count = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, (int) blockIdx.x, list, &a);
+    if (!count || a < 0) return;
+    const LoraAdapter ad = ads[a];
+    const int rc = (int) blockIdx.z * LORA_RC;
+    if (rc >= ad.rank) return;
+    const int64_t k0 = (int64_t) blockIdx.y * k_split, k1 = min(a_ld, k0 + k_split);
+    float * us = u + (int64_t) blockIdx.y * T * u_ld;
+    for (int t0 = 0; t0 < count; t0 += LT) {
+        if (ad.f32) shrink_tile<float, VEC>(ad, list + t0, min(LT, count - t0), rc, x, ldx, n_in, a_ld, k0, k1, us, u_ld, red);
+        else        shrink_tile<__half, VEC>(ad, list + t0, min(LT, count - t0), rc, x, ldx, n_in, a_ld, k0, k1, us, u_ld, red);
     }
 }
 
+// ---- y[token][o] = base[token][o] + sum_r (scale sum_split u[split][token][r]) B[o][r] ----------------------------------
 template <bool VEC>
-__global__ __launch_bounds__(256)
-void lora_shrink_kernel(const LoraAdapter * __restrict__ ads, const LoraTile * __restrict__ tiles, const int * __restrict__ n_tiles, const int * __restrict__ perm,
-                        const float * __restrict__ x, int64_t ldx, int64_t n_in, int64_t a_ld, int64_t T, int64_t k_split, float * __restrict__ u, int u_ld) {
-    __shared__ float red[4][LT][LORA_RC + 1];
-    if ((int) blockIdx.x >= *n_tiles) return;
-    const LoraTile tile = tiles[blockIdx.x];
-    if (tile.adapter < 0) return;
-    const LoraAdapter ad = ads[tile.adapter];
-    const int64_t k0 = (int64_t) blockIdx.y * k_split, k1 = min(a_ld, k0 + k_split);
-    float * us = u + (int64_t) blockIdx.y * T * u_ld;
-    if (ad.f32) shrink_body<float, VEC>(ad, tile, perm, x, ldx, n_in, a_ld, k0, k1, us, u_ld, red);
-    else        shrink_body<__half, VEC>(ad, tile, perm, x, ldx, n_in, a_ld, k0, k1, us, u_ld, red);
-}
-
-// ---- y[token][o] = base[token][o] + sum_r (scale sum_split u[split][place][r]) B[o][r] --------------------------------
-template <bool VEC>
-__device__ __forceinline__ float4 row_load4(const float * p, int64_t o, int64_t n) {
-    if constexpr (VEC) return *reinterpret_cast<const float4 *>(p + o);
-    float4 v = make_float4(p[o], 0.0f, 0.0f, 0.0f);
-    if (o + 1 < n) v.y = p[o + 1];
-    if (o + 2 < n) v.z = p[o + 2];
-    if (o + 3 < n) v.w = p[o + 3];
+__device__ __forceinline__ v4f row_load4(const float * p, int o, int n) {
+    if constexpr (VEC) return *reinterpret_cast<const v4f *>(p + o);
+    v4f v = {p[o], 0.0f, 0.0f, 0.0f};
+    if (o + 1 < n) v[1] = p[o + 1];
+    if (o + 2 < n) v[2] = p[o + 2];
+    if (o + 3 < n) v[3] = p[o + 3];
     return v;
 }
 template <bool VEC>
-__device__ __forceinline__ void row_store4(float * p, int64_t o, int64_t n, float4 v) {
-    if constexpr (VEC) { *reinterpret_cast<float4 *>(p + o) = v; return; }
-    p[o] = v.x;
-    if (o + 1 < n) p[o + 1] = v.y;
-    if (o + 2 < n) p[o + 2] = v.z;
-    if (o + 3 < n) p[o + 3] = v.w;
+__device__ __forceinline__ void row_store4(float * p, int o, int n, v4f v) {
+    if constexpr (VEC) { *reinterpret_cast<v4f *>(p + o) = v; return; }
+    p[o] = v[0];
+    if (o + 1 < n) p[o + 1] = v[1];
+    if (o + 2 < n) p[o + 2] = v[2];
+    if (o + 3 < n) p[o + 3] = v[3];
 }
-
-template <typename W, bool VEC>
-__device__ void expand_body(const LoraAdapter & ad, const LoraTile & tile, const int * perm, const float * us, int64_t o, int64_t n_out,
-                            const float * base, int64_t ldb, float * y, int64_t ldy) {
-    constexpr int TC = 8;                                   // tokens per pass over the rank
-    const W * B = (const W *) ad.b;
-    const W * br[4];
+// A wave owns 64 columns (four fragments of 16) and takes its tokens 16 at a time; the next 16 tokens' base is asked for before the
+// present ones are multiplied. The result has column 4 (lane >> 4) + i in register i and token lane & 15: base and y are 16 bytes per
+// lane, 64 consecutive bytes of 16 tokens per instruction (a copy in this order runs at 5.1 TB/s, in whole rows at 5.2 to 5.6).
+struct ExpandWave {
+    const int * list; int count;           // tokens
+    const float * us; int us_ld;           // scale * u of them, in LDS
+    int64_t o0, n_out;                     // columns, o0 the same in all lanes
+    const float * base; int64_t ldb; float * y; int64_t ldy;
+};
+template <bool VEC>
+__device__ __forceinline__ void expand_base(const ExpandWave & e, int t0, v4f (&acc)[4]) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) br[c] = B + min(o + c, n_out - 1) * ad.r_ld;
-    for (int t0 = 0; t0 < tile.count; t0 += TC) {
-        int64_t tok[TC];
-        float4 acc[TC];
+    for (int j = 0; j < 4; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (!e.base) return;
+    const float * p = e.base + e.list[min(t0 + (lane & 15), e.count - 1)] * e.ldb + e.o0 + 4 * (lane >> 4);
+    const int left = (int) min(e.n_out - e.o0, (int64_t) 64) - 4 * (lane >> 4);
 #pragma unroll
-        for (int t = 0; t < TC; ++t) {
-            tok[t] = perm[tile.start + min(t0 + t, tile.count - 1)];
-            acc[t] = base ? row_load4<VEC>(base + tok[t] * ldb, o, n_out) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int j = 0; j < 4; ++j) if (16 * j < left) acc[j] = row_load4<VEC>(p, 16 * j, left);
+}
+template <bool VEC>
+__device__ __forceinline__ void expand_store(const ExpandWave & e, int t0, const v4f (&acc)[4]) {
+    const int lane = threadIdx.x & 63, t = t0 + (lane & 15);
+    if (t >= e.count) return;
+    float * p = e.y + e.list[t] * e.ldy + e.o0 + 4 * (lane >> 4);
+    const int left = (int) min(e.n_out - e.o0, (int64_t) 64) - 4 * (lane >> 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) if (16 * j < left) row_store4<VEC>(p, 16 * j, left, acc[j]);
+}
+// KQ: ranks per lane of a fragment: 4, or 2 for the one of 8 ranks
+template <typename W, int KQ, bool VEC>
+__device__ __forceinline__ void expand_wave(const ExpandWave & e, const W * b_all, int r_ld, v4f (&next)[4]) {
+    const int lane = threadIdx.x & 63;
+    const int last = (int) ((e.n_out - 1) >> 4), tile = (int) (e.o0 >> 4);
+#pragma unroll 1
+    for (int t0 = 0; t0 < e.count; t0 += 16) {
+        v4f acc[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = next[j];
+        if (t0 + 16 < e.count) expand_base<VEC>(e, t0 + 16, next);
+        const float * ur = e.us + (t0 + (lane & 15)) * e.us_ld + KQ * (lane >> 4);
+#pragma unroll 1
+        for (int r = 0; r < r_ld; r += 4 * KQ) {
+            float b[4][KQ], uv[KQ];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) load_n<KQ>(b_all + ((int64_t) min(tile + j, last) * r_ld + r) * 16 + KQ * lane, b[j]);
+            load_n<KQ>(ur + r, uv);
+#pragma unroll
+            for (int q = 0; q < KQ; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[j][q], uv[q], acc[j], 0, 0, 0);
         }
-        for (int r = 0; r < ad.r_ld; r += 8) {
-            float b[4][8];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) load8(br[c] + r, b[c]);
-#pragma unroll
-            for (int t = 0; t < TC; ++t) {
-                float uv[8];
-                load8(us + (t0 + t) * ad.r_ld + r, uv);
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    acc[t].x = fmaf(uv[q], b[0][q], acc[t].x); acc[t].y = fmaf(uv[q], b[1][q], acc[t].y);
-                    acc[t].z = fmaf(uv[q], b[2][q], acc[t].z); acc[t].w = fmaf(uv[q], b[3][q], acc[t].w);
-                }
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < TC; ++t)
-            if (t0 + t < tile.count) row_store4<VEC>(y + tok[t] * ldy, o, n_out, acc[t]);
+        expand_store<VEC>(e, t0, acc);
     }
 }
 
-template <bool VEC>
-__global__ __launch_bounds__(256)
-void lora_expand_kernel(const LoraAdapter * __restrict__ ads, const LoraTile * __restrict__ tiles, const int * __restrict__ n_tiles, const int * __restrict__ perm,
-                        const float * __restrict__ u, int u_ld, int splits, int64_t T, int64_t n_out, const float * base, int64_t ldb, float * y, int64_t ldy) {
-    extern __shared__ __align__(16) float us[];             // [LT][r_ld]
-    if ((int) blockIdx.x >= *n_tiles) return;
-    const LoraTile tile = tiles[blockIdx.x];
-    const int64_t o = 4 * ((int64_t) blockIdx.y * 256 + threadIdx.x);
-    if (tile.adapter < 0) {                                 // no adapter: y is the base
-        if (base == y || o >= n_out) return;
-        for (int t = 0; t < tile.count; ++t) {
-            const int64_t tok = perm[tile.start + t];
-            row_store4<VEC>(y + tok * ldy, o, n_out, base ? row_load4<VEC>(base + tok * ldb, o, n_out) : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+// tokens whose u is in LDS at a time: 34 KB at most
+__host__ __device__ constexpr int lora_expand_tokens(int r_ld) { return r_ld > 256 ? 16 : r_ld > 64 ? 32 : 128; }
+
+template <bool PLAN, bool VEC>
+__global__ __launch_bounds__(256, 4)
+void lora_expand_kernel(const LoraAdapter * __restrict__ ads, int n, const int * __restrict__ ids, const LoraTile * __restrict__ tiles, const int * __restrict__ n_tiles,
+                        const int * __restrict__ perm, const float * __restrict__ u, int u_ld, int splits, int64_t T, int64_t n_out,
+                        const float * base, int64_t ldb, float * y, int64_t ldy) {
+    extern __shared__ __align__(16) float us[];             // [lora_expand_tokens][r_ld + 4]
+    __shared__ int lists[4][PLAN ? ET : 64];
+    // neighbouring workgroups take neighbouring columns of the same tokens
+    const int n_col = (int) ((n_out + 255) >> 8), at = (int) (blockIdx.x / (unsigned) n_col), col = (int) (blockIdx.x % (unsigned) n_col);
+    const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
+    int * list = lists[wave];
+    int a = -1;
+    const int all = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, at, list, &a);
+    if (!all || (a < 0 && base == y)) return;
+    ExpandWave e{list, all, us, 0, (int64_t) col * 256 + 64 * wave, n_out, base, ldb, y, ldy};
+    v4f next[4];
+    if (a < 0) {                                            // no adapter: y is the base
+#pragma unroll 1
+        for (int t0 = 0; t0 < all; t0 += 16) {
+            expand_base<VEC>(e, t0, next);
+            expand_store<VEC>(e, t0, next);
         }
         return;
     }
-    const LoraAdapter ad = ads[tile.adapter];
-    for (int e = threadIdx.x; e < LT * ad.r_ld; e += 256) {
-        const int t = e / ad.r_ld, r = e - t * ad.r_ld;
-        float v = 0.0f;
-        if (t < tile.count)
-            for (int s = 0; s < splits; ++s) v += u[((int64_t) s * T + tile.start + t) * u_ld + r];
-        us[e] = ad.scale * v;
+    const LoraAdapter ad = ads[a];
+    e.us_ld = ad.r_ld + 4;                                  // 16-byte rows that start on different banks
+    const int step = lora_expand_tokens(ad.r_ld), n4 = ad.r_ld >> 2;
+    for (int t0 = 0; t0 < all; t0 += step) {
+        e.list = list + t0;
+        e.count = min(step, all - t0);
+        expand_base<VEC>(e, 0, next);
+        if (t0) __syncthreads();
+#pragma unroll 1
+        for (int i = threadIdx.x; i < (e.count + 15) / 16 * 16 * n4; i += 256) {
+            const int t = i / n4, r = 4 * (i - t * n4);
+            v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (t < e.count) {
+                const float * up = u + (int64_t) e.list[t] * u_ld + r;
+#pragma unroll 1
+                for (int s0 = 0; s0 < splits; s0 += 4) {    // four at a time in flight; past the last split: the last one, not added
+                    v4f p[4];
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) p[s] = *reinterpret_cast<const v4f *>(up + min(s0 + s, splits - 1) * T * u_ld);
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) if (s0 + s < splits) v += p[s];
+                }
+            }
+            *reinterpret_cast<v4f *>(us + t * e.us_ld + r) = ad.scale * v;
+        }
+        __syncthreads();
+        const auto wave = [&](auto type) {
+            using W = decltype(type);
+            const W * B = (const W *) ad.b;
+            if (ad.r_ld == 8) expand_wave<W, 2, VEC>(e, B, ad.r_ld, next);
+            else              expand_wave<W, 4, VEC>(e, B, ad.r_ld, next);
+        };
+        if (ad.f32) wave(float{}); else wave(__half{});
     }
+}
+
+// ---- one launch for one to four tokens ----------------------------------------------------------------------------------
+// dot products of R rows of A with one token, one wave; every lane returns the sums
+template <typename W, int R, bool VEC>
+__device__ __forceinline__ void wave_dots(const W * const (&ar)[R], const float * x, int64_t n_in, int64_t a_ld, float (&acc)[R]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = 0.0f;
+    for (int64_t k = 8 * lane; k < a_ld; k += 512) {
+        float xv[8];
+        load8x<VEC>(x, k, n_in, xv);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float av[8];
+            load8(ar[r] + k, av);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) acc[r] = fmaf(av[q], xv[q], acc[r]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        for (int m = 32; m > 0; m >>= 1) acc[r] += __shfl_xor(acc[r], m, 64);
+}
+
+template <typename W, bool VEC>
+__device__ void fused_u(const LoraAdapter & ad, const float * x, int64_t n_in, int64_t a_ld, float * us) {
+    const W * A = (const W *) ad.a;
+    for (int r0 = 2 * (threadIdx.x >> 6); r0 < ad.r_ld; r0 += 16) {
+        const W * const ar[2] = {A + (int64_t) min(r0, ad.rank - 1) * a_ld, A + (int64_t) min(r0 + 1, ad.rank - 1) * a_ld};
+        float acc[2];
+        wave_dots<W, 2, VEC>(ar, x, n_in, a_ld, acc);
+        if ((threadIdx.x & 63) == 0) {                      // columns between rank and r_ld are zero, whatever x holds
+            us[r0] = r0 < ad.rank ? ad.scale * acc[0] : 0.0f;
+            us[r0 + 1] = r0 + 1 < ad.rank ? ad.scale * acc[1] : 0.0f;
+        }
+    }
+}
+
+// one column: v + sum_r us[r] B[o][r]
+template <typename W>
+__device__ __forceinline__ float fused_column(const LoraAdapter & ad, int64_t o, const float * us, float v) {
+    const W * B = (const W *) ad.b + (o >> 4) * 16 * ad.r_ld;
+    if (ad.r_ld == 8) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float b[2];
+            load_n<2>(B + g * 32 + 2 * (o & 15), b);
+            v = fmaf(us[2 * g], b[0], v);
+            v = fmaf(us[2 * g + 1], b[1], v);
+        }
+        return v;
+    }
+    for (int r = 0; r < ad.r_ld; r += 16)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float b[4];
+            load_n<4>(B + r * 16 + g * 64 + 4 * (o & 15), b);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v = fmaf(us[r + 4 * g + q], b[q], v);
+        }
+    return v;
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(512)
+void lora_fused_kernel(const LoraAdapter * __restrict__ ads, int n, const int * __restrict__ ids, const float * __restrict__ x, int64_t ldx, int64_t n_in, int64_t a_ld,
+                       int64_t n_out, const float * base, int64_t ldb, float * y, int64_t ldy) {
+    __shared__ __align__(16) float us[SDH_LORA_MAX_RANK];
+    const int64_t t = blockIdx.x, o = (int64_t) blockIdx.y * 512 + threadIdx.x;
+    const int a = ids ? ids[t] : 0;
+    const float v = base && o < n_out ? base[t * ldb + o] : 0.0f;
+    if ((unsigned) a >= (unsigned) n) {
+        if (o < n_out && base != y) y[t * ldy + o] = v;
+        return;
+    }
+    const LoraAdapter ad = ads[a];
+    if (ad.f32) fused_u<float, VEC>(ad, x + t * ldx, n_in, a_ld, us);
+    else        fused_u<__half, VEC>(ad, x + t * ldx, n_in, a_ld, us);
     __syncthreads();
     if (o >= n_out) return;
-    if (ad.f32) expand_body<float, VEC>(ad, tile, perm, us, o, n_out, base, ldb, y, ldy);
-    else        expand_body<__half, VEC>(ad, tile, perm, us, o, n_out, base, ldb, y, ldy);
+    y[t * ldy + o] = ad.f32 ? fused_column<float>(ad, o, us, v) : fused_column<__half>(ad, o, us, v);
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
@@ -282,18 +517,21 @@ static int lora_check(const char * what, int i, const sdh_tensor & t, int64_t ne
     return SDH_OK;
 }
 
-// rows of t (F16 / F32, any strides) to dst with `ld` elements a row, as they are or widened
-static void lora_pack(const sdh_tensor & t, bool f32, uint8_t * dst, int64_t ld) {
+// t (F16 / F32, any strides) as contiguous rows, as it is or widened
+static std::vector<uint8_t> lora_rows(const sdh_tensor & t, bool f32) {
+    const size_t n0 = (size_t) t.ne[0], n1 = (size_t) t.ne[1], es = f32 ? 4 : 2;
+    std::vector<uint8_t> out(n0 * n1 * es);
     if (f32) {
         const std::vector<float> v = tensor_f32(t);
-        for (int64_t i1 = 0; i1 < t.ne[1]; ++i1) memcpy(dst + i1 * ld * 4, v.data() + i1 * t.ne[0], (size_t) t.ne[0] * 4);
-        return;
+        memcpy(out.data(), v.data(), out.size());
+        return out;
     }
-    for (int64_t i1 = 0; i1 < t.ne[1]; ++i1) {
-        const uint8_t * row = (const uint8_t *) t.data + i1 * t.nb[1];
-        if (t.nb[0] == 2) memcpy(dst + i1 * ld * 2, row, (size_t) t.ne[0] * 2);
-        else for (int64_t i0 = 0; i0 < t.ne[0]; ++i0) memcpy(dst + (i1 * ld + i0) * 2, row + i0 * t.nb[0], 2);
+    for (size_t i1 = 0; i1 < n1; ++i1) {
+        const uint8_t * row = (const uint8_t *) t.data + (int64_t) i1 * t.nb[1];
+        if (t.nb[0] == 2) memcpy(out.data() + i1 * n0 * 2, row, n0 * 2);
+        else for (size_t i0 = 0; i0 < n0; ++i0) memcpy(out.data() + (i1 * n0 + i0) * 2, row + (int64_t) i0 * t.nb[0], 2);
     }
+    return out;
 }
 
 static int lora_create(int64_t n_in, int64_t n_out, const sdh_lora_desc * d, int n, LoraSet ** out) {
@@ -302,6 +540,7 @@ static int lora_create(int64_t n_in, int64_t n_out, const sdh_lora_desc * d, int
     LoraSet l;
     l.n_in = n_in; l.n_out = n_out; l.n = n;
     l.a_ld = (n_in + 31) / 32 * 32;
+    const int64_t b_rows = (n_out + 15) / 16 * 16;
     std::vector<LoraAdapter> tab((size_t) n);
     std::vector<size_t> at_a((size_t) n), at_b((size_t) n);
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
@@ -313,13 +552,14 @@ static int lora_create(int64_t n_in, int64_t n_out, const sdh_lora_desc * d, int
         if (rc == SDH_OK) rc = lora_check("lora_b", i, d[i].b, r, n_out);
         if (rc != SDH_OK) return rc;
         LoraAdapter & a = tab[(size_t) i];
-        a.rank = (int) r; a.r_ld = (int) (r + 7) / 8 * 8; a.scale = d[i].scale;
+        a.rank = (int) r; a.r_ld = r <= 8 ? 8 : (int) (r + 15) / 16 * 16; a.scale = d[i].scale;
         a.f32 = d[i].a.type == SDH_TYPE_F32 || d[i].b.type == SDH_TYPE_F32;
         l.u_ld = std::max(l.u_ld, a.r_ld);
         l.stored_bytes += r * n_in * (d[i].a.type == SDH_TYPE_F32 ? 4 : 2) + r * n_out * (d[i].b.type == SDH_TYPE_F32 ? 4 : 2);
         const size_t es = a.f32 ? 4 : 2;
         at_a[(size_t) i] = total; total += up((size_t) (r * l.a_ld) * es);
-        at_b[(size_t) i] = total; total += up((size_t) n_out * (size_t) a.r_ld * es);
+        at_b[(size_t) i] = total; total += up((size_t) b_rows * (size_t) a.r_ld * es);
+        l.any_f32 |= a.f32 != 0;
     }
     if (const int rc = ready_on_device("sdh_lora_create")) return rc;
     SDH_HIP_CHECK(hipMalloc((void **) &l.dev, total));
@@ -330,11 +570,15 @@ static int lora_create(int64_t n_in, int64_t n_out, const sdh_lora_desc * d, int
         LoraAdapter & a = tab[(size_t) i];
         const size_t es = a.f32 ? 4 : 2;
         a.a = l.dev + at_a[(size_t) i]; a.b = l.dev + at_b[(size_t) i];
+        std::vector<uint8_t> rows = lora_rows(d[i].a, a.f32 != 0);
         buf.assign((size_t) (a.rank * l.a_ld) * es, 0);
-        lora_pack(d[i].a, a.f32 != 0, buf.data(), l.a_ld);
+        for (int64_t r = 0; r < a.rank; ++r) memcpy(&buf[(size_t) (r * l.a_ld) * es], &rows[(size_t) (r * n_in) * es], (size_t) n_in * es);
         SDH_HIP_CHECK(upload(at_a[(size_t) i], buf.size()));
-        buf.assign((size_t) n_out * (size_t) a.r_ld * es, 0);
-        lora_pack(d[i].b, a.f32 != 0, buf.data(), a.r_ld);
+        rows = lora_rows(d[i].b, a.f32 != 0);
+        buf.assign((size_t) b_rows * (size_t) a.r_ld * es, 0);
+        for (int64_t o = 0; o < n_out; ++o)
+            for (int r = 0; r < a.rank; r += 2)             // pairs of ranks stay neighbours in either fragment form
+                memcpy(&buf[(size_t) lora_b_at(o, r, a.r_ld) * es], &rows[(size_t) (o * a.rank + r) * es], (size_t) std::min(2, a.rank - r) * es);
         SDH_HIP_CHECK(upload(at_b[(size_t) i], buf.size()));
     }
     buf.resize(tab.size() * sizeof(LoraAdapter));
@@ -354,16 +598,40 @@ static int sdh_lora_create_impl(int64_t n_in, int64_t n_out, const sdh_lora_desc
     return rc;
 }
 
-template <bool VX, bool VY>
-static void lora_launch(const LoraSet & l, const LoraWs & w, const int * ids, const float * x, int64_t ldx, int64_t T,
-                        const float * base, int64_t ldb, float * y, int64_t ldy, hipStream_t s) {
+struct LoraCall { const int * ids; const float * x; int64_t ldx, T; const float * base; int64_t ldb; float * y; int64_t ldy; bool vx, vy; };
+
+template <bool PLAN>
+static void lora_two_steps(const LoraSet & l, const LoraWs & w, const LoraCall & c, hipStream_t s) {
     const LoraAdapter * ads = (const LoraAdapter *) l.dev;
     const int64_t k_split = ((l.a_ld + w.splits - 1) / w.splits + 127) / 128 * 128;
-    const unsigned splits = (unsigned) ((l.a_ld + k_split - 1) / k_split);
-    hipLaunchKernelGGL(lora_plan_kernel, dim3(1), dim3(1024), (size_t) (l.n + 1) * 12, s, ids, T, l.n, w.perm, w.tiles, w.n_tiles);
-    hipLaunchKernelGGL((lora_shrink_kernel<VX>), dim3((unsigned) w.max_tiles, splits), dim3(256), 0, s, ads, w.tiles, w.n_tiles, w.perm, x, ldx, l.n_in, l.a_ld, T, k_split, w.u, l.u_ld);
-    hipLaunchKernelGGL((lora_expand_kernel<VY>), dim3((unsigned) w.max_tiles, (unsigned) ((l.n_out + 1023) / 1024)), dim3(256), (size_t) (LT * l.u_ld) * 4, s,
-                       ads, w.tiles, w.n_tiles, w.perm, w.u, l.u_ld, (int) splits, T, l.n_out, base, ldb, y, ldy);
+    const unsigned gx = (unsigned) (PLAN ? w.max_tiles : c.T), splits = (unsigned) ((l.a_ld + k_split - 1) / k_split);
+    const auto shrink = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(gx, splits, (unsigned) ((l.u_ld + LORA_RC - 1) / LORA_RC)), dim3(256), 0, s, ads, l.n, c.ids, w.tiles, w.n_tiles, w.perm, c.x, c.ldx, l.n_in, l.a_ld, c.T, k_split, w.u, l.u_ld);
+    };
+    if (c.vx) shrink(lora_shrink_kernel<PLAN, true>); else shrink(lora_shrink_kernel<PLAN, false>);
+    int lds = 0;                                            // the most that any rank up to u_ld takes
+    for (int r : {64, 256, SDH_LORA_MAX_RANK}) lds = std::max(lds, lora_expand_tokens(std::min(r, l.u_ld)) * (std::min(r, l.u_ld) + 4));
+    lds = PLAN ? std::min(lds, w.et * (l.u_ld + 4)) : std::min(lds, 64 * (l.u_ld + 4));
+    const unsigned n_col = (unsigned) ((l.n_out + 255) / 256);
+    const auto expand = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned) (PLAN ? w.max_etiles : c.T) * n_col), dim3(256), (size_t) lds * 4, s,
+                           ads, l.n, c.ids, w.etiles, w.n_tiles + 1, w.perm, w.u, l.u_ld, (int) splits, c.T, l.n_out, c.base, c.ldb, c.y, c.ldy);
+    };
+    if (c.vy) expand(lora_expand_kernel<PLAN, true>); else expand(lora_expand_kernel<PLAN, false>);
+}
+
+static void lora_launch(const LoraSet & l, const LoraWs & w, const LoraCall & c, hipStream_t s) {
+    // one launch while every workgroup can read all of A in about the time of a launch: 128 KB of F16 7.5 us, two launches 10.8 us
+    if (c.T <= 4 && (int64_t) l.u_ld * l.a_ld * (l.any_f32 ? 4 : 2) <= (256 << 10)) {
+        const auto fused = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned) c.T, (unsigned) ((l.n_out + 511) / 512)), dim3(512), 0, s, (const LoraAdapter *) l.dev, l.n, c.ids, c.x, c.ldx, l.n_in, l.a_ld, l.n_out, c.base, c.ldb, c.y, c.ldy);
+        };
+        if (c.vx) fused(lora_fused_kernel<true>); else fused(lora_fused_kernel<false>);
+    } else if (c.T <= 64) lora_two_steps<false>(l, w, c, s);
+    else {
+        hipLaunchKernelGGL(lora_plan_kernel, dim3(1), dim3(1024), (size_t) (l.n + 1) * 8, s, c.ids, c.T, l.n, w.perm, w.tiles, w.etiles, w.et, w.n_tiles);
+        lora_two_steps<true>(l, w, c, s);
+    }
 }
 
 static int sdh_lora_apply_impl(const sdh_lora * h, const int32_t * ids, const float * x, int64_t ldx, int64_t T,
@@ -383,11 +651,7 @@ static int sdh_lora_apply_impl(const sdh_lora * h, const int32_t * ids, const fl
     if (ws_bytes < w.bytes) { set_error("%s: the workspace holds %lld bytes, %lld are needed", who, (long long) ws_bytes, (long long) w.bytes); return SDH_ERR_INVALID; }
     const bool vx = aligned(x, 16) && ldx % 4 == 0;
     const bool vy = aligned(y, 16) && ldy % 4 == 0 && l.n_out % 4 == 0 && (!base || (aligned(base, 16) && ldb % 4 == 0));
-    hipStream_t s = (hipStream_t) stream;
-    if (vx && vy)      lora_launch<true, true>(l, w, ids, x, ldx, T, base, ldb, y, ldy, s);
-    else if (vx)       lora_launch<true, false>(l, w, ids, x, ldx, T, base, ldb, y, ldy, s);
-    else if (vy)       lora_launch<false, true>(l, w, ids, x, ldx, T, base, ldb, y, ldy, s);
-    else               lora_launch<false, false>(l, w, ids, x, ldx, T, base, ldb, y, ldy, s);
+    lora_launch(l, w, LoraCall{ids, x, ldx, T, base, ldb, y, ldy, vx, vy}, (hipStream_t) stream);
     SDH_HIP_CHECK(hipGetLastError());
     return SDH_OK;
 }
