@@ -46,7 +46,6 @@ struct LoraSet {
 };
 
 constexpr int LT = 32;                     // tokens per tile of the shrink kernel
-constexpr int ET = 128;                    // ... of the expand kernel, where there are many (else 32)
 constexpr int LORA_RC = 32;                // ranks per workgroup of the shrink kernel
 
 struct LoraTile { int adapter, start, count, pad; };       // adapter -1: none
@@ -60,11 +59,11 @@ struct LoraWs {
 static LoraWs lora_ws(const LoraSet & l, int64_t T, uint8_t * base) {
     LoraWs w{};
     auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
-    w.et = T >= 2048 && l.u_ld <= 64 ? ET : LT;
+    w.et = 16;
     w.max_tiles = (T + LT - 1) / LT + std::min<int64_t>(T, l.n + 1);
     w.max_etiles = (T + w.et - 1) / w.et + std::min<int64_t>(T, l.n + 1);
-    // K splits of the shrink step: about four workgroups per CU, at least 128 columns each
-    const int64_t tiles = (T + LT - 1) / LT, most = std::max<int64_t>(1, l.n_in / 128);
+    // K splits of the shrink step: about four workgroups per CU, 512 columns each (four steps of its four waves) or a multiple
+    const int64_t tiles = (T + LT - 1) / LT, most = (l.n_in + 511) / 512;
     w.splits = (int) std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, most), 1024 / tiles));
     int64_t at = 0;
     w.perm = (int *) (base + at);         at += up(T * 4);
@@ -208,6 +207,47 @@ __device__ __forceinline__ int lora_tokens(const LoraTile * tiles, const int * n
 // A workgroup: one tile, LORA_RC ranks, one split of the columns; its four waves take steps of 32 columns in turn and are joined in
 // LDS. 16x16x4 operands: row / column lane & 15, k = lane >> 4; in a step lane group g holds columns 4 g .. 4 g + 3 and 16 + 4 g ..,
 // so that a load instruction takes 64 consecutive bytes of 16 tokens.
+// NS: groups of 16 tokens, NJ: fragments of 16 ranks. Steps of 32 columns k, k + 128, ... below k_end; CHECK: some columns of a step
+// may lie past n_in (or x is not aligned). Without branches in the loop the loads of several steps are in flight.
+template <typename W, int NS, int NJ, bool CHECK>
+__device__ __forceinline__ void shrink_steps(const float * const (&xr)[2], const W * const (&ar)[LORA_RC / 16], int64_t n_in, int64_t k, int64_t k_end, v4f (&acc)[2][LORA_RC / 16]) {
+    constexpr int U = CHECK ? 1 : 4;
+    const int g = ((int) threadIdx.x & 63) >> 4;
+    const auto step = [&](int64_t at, float (&xv)[NS][2][4], float (&av)[NJ][2][4]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t c = at + 16 * h + 4 * g;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) { if constexpr (CHECK) load4x<false>(xr[i], c, n_in, xv[i][h]); else load_n<4>(xr[i] + c, xv[i][h]); }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) load_n<4>(ar[j] + c, av[j][h]);
+        }
+    };
+    const auto mult = [&](const float (&xv)[NS][2][4], const float (&av)[NJ][2][4]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[i][h][q], av[j][h][q], acc[i][j], 0, 0, 0);
+    };
+    for (; k + 128 * (U - 1) < k_end; k += 128 * U) {
+        float xv[U][NS][2][4], av[U][NJ][2][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u) step(k + 128 * u, xv[u], av[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) mult(xv[u], av[u]);
+    }
+    if constexpr (U > 1)
+        for (; k < k_end; k += 128) {
+            float xv[NS][2][4], av[NJ][2][4];
+            step(k, xv, av);
+            mult(xv, av);
+        }
+}
+
 template <typename W, bool VEC>
 __device__ void shrink_tile(const LoraAdapter & ad, const int * list, int count, int rc, const float * x, int64_t ldx, int64_t n_in, int64_t a_ld,
                             int64_t k_begin, int64_t k_end, float * u, int u_ld, float (*red)[LT][LORA_RC + 1]) {
@@ -217,8 +257,6 @@ __device__ void shrink_tile(const LoraAdapter & ad, const int * list, int count,
     const float * xr[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) xr[i] = x + (int64_t) list[min(16 * i + m, count - 1)] * ldx;
-    const bool two = count > 16;
-    const int nj = min(NJ, (ad.rank - rc + 15) / 16);
     const W * ar[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) ar[j] = A + (int64_t) min(rc + 16 * j + m, ad.rank - 1) * a_ld;
@@ -227,29 +265,16 @@ __device__ void shrink_tile(const LoraAdapter & ad, const int * list, int count,
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t k = k_begin + 32 * wave; k < k_end; k += 128) {
-        float xv[2][2][4], av[NJ][2][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t at = k + 16 * h + 4 * g;
-            load4x<VEC>(xr[0], at, n_in, xv[0][h]);
-            if (two) load4x<VEC>(xr[1], at, n_in, xv[1][h]);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) if (j < nj) load_n<4>(ar[j] + at, av[j][h]);
-        }
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            if (j < nj) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        acc[0][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[0][h][q], av[j][h][q], acc[0][j], 0, 0, 0);
-                        if (two) acc[1][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[1][h][q], av[j][h][q], acc[1][j], 0, 0, 0);
-                    }
-            }
-        }
+    const bool two = count > 16, more = ad.rank - rc > 16;
+    const int64_t k = k_begin + 32 * wave, whole = VEC ? min(k_end, n_in / 32 * 32) : 0;      // from `whole` on with checks
+    if (k < whole) {
+        if (two && more) shrink_steps<W, 2, 2, false>(xr, ar, n_in, k, whole, acc);
+        else if (two)    shrink_steps<W, 2, 1, false>(xr, ar, n_in, k, whole, acc);
+        else if (more)   shrink_steps<W, 1, 2, false>(xr, ar, n_in, k, whole, acc);
+        else             shrink_steps<W, 1, 1, false>(xr, ar, n_in, k, whole, acc);
     }
+    const int64_t rest = max(k, k + (whole - k + 127) / 128 * 128);                            // this wave's first step at or past it
+    if (rest < k_end) shrink_steps<W, 2, 2, true>(xr, ar, n_in, rest, k_end, acc);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -289,89 +314,66 @@ void lora_shrink_kernel(const LoraAdapter * __restrict__ ads, int n, const int *
 }
 
 // ---- y[token][o] = base[token][o] + sum_r (scale sum_split u[split][token][r]) B[o][r] ----------------------------------
-template <bool VEC>
-__device__ __forceinline__ v4f row_load4(const float * p, int o, int n) {
-    if constexpr (VEC) return *reinterpret_cast<const v4f *>(p + o);
-    v4f v = {p[o], 0.0f, 0.0f, 0.0f};
-    if (o + 1 < n) v[1] = p[o + 1];
-    if (o + 2 < n) v[2] = p[o + 2];
-    if (o + 3 < n) v[3] = p[o + 3];
-    return v;
-}
-template <bool VEC>
-__device__ __forceinline__ void row_store4(float * p, int o, int n, v4f v) {
-    if constexpr (VEC) { *reinterpret_cast<v4f *>(p + o) = v; return; }
-    p[o] = v[0];
-    if (o + 1 < n) p[o + 1] = v[1];
-    if (o + 2 < n) p[o + 2] = v[2];
-    if (o + 3 < n) p[o + 3] = v[3];
-}
-// A wave owns 64 columns (four fragments of 16) and takes its tokens 16 at a time; the next 16 tokens' base is asked for before the
-// present ones are multiplied. The result has column 4 (lane >> 4) + i in register i and token lane & 15: base and y are 16 bytes per
-// lane, 64 consecutive bytes of 16 tokens per instruction (a copy in this order runs at 5.1 TB/s, in whole rows at 5.2 to 5.6).
+// A wave owns 64 columns (four fragments of 16) and takes its tokens 16 at a time. u is the A operand, so the result has token
+// 4 (lane >> 4) + i in register i and column lane & 15: a load or store of base and y takes 64 consecutive bytes of 4 tokens, four
+// cache accesses. (The other way round a lane has four columns and an instruction moves 16 bytes per lane, but neighbouring lanes
+// are in different rows, which costs an access per lane: 107 us against 92 for the 4096 tokens below.)
 struct ExpandWave {
     const int * list; int count;           // tokens
     const float * us; int us_ld;           // scale * u of them, in LDS
     int64_t o0, n_out;                     // columns, o0 the same in all lanes
     const float * base; int64_t ldb; float * y; int64_t ldy;
 };
-template <bool VEC>
-__device__ __forceinline__ void expand_base(const ExpandWave & e, int t0, v4f (&acc)[4]) {
-    const int lane = threadIdx.x & 63;
+__device__ __forceinline__ void expand_base(const ExpandWave & e, v4f (&acc)[4]) {
+    const int m = (int) threadIdx.x & 15, t = ((int) threadIdx.x & 63) >> 4 << 2;
+    const int left = (int) min(e.n_out - e.o0, (int64_t) 64) - m;
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (!e.base) return;
-    const float * p = e.base + e.list[min(t0 + (lane & 15), e.count - 1)] * e.ldb + e.o0 + 4 * (lane >> 4);
-    const int left = (int) min(e.n_out - e.o0, (int64_t) 64) - 4 * (lane >> 4);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) if (16 * j < left) acc[j] = row_load4<VEC>(p, 16 * j, left);
+    for (int i = 0; i < 4; ++i) {
+        const float * p = e.base + e.list[min(t + i, e.count - 1)] * e.ldb + e.o0 + m;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (16 * j < left && t + i < e.count) acc[j][i] = p[16 * j];
+    }
 }
-template <bool VEC>
-__device__ __forceinline__ void expand_store(const ExpandWave & e, int t0, const v4f (&acc)[4]) {
-    const int lane = threadIdx.x & 63, t = t0 + (lane & 15);
-    if (t >= e.count) return;
-    float * p = e.y + e.list[t] * e.ldy + e.o0 + 4 * (lane >> 4);
-    const int left = (int) min(e.n_out - e.o0, (int64_t) 64) - 4 * (lane >> 4);
+__device__ __forceinline__ void expand_store(const ExpandWave & e, const v4f (&acc)[4]) {
+    const int m = (int) threadIdx.x & 15, t = ((int) threadIdx.x & 63) >> 4 << 2;
+    const int left = (int) min(e.n_out - e.o0, (int64_t) 64) - m;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) if (16 * j < left) row_store4<VEC>(p, 16 * j, left, acc[j]);
+    for (int i = 0; i < 4; ++i)
+        if (t + i < e.count) {
+            float * p = e.y + e.list[t + i] * e.ldy + e.o0 + m;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (16 * j < left) p[16 * j] = acc[j][i];
+        }
 }
 // KQ: ranks per lane of a fragment: 4, or 2 for the one of 8 ranks
-template <typename W, int KQ, bool VEC>
-__device__ __forceinline__ void expand_wave(const ExpandWave & e, const W * b_all, int r_ld, v4f (&next)[4]) {
+template <typename W, int KQ>
+__device__ __forceinline__ void expand_mult(const ExpandWave & e, const W * b_all, int r_ld, v4f (&acc)[4]) {
     const int lane = threadIdx.x & 63;
     const int last = (int) ((e.n_out - 1) >> 4), tile = (int) (e.o0 >> 4);
+    const float * ur = e.us + (lane & 15) * e.us_ld + KQ * (lane >> 4);
 #pragma unroll 1
-    for (int t0 = 0; t0 < e.count; t0 += 16) {
-        v4f acc[4];
+    for (int r = 0; r < r_ld; r += 4 * KQ) {
+        float b[4][KQ], uv[KQ];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = next[j];
-        if (t0 + 16 < e.count) expand_base<VEC>(e, t0 + 16, next);
-        const float * ur = e.us + (t0 + (lane & 15)) * e.us_ld + KQ * (lane >> 4);
-#pragma unroll 1
-        for (int r = 0; r < r_ld; r += 4 * KQ) {
-            float b[4][KQ], uv[KQ];
+        for (int j = 0; j < 4; ++j) load_n<KQ>(b_all + ((int64_t) min(tile + j, last) * r_ld + r) * 16 + KQ * lane, b[j]);
+        load_n<KQ>(ur + r, uv);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) load_n<KQ>(b_all + ((int64_t) min(tile + j, last) * r_ld + r) * 16 + KQ * lane, b[j]);
-            load_n<KQ>(ur + r, uv);
+        for (int q = 0; q < KQ; ++q)
 #pragma unroll
-            for (int q = 0; q < KQ; ++q)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[j][q], uv[q], acc[j], 0, 0, 0);
-        }
-        expand_store<VEC>(e, t0, acc);
+            for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(uv[q], b[j][q], acc[j], 0, 0, 0);
     }
 }
 
-// tokens whose u is in LDS at a time: 34 KB at most
-__host__ __device__ constexpr int lora_expand_tokens(int r_ld) { return r_ld > 256 ? 16 : r_ld > 64 ? 32 : 128; }
-
-template <bool PLAN, bool VEC>
-__global__ __launch_bounds__(256, 4)
+template <bool PLAN>
+__global__ __launch_bounds__(256, 6)
 void lora_expand_kernel(const LoraAdapter * __restrict__ ads, int n, const int * __restrict__ ids, const LoraTile * __restrict__ tiles, const int * __restrict__ n_tiles,
                         const int * __restrict__ perm, const float * __restrict__ u, int u_ld, int splits, int64_t T, int64_t n_out,
                         const float * base, int64_t ldb, float * y, int64_t ldy) {
-    extern __shared__ __align__(16) float us[];             // [lora_expand_tokens][r_ld + 4]
-    __shared__ int lists[4][PLAN ? ET : 64];
+    extern __shared__ __align__(16) float us[];             // [16][r_ld + 4]
+    __shared__ int lists[4][PLAN ? LT : 64];
     // neighbouring workgroups take neighbouring columns of the same tokens
     const int n_col = (int) ((n_out + 255) >> 8), at = (int) (blockIdx.x / (unsigned) n_col), col = (int) (blockIdx.x % (unsigned) n_col);
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
@@ -379,49 +381,49 @@ void lora_expand_kernel(const LoraAdapter * __restrict__ ads, int n, const int *
     int a = -1;
     const int all = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, at, list, &a);
     if (!all || (a < 0 && base == y)) return;
-    ExpandWave e{list, all, us, 0, (int64_t) col * 256 + 64 * wave, n_out, base, ldb, y, ldy};
-    v4f next[4];
-    if (a < 0) {                                            // no adapter: y is the base
-#pragma unroll 1
-        for (int t0 = 0; t0 < all; t0 += 16) {
-            expand_base<VEC>(e, t0, next);
-            expand_store<VEC>(e, t0, next);
-        }
-        return;
-    }
-    const LoraAdapter ad = ads[a];
+    ExpandWave e{list, all, us, 0, 0, n_out, base, ldb, y, ldy};
+    LoraAdapter ad{};
+    if (a >= 0) ad = ads[a];
     e.us_ld = ad.r_ld + 4;                                  // 16-byte rows that start on different banks
-    const int step = lora_expand_tokens(ad.r_ld), n4 = ad.r_ld >> 2;
-    for (int t0 = 0; t0 < all; t0 += step) {
+    const int n4 = ad.r_ld >> 2;
+#pragma unroll 1
+    for (int t0 = 0; t0 < all; t0 += 16) {
         e.list = list + t0;
-        e.count = min(step, all - t0);
-        expand_base<VEC>(e, 0, next);
-        if (t0) __syncthreads();
+        e.count = min(16, all - t0);
+        int64_t o0 = (int64_t) col * 256 + 64 * wave;
+        asm volatile("" : "+s"(o0));                        // addresses are formed here, not kept across (and spilled) by the loop
+        e.o0 = o0;
+        v4f acc[4];
+        expand_base(e, acc);                        // asked for first: it takes the longest way
+        if (a >= 0) {                                       // no adapter: y is the base
+            if (t0) __syncthreads();
 #pragma unroll 1
-        for (int i = threadIdx.x; i < (e.count + 15) / 16 * 16 * n4; i += 256) {
-            const int t = i / n4, r = 4 * (i - t * n4);
-            v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (t < e.count) {
-                const float * up = u + (int64_t) e.list[t] * u_ld + r;
+            for (int i = threadIdx.x; i < 16 * n4; i += 256) {
+                const int t = i / n4, r = 4 * (i - t * n4);
+                v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (t < e.count) {
+                    const float * up = u + (int64_t) e.list[t] * u_ld + r;
 #pragma unroll 1
-                for (int s0 = 0; s0 < splits; s0 += 4) {    // four at a time in flight; past the last split: the last one, not added
-                    v4f p[4];
+                    for (int s0 = 0; s0 < splits; s0 += 4) {            // four at a time in flight; past the last split: the last one, not added
+                        v4f p[4];
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) p[s] = *reinterpret_cast<const v4f *>(up + min(s0 + s, splits - 1) * T * u_ld);
+                        for (int s = 0; s < 4; ++s) p[s] = *reinterpret_cast<const v4f *>(up + min(s0 + s, splits - 1) * T * u_ld);
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) if (s0 + s < splits) v += p[s];
+                        for (int s = 0; s < 4; ++s) if (s0 + s < splits) v += p[s];
+                    }
                 }
+                *reinterpret_cast<v4f *>(us + t * e.us_ld + r) = ad.scale * v;
             }
-            *reinterpret_cast<v4f *>(us + t * e.us_ld + r) = ad.scale * v;
+            __syncthreads();
+            if (ad.f32) {
+                if (ad.r_ld == 8) expand_mult<float, 2>(e, (const float *) ad.b, ad.r_ld, acc);
+                else              expand_mult<float, 4>(e, (const float *) ad.b, ad.r_ld, acc);
+            } else {
+                if (ad.r_ld == 8) expand_mult<__half, 2>(e, (const __half *) ad.b, ad.r_ld, acc);
+                else              expand_mult<__half, 4>(e, (const __half *) ad.b, ad.r_ld, acc);
+            }
         }
-        __syncthreads();
-        const auto wave = [&](auto type) {
-            using W = decltype(type);
-            const W * B = (const W *) ad.b;
-            if (ad.r_ld == 8) expand_wave<W, 2, VEC>(e, B, ad.r_ld, next);
-            else              expand_wave<W, 4, VEC>(e, B, ad.r_ld, next);
-        };
-        if (ad.f32) wave(float{}); else wave(__half{});
+        expand_store(e, acc);
     }
 }
 
@@ -598,26 +600,23 @@ static int sdh_lora_create_impl(int64_t n_in, int64_t n_out, const sdh_lora_desc
     return rc;
 }
 
-struct LoraCall { const int * ids; const float * x; int64_t ldx, T; const float * base; int64_t ldb; float * y; int64_t ldy; bool vx, vy; };
+struct LoraCall { const int * ids; const float * x; int64_t ldx, T; const float * base; int64_t ldb; float * y; int64_t ldy; bool vx; };
 
 template <bool PLAN>
 static void lora_two_steps(const LoraSet & l, const LoraWs & w, const LoraCall & c, hipStream_t s) {
     const LoraAdapter * ads = (const LoraAdapter *) l.dev;
-    const int64_t k_split = ((l.a_ld + w.splits - 1) / w.splits + 127) / 128 * 128;
+    const int64_t k_split = ((l.a_ld + w.splits - 1) / w.splits + 511) / 512 * 512;
     const unsigned gx = (unsigned) (PLAN ? w.max_tiles : c.T), splits = (unsigned) ((l.a_ld + k_split - 1) / k_split);
     const auto shrink = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(gx, splits, (unsigned) ((l.u_ld + LORA_RC - 1) / LORA_RC)), dim3(256), 0, s, ads, l.n, c.ids, w.tiles, w.n_tiles, w.perm, c.x, c.ldx, l.n_in, l.a_ld, c.T, k_split, w.u, l.u_ld);
     };
     if (c.vx) shrink(lora_shrink_kernel<PLAN, true>); else shrink(lora_shrink_kernel<PLAN, false>);
-    int lds = 0;                                            // the most that any rank up to u_ld takes
-    for (int r : {64, 256, SDH_LORA_MAX_RANK}) lds = std::max(lds, lora_expand_tokens(std::min(r, l.u_ld)) * (std::min(r, l.u_ld) + 4));
-    lds = PLAN ? std::min(lds, w.et * (l.u_ld + 4)) : std::min(lds, 64 * (l.u_ld + 4));
     const unsigned n_col = (unsigned) ((l.n_out + 255) / 256);
     const auto expand = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned) (PLAN ? w.max_etiles : c.T) * n_col), dim3(256), (size_t) lds * 4, s,
+        hipLaunchKernelGGL(kernel, dim3((unsigned) (PLAN ? w.max_etiles : c.T) * n_col), dim3(256), (size_t) (16 * (l.u_ld + 4)) * 4, s,
                            ads, l.n, c.ids, w.etiles, w.n_tiles + 1, w.perm, w.u, l.u_ld, (int) splits, c.T, l.n_out, c.base, c.ldb, c.y, c.ldy);
     };
-    if (c.vy) expand(lora_expand_kernel<PLAN, true>); else expand(lora_expand_kernel<PLAN, false>);
+    expand(lora_expand_kernel<PLAN>);
 }
 
 static void lora_launch(const LoraSet & l, const LoraWs & w, const LoraCall & c, hipStream_t s) {
@@ -650,8 +649,7 @@ static int sdh_lora_apply_impl(const sdh_lora * h, const int32_t * ids, const fl
     const LoraWs w = lora_ws(l, T, (uint8_t *) ws);
     if (ws_bytes < w.bytes) { set_error("%s: the workspace holds %lld bytes, %lld are needed", who, (long long) ws_bytes, (long long) w.bytes); return SDH_ERR_INVALID; }
     const bool vx = aligned(x, 16) && ldx % 4 == 0;
-    const bool vy = aligned(y, 16) && ldy % 4 == 0 && l.n_out % 4 == 0 && (!base || (aligned(base, 16) && ldb % 4 == 0));
-    lora_launch(l, w, LoraCall{ids, x, ldx, T, base, ldb, y, ldy, vx, vy}, (hipStream_t) stream);
+    lora_launch(l, w, LoraCall{ids, x, ldx, T, base, ldb, y, ldy, vx}, (hipStream_t) stream);
     SDH_HIP_CHECK(hipGetLastError());
     return SDH_OK;
 }
