@@ -20,9 +20,10 @@ namespace sdh {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 
-// A: [rank][a_ld], columns past n_in zero. B in the order of the expand kernel's fragments: per 16 output rows, per 16 ranks,
-// [lane][4] with row lane & 15 and ranks 4 (lane >> 4) ..; up to rank 8 one [lane][2] with ranks 2 (lane >> 4) ..; rows past n_out
-// and ranks past `rank` zero.
+// A in the order of the shrink kernel's fragments: per 16 ranks (8 up to rank 8), per 32 columns, lane' = 16 (or 8) * group + rank with
+// columns 4 group .. and 16 + 4 group ..: eight consecutive halves, or four floats in each of two halves of the block. B in the order of the expand kernel's fragments: per 16 output rows, per 16 ranks,
+// [lane][4] with row lane & 15 and ranks 4 (lane >> 4) ..; up to rank 8 one [lane][2] with ranks 2 (lane >> 4) ... Whatever lies past
+// n_in, n_out or `rank` is zero.
 struct LoraAdapter {
     const void * a;
     const void * b;
@@ -30,7 +31,14 @@ struct LoraAdapter {
     int rank, r_ld, f32;   // r_ld: 8, or rank rounded up to 16
 };
 
-__host__ __device__ inline int64_t lora_b_at(int64_t o, int r, int r_ld) {
+inline int64_t lora_a_at(int64_t k, int r, int r_ld, int64_t a_ld, bool f32) {
+    const int rw = r_ld == 8 ? 8 : 16, h = (int) (k >> 4) & 1, g = (int) (k >> 2) & 3, q = (int) k & 3;
+    const int64_t block = ((r / rw) * (a_ld / 32) + (k >> 5)) * rw * 32;
+    const int lane = g * rw + r % rw;
+    return block + (f32 ? h * rw * 16 + lane * 4 + q : lane * 8 + h * 4 + q);
+}
+
+inline int64_t lora_b_at(int64_t o, int r, int r_ld) {
     const int64_t tile = (o >> 4) * 16 * r_ld;
     const int row = (int) (o & 15);
     if (r_ld == 8) return tile + (((r >> 1) * 16 + row) << 1) + (r & 1);
@@ -62,9 +70,10 @@ static LoraWs lora_ws(const LoraSet & l, int64_t T, uint8_t * base) {
     w.et = 16;
     w.max_tiles = (T + LT - 1) / LT + std::min<int64_t>(T, l.n + 1);
     w.max_etiles = (T + w.et - 1) / w.et + std::min<int64_t>(T, l.n + 1);
-    // K splits of the shrink step: about four workgroups per CU, 512 columns each (four steps of its four waves) or a multiple
-    const int64_t tiles = (T + LT - 1) / LT, most = (l.n_in + 511) / 512;
-    w.splits = (int) std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, most), 1024 / tiles));
+    // K splits of the shrink step: about four workgroups per CU, at least 256 columns each; a power of two, so that from 8 on a split
+    // stays on one XCD (round-robin dispatch) with its slice of A for all tiles
+    const int64_t tiles = (T + LT - 1) / LT;
+    for (w.splits = 1; w.splits < 16 && 2 * w.splits * tiles <= 1024 && l.a_ld / (2 * w.splits) >= 256;) w.splits *= 2;
     int64_t at = 0;
     w.perm = (int *) (base + at);         at += up(T * 4);
     w.tiles = (LoraTile *) (base + at);   at += up(w.max_tiles * (int64_t) sizeof(LoraTile));
@@ -142,20 +151,6 @@ void lora_plan_kernel(const int * __restrict__ ids, int64_t T, int n, int * __re
     }
 }
 
-// eight consecutive weights as F32
-__device__ __forceinline__ void load8(const __half * p, float (&v)[8]) {
-    const uint4 q = *reinterpret_cast<const uint4 *>(p);
-    const unsigned w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        __half2 h; __builtin_memcpy(&h, &w[i], 4);
-        v[2 * i] = __low2float(h); v[2 * i + 1] = __high2float(h);
-    }
-}
-__device__ __forceinline__ void load8(const float * p, float (&v)[8]) {
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
 template <int N> __device__ __forceinline__ void load_n(const __half * p, float (&v)[N]) {
     __half h[N];
     __builtin_memcpy(h, __builtin_assume_aligned(p, 2 * N), 2 * N);
@@ -164,19 +159,30 @@ template <int N> __device__ __forceinline__ void load_n(const __half * p, float 
 }
 template <int N> __device__ __forceinline__ void load_n(const float * p, float (&v)[N]) { __builtin_memcpy(v, __builtin_assume_aligned(p, 4 * N), 4 * N); }
 
-// eight consecutive activations; past n: zero
-template <bool VEC>
-__device__ __forceinline__ void load8x(const float * p, int64_t k, int64_t n, float (&v)[8]) {
-    if (VEC && k + 8 <= n) { load8(p + k, v); return; }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < n ? p[k + i] : 0.0f;
-}
+// a lane's eight values of a fragment of A, as stored; `at`: the block, `lane`: lane'
+template <typename W> struct AFrag;
+template <> struct AFrag<__half> {
+    __half v[8];
+    __device__ __forceinline__ void load(const __half * at, int, int lane) { __builtin_memcpy(v, __builtin_assume_aligned(at + lane * 8, 16), 16); }
+    __device__ __forceinline__ float get(int h, int q) const { return __half2float(v[4 * h + q]); }
+};
+template <> struct AFrag<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float * at, int rw, int lane) {
+        __builtin_memcpy(v, __builtin_assume_aligned(at + lane * 4, 16), 16);
+        __builtin_memcpy(v + 4, __builtin_assume_aligned(at + rw * 16 + lane * 4, 16), 16);
+    }
+    __device__ __forceinline__ float get(int h, int q) const { return v[4 * h + q]; }
+};
 
-template <bool VEC>
-__device__ __forceinline__ void load4x(const float * p, int64_t k, int64_t n, float (&v)[4]) {
-    if (VEC && k + 4 <= n) { load_n<4>(p + k, v); return; }
+// four consecutive activations (4-byte aligned; a 16-byte load takes that); CHECK: past n zero
+template <bool CHECK>
+__device__ __forceinline__ v4f load4x(const float * p, int64_t k, int64_t n) {
+    v4f v;
+    if (!CHECK || k + 4 <= n) { __builtin_memcpy(&v, p + k, 16); return v; }
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = k + i < n ? p[k + i] : 0.0f;
+    return v;
 }
 
 // ---- the tokens of a workgroup --------------------------------------------------------------------------------------
@@ -205,111 +211,135 @@ __device__ __forceinline__ int lora_tokens(const LoraTile * tiles, const int * n
 
 // ---- u[split][token][r] = sum over the split's columns of A[r][k] x[token][k] -------------------------------------------
 // A workgroup: one tile, LORA_RC ranks, one split of the columns; its four waves take steps of 32 columns in turn and are joined in
-// LDS. 16x16x4 operands: row / column lane & 15, k = lane >> 4; in a step lane group g holds columns 4 g .. 4 g + 3 and 16 + 4 g ..,
-// so that a load instruction takes 64 consecutive bytes of 16 tokens.
-// NS: groups of 16 tokens, NJ: fragments of 16 ranks. Steps of 32 columns k, k + 128, ... below k_end; CHECK: some columns of a step
-// may lie past n_in (or x is not aligned). Without branches in the loop the loads of several steps are in flight.
+// LDS. 16x16x4 operands: row / column lane & 15, k = lane >> 4; in a step lane group g holds columns 4 g .. 4 g + 3 and 16 + 4 g ...
+// Fragments of x read from memory would put neighbouring lanes into different rows, a cache access per lane (what bounded this step:
+// 28 us for the 512 tokens below): a wave loads 128 consecutive bytes of 8 rows per instruction and turns them in a corner of LDS of
+// its own (16-byte chunks of a row at chunk ^ ((row >> 1) & 7): no bank twice; LDS works in order within a wave, so no barrier).
+// A is stored as its fragments are.
+constexpr int SU = 2;                                       // steps in flight per wave
+
+// NS: groups of 16 tokens, NJ: fragments of A. Steps k, k + 128, ... below k_end; CHECK: some columns of a step may lie past n_in.
 template <typename W, int NS, int NJ, bool CHECK>
-__device__ __forceinline__ void shrink_steps(const float * const (&xr)[2], const W * const (&ar)[LORA_RC / 16], int64_t n_in, int64_t k, int64_t k_end, v4f (&acc)[2][LORA_RC / 16]) {
-    constexpr int U = CHECK ? 1 : 4;
-    const int g = ((int) threadIdx.x & 63) >> 4;
-    const auto step = [&](int64_t at, float (&xv)[NS][2][4], float (&av)[NJ][2][4]) {
+__device__ __forceinline__ void shrink_steps(const float * const (&xr)[4], const W * A, int rw, int64_t tile_ld, int64_t n_in, int64_t k, int64_t k_end, v4f * turn, v4f (&acc)[2][LORA_RC / 16]) {
+    constexpr int U = CHECK ? 1 : SU;
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, lr = lane >> 3, lc = lane & 7;
+    const int al = g * rw + (m & (rw - 1)), st = lr * 8 + (lc ^ ((lr >> 1) & 7)), key = (m >> 1) & 7;
+    v4f xn[U][2 * NS];
+    AFrag<W> an[U][NJ];
+    const auto load = [&](int64_t k0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t c = at + 16 * h + 4 * g;
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = CHECK ? k0 : min(k0 + 128 * u, k_end - 32);       // past the end: in bounds and not used
 #pragma unroll
-            for (int i = 0; i < NS; ++i) { if constexpr (CHECK) load4x<false>(xr[i], c, n_in, xv[i][h]); else load_n<4>(xr[i] + c, xv[i][h]); }
+            for (int i = 0; i < 2 * NS; ++i) xn[u][i] = load4x<CHECK>(xr[i], at + 4 * lc, n_in);
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) load_n<4>(ar[j] + c, av[j][h]);
+            for (int j = 0; j < NJ; ++j) an[u][j].load(A + j * tile_ld + at * rw, rw, al);
         }
     };
-    const auto mult = [&](const float (&xv)[NS][2][4], const float (&av)[NJ][2][4]) {
+    load(k);
+    for (; k < k_end; k += 128 * U) {
+        AFrag<W> ac[U][NJ];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int i = 0; i < 2 * NS; ++i) turn[u * 256 + i * 64 + (i & 1 ? st ^ 4 : st)] = xn[u][i];     // rows 8 i + lr: 8 more rows flip bit 2 of the key
 #pragma unroll
-                for (int j = 0; j < NJ; ++j)
+            for (int j = 0; j < NJ; ++j) ac[u][j] = an[u][j];
+        }
+        if (k + 128 * U < k_end) load(k + 128 * U);
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                    for (int i = 0; i < NS; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[i][h][q], av[j][h][q], acc[i][j], 0, 0, 0);
-    };
-    for (; k + 128 * (U - 1) < k_end; k += 128 * U) {
-        float xv[U][NS][2][4], av[U][NJ][2][4];
+        for (int u = 0; u < U; ++u) {
+            if (u && k + 128 * u >= k_end) break;
+            v4f xv[NS][2];
 #pragma unroll
-        for (int u = 0; u < U; ++u) step(k + 128 * u, xv[u], av[u]);
+            for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int u = 0; u < U; ++u) mult(xv[u], av[u]);
+                for (int h = 0; h < 2; ++h) xv[i][h] = turn[u * 256 + (16 * i + m) * 8 + ((4 * h + g) ^ key)];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int i = 0; i < NS; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[i][h][q], ac[u][j].get(h, q), acc[i][j], 0, 0, 0);
+        }
+        __builtin_amdgcn_wave_barrier();
     }
-    if constexpr (U > 1)
-        for (; k < k_end; k += 128) {
-            float xv[NS][2][4], av[NJ][2][4];
-            step(k, xv, av);
-            mult(xv, av);
-        }
 }
 
-template <typename W, bool VEC>
+template <typename W>
 __device__ void shrink_tile(const LoraAdapter & ad, const int * list, int count, int rc, const float * x, int64_t ldx, int64_t n_in, int64_t a_ld,
-                            int64_t k_begin, int64_t k_end, float * u, int u_ld, float (*red)[LT][LORA_RC + 1]) {
+                            int64_t k_begin, int64_t k_end, float * u, int u_ld, v4f * lds) {
     constexpr int NJ = LORA_RC / 16;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
-    const W * A = (const W *) ad.a;
-    const float * xr[2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
+    const int rw = ad.r_ld == 8 ? 8 : 16;
+    const int64_t tile_ld = a_ld * rw;
+    const W * A = (const W *) ad.a + (rc / 16) * tile_ld;
+    v4f * turn = lds + wave * SU * 256;
+    const float * xr[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) xr[i] = x + (int64_t) list[min(16 * i + m, count - 1)] * ldx;
-    const W * ar[NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) ar[j] = A + (int64_t) min(rc + 16 * j + m, ad.rank - 1) * a_ld;
+    for (int i = 0; i < 4; ++i) xr[i] = x + (int64_t) list[min(8 * i + (lane >> 3), count - 1)] * ldx;
     v4f acc[2][NJ];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     const bool two = count > 16, more = ad.rank - rc > 16;
-    const int64_t k = k_begin + 32 * wave, whole = VEC ? min(k_end, n_in / 32 * 32) : 0;      // from `whole` on with checks
+    const int64_t k = k_begin + 32 * wave, whole = min(k_end, n_in / 32 * 32);                 // from `whole` on with checks
     if (k < whole) {
-        if (two && more) shrink_steps<W, 2, 2, false>(xr, ar, n_in, k, whole, acc);
-        else if (two)    shrink_steps<W, 2, 1, false>(xr, ar, n_in, k, whole, acc);
-        else if (more)   shrink_steps<W, 1, 2, false>(xr, ar, n_in, k, whole, acc);
-        else             shrink_steps<W, 1, 1, false>(xr, ar, n_in, k, whole, acc);
+        if (two && more) shrink_steps<W, 2, 2, false>(xr, A, rw, tile_ld, n_in, k, whole, turn, acc);
+        else if (two)    shrink_steps<W, 2, 1, false>(xr, A, rw, tile_ld, n_in, k, whole, turn, acc);
+        else if (more)   shrink_steps<W, 1, 2, false>(xr, A, rw, tile_ld, n_in, k, whole, turn, acc);
+        else             shrink_steps<W, 1, 1, false>(xr, A, rw, tile_ld, n_in, k, whole, turn, acc);
     }
-    const int64_t rest = max(k, k + (whole - k + 127) / 128 * 128);                            // this wave's first step at or past it
-    if (rest < k_end) shrink_steps<W, 2, 2, true>(xr, ar, n_in, rest, k_end, acc);
+    const int64_t rest = k < whole ? k + (whole - k + 127) / 128 * 128 : k;                    // this wave's first step at or past it
+    if (rest < k_end) {
+        if (more) shrink_steps<W, 2, 2, true>(xr, A, rw, tile_ld, n_in, rest, k_end, turn, acc);
+        else      shrink_steps<W, 2, 1, true>(xr, A, rw, tile_ld, n_in, rest, k_end, turn, acc);
+    }
+    __syncthreads();
+    float * red = reinterpret_cast<float *>(lds);           // [4][LT][LORA_RC + 1]
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) red[wave][16 * i + 4 * g + q][16 * j + m] = acc[i][j][q];
+            for (int q = 0; q < 4; ++q) red[(wave * LT + 16 * i + 4 * g + q) * (LORA_RC + 1) + 16 * j + m] = acc[i][j][q];
     __syncthreads();
     const int nr = min(LORA_RC, ad.r_ld - rc);
     for (int e = threadIdx.x; e < count * LORA_RC; e += 256) {
         const int t = e / LORA_RC, r = e % LORA_RC;
+        const auto part = [&](int w) { return red[(w * LT + t) * (LORA_RC + 1) + r]; };
         if (r < nr)                                         // columns between rank and r_ld are zero, whatever x holds
-            u[(int64_t) list[t] * u_ld + rc + r] = rc + r < ad.rank ? (red[0][t][r] + red[1][t][r]) + (red[2][t][r] + red[3][t][r]) : 0.0f;
+            u[(int64_t) list[t] * u_ld + rc + r] = rc + r < ad.rank ? (part(0) + part(1)) + (part(2) + part(3)) : 0.0f;
     }
     __syncthreads();
 }
 
-template <bool PLAN, bool VEC>
-__global__ __launch_bounds__(256)
+template <bool PLAN>
+__global__ __launch_bounds__(256, 3)
 void lora_shrink_kernel(const LoraAdapter * __restrict__ ads, int n, const int * __restrict__ ids, const LoraTile * __restrict__ tiles, const int * __restrict__ n_tiles,
-                        const int * __restrict__ perm, const float * __restrict__ x, int64_t ldx, int64_t n_in, int64_t a_ld, int64_t T, int64_t k_split,
+                        const int * __restrict__ perm, const float * __restrict__ x, int64_t ldx, int64_t n_in, int64_t a_ld, int64_t T, int splits, int64_t k_split, int n_z,
                         float * __restrict__ u, int u_ld) {
-    __shared__ float red[4][LT][LORA_RC + 1];
+    __shared__ v4f lds[4 * SU * 256];
+    static_assert(sizeof(lds) >= 4 * LT * (LORA_RC + 1) * 4, "room for the join");
     __shared__ int lists[4][64];
     int * list = lists[threadIdx.x >> 6];
+    // the split is the fastest index, then the ranks: all workgroups of a split on one XCD (8 splits and more), those that read the
+    // same columns of x one after the other
+    const int split = (int) (blockIdx.x % (unsigned) splits), rest = (int) (blockIdx.x / (unsigned) splits), rc = rest % n_z * LORA_RC;
     int a = -1;
-    const int count = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, (int) blockIdx.x, list, &a);
+    const int count = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, rest / n_z, list, &a);
     if (!count || a < 0) return;
     const LoraAdapter ad = ads[a];
-    const int rc = (int) blockIdx.z * LORA_RC;
     if (rc >= ad.rank) return;
-    const int64_t k0 = (int64_t) blockIdx.y * k_split, k1 = min(a_ld, k0 + k_split);
-    float * us = u + (int64_t) blockIdx.y * T * u_ld;
+    const int64_t k0 = split * k_split, k1 = min(a_ld, k0 + k_split);
+    float * us = u + split * T * u_ld;
     for (int t0 = 0; t0 < count; t0 += LT) {
-        if (ad.f32) shrink_tile<float, VEC>(ad, list + t0, min(LT, count - t0), rc, x, ldx, n_in, a_ld, k0, k1, us, u_ld, red);
-        else        shrink_tile<__half, VEC>(ad, list + t0, min(LT, count - t0), rc, x, ldx, n_in, a_ld, k0, k1, us, u_ld, red);
+        if (ad.f32) shrink_tile<float>(ad, list + t0, min(LT, count - t0), rc, x, ldx, n_in, a_ld, k0, k1, us, u_ld, lds);
+        else        shrink_tile<__half>(ad, list + t0, min(LT, count - t0), rc, x, ldx, n_in, a_ld, k0, k1, us, u_ld, lds);
     }
 }
 
@@ -368,7 +398,7 @@ __device__ __forceinline__ void expand_mult(const ExpandWave & e, const W * b_al
 }
 
 template <bool PLAN>
-__global__ __launch_bounds__(256, 6)
+__global__ __launch_bounds__(256, 5)
 void lora_expand_kernel(const LoraAdapter * __restrict__ ads, int n, const int * __restrict__ ids, const LoraTile * __restrict__ tiles, const int * __restrict__ n_tiles,
                         const int * __restrict__ perm, const float * __restrict__ u, int u_ld, int splits, int64_t T, int64_t n_out,
                         const float * base, int64_t ldb, float * y, int64_t ldy) {
@@ -428,39 +458,37 @@ void lora_expand_kernel(const LoraAdapter * __restrict__ ads, int n, const int *
 }
 
 // ---- one launch for one to four tokens ----------------------------------------------------------------------------------
-// dot products of R rows of A with one token, one wave; every lane returns the sums
-template <typename W, int R, bool VEC>
-__device__ __forceinline__ void wave_dots(const W * const (&ar)[R], const float * x, int64_t n_in, int64_t a_ld, float (&acc)[R]) {
-    const int lane = threadIdx.x & 63;
+// us[r] = scale * sum_k A[r][k] x[k], 16 (or 8) ranks at a time: a wave takes every eighth block of 32 columns, a lane its rank and
+// eight of them; joined over the lane groups by exchanges and over the waves in LDS.
+template <typename W>
+__device__ void fused_u(const LoraAdapter & ad, const float * x, int64_t n_in, int64_t a_ld, float * us, float (*red)[16]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+    const int rw = ad.r_ld == 8 ? 8 : 16, al = g * rw + (m & (rw - 1));
+    for (int rc = 0; rc < ad.r_ld; rc += rw) {
+        const W * A = (const W *) ad.a + (int64_t) (rc / rw) * rw * a_ld;
+        float acc = 0.0f;
+#pragma unroll 4
+        for (int64_t k = 32 * wave; k < a_ld; k += 256) {
+            AFrag<W> av;
+            av.load(A + k * rw, rw, al);
 #pragma unroll
-    for (int r = 0; r < R; ++r) acc[r] = 0.0f;
-    for (int64_t k = 8 * lane; k < a_ld; k += 512) {
-        float xv[8];
-        load8x<VEC>(x, k, n_in, xv);
+            for (int h = 0; h < 2; ++h) {
+                const v4f xv = load4x<true>(x, k + 16 * h + 4 * g, n_in);
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float av[8];
-            load8(ar[r] + k, av);
-#pragma unroll
-            for (int q = 0; q < 8; ++q) acc[r] = fmaf(av[q], xv[q], acc[r]);
+                for (int q = 0; q < 4; ++q) acc = fmaf(av.get(h, q), xv[q], acc);
+            }
         }
-    }
+        acc += __shfl_xor(acc, 16, 64);
+        acc += __shfl_xor(acc, 32, 64);
+        if (lane < rw) red[wave][lane] = acc;
+        __syncthreads();
+        if ((int) threadIdx.x < rw) {
+            float v = 0.0f;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-        for (int m = 32; m > 0; m >>= 1) acc[r] += __shfl_xor(acc[r], m, 64);
-}
-
-template <typename W, bool VEC>
-__device__ void fused_u(const LoraAdapter & ad, const float * x, int64_t n_in, int64_t a_ld, float * us) {
-    const W * A = (const W *) ad.a;
-    for (int r0 = 2 * (threadIdx.x >> 6); r0 < ad.r_ld; r0 += 16) {
-        const W * const ar[2] = {A + (int64_t) min(r0, ad.rank - 1) * a_ld, A + (int64_t) min(r0 + 1, ad.rank - 1) * a_ld};
-        float acc[2];
-        wave_dots<W, 2, VEC>(ar, x, n_in, a_ld, acc);
-        if ((threadIdx.x & 63) == 0) {                      // columns between rank and r_ld are zero, whatever x holds
-            us[r0] = r0 < ad.rank ? ad.scale * acc[0] : 0.0f;
-            us[r0 + 1] = r0 + 1 < ad.rank ? ad.scale * acc[1] : 0.0f;
+            for (int w = 0; w < 8; ++w) v += red[w][threadIdx.x];
+            us[rc + threadIdx.x] = rc + (int) threadIdx.x < ad.rank ? ad.scale * v : 0.0f;     // between rank and r_ld zero, whatever x holds
         }
+        __syncthreads();
     }
 }
 
@@ -489,11 +517,11 @@ __device__ __forceinline__ float fused_column(const LoraAdapter & ad, int64_t o,
     return v;
 }
 
-template <bool VEC>
 __global__ __launch_bounds__(512)
 void lora_fused_kernel(const LoraAdapter * __restrict__ ads, int n, const int * __restrict__ ids, const float * __restrict__ x, int64_t ldx, int64_t n_in, int64_t a_ld,
                        int64_t n_out, const float * base, int64_t ldb, float * y, int64_t ldy) {
     __shared__ __align__(16) float us[SDH_LORA_MAX_RANK];
+    __shared__ float red[8][16];
     const int64_t t = blockIdx.x, o = (int64_t) blockIdx.y * 512 + threadIdx.x;
     const int a = ids ? ids[t] : 0;
     const float v = base && o < n_out ? base[t * ldb + o] : 0.0f;
@@ -502,9 +530,8 @@ void lora_fused_kernel(const LoraAdapter * __restrict__ ads, int n, const int * 
         return;
     }
     const LoraAdapter ad = ads[a];
-    if (ad.f32) fused_u<float, VEC>(ad, x + t * ldx, n_in, a_ld, us);
-    else        fused_u<__half, VEC>(ad, x + t * ldx, n_in, a_ld, us);
-    __syncthreads();
+    if (ad.f32) fused_u<float>(ad, x + t * ldx, n_in, a_ld, us, red);
+    else        fused_u<__half>(ad, x + t * ldx, n_in, a_ld, us, red);
     if (o >= n_out) return;
     y[t * ldy + o] = ad.f32 ? fused_column<float>(ad, o, us, v) : fused_column<__half>(ad, o, us, v);
 }
@@ -559,7 +586,7 @@ static int lora_create(int64_t n_in, int64_t n_out, const sdh_lora_desc * d, int
         l.u_ld = std::max(l.u_ld, a.r_ld);
         l.stored_bytes += r * n_in * (d[i].a.type == SDH_TYPE_F32 ? 4 : 2) + r * n_out * (d[i].b.type == SDH_TYPE_F32 ? 4 : 2);
         const size_t es = a.f32 ? 4 : 2;
-        at_a[(size_t) i] = total; total += up((size_t) (r * l.a_ld) * es);
+        at_a[(size_t) i] = total; total += up((size_t) (a.r_ld * l.a_ld) * es);
         at_b[(size_t) i] = total; total += up((size_t) b_rows * (size_t) a.r_ld * es);
         l.any_f32 |= a.f32 != 0;
     }
@@ -573,8 +600,10 @@ static int lora_create(int64_t n_in, int64_t n_out, const sdh_lora_desc * d, int
         const size_t es = a.f32 ? 4 : 2;
         a.a = l.dev + at_a[(size_t) i]; a.b = l.dev + at_b[(size_t) i];
         std::vector<uint8_t> rows = lora_rows(d[i].a, a.f32 != 0);
-        buf.assign((size_t) (a.rank * l.a_ld) * es, 0);
-        for (int64_t r = 0; r < a.rank; ++r) memcpy(&buf[(size_t) (r * l.a_ld) * es], &rows[(size_t) (r * n_in) * es], (size_t) n_in * es);
+        buf.assign((size_t) (a.r_ld * l.a_ld) * es, 0);
+        for (int r = 0; r < a.rank; ++r)
+            for (int64_t k = 0; k < n_in; k += 4)           // four columns stay neighbours in either fragment form
+                memcpy(&buf[(size_t) lora_a_at(k, r, a.r_ld, l.a_ld, a.f32 != 0) * es], &rows[(size_t) (r * n_in + k) * es], (size_t) std::min<int64_t>(4, n_in - k) * es);
         SDH_HIP_CHECK(upload(at_a[(size_t) i], buf.size()));
         rows = lora_rows(d[i].b, a.f32 != 0);
         buf.assign((size_t) b_rows * (size_t) a.r_ld * es, 0);
@@ -600,21 +629,21 @@ static int sdh_lora_create_impl(int64_t n_in, int64_t n_out, const sdh_lora_desc
     return rc;
 }
 
-struct LoraCall { const int * ids; const float * x; int64_t ldx, T; const float * base; int64_t ldb; float * y; int64_t ldy; bool vx; };
+struct LoraCall { const int * ids; const float * x; int64_t ldx, T; const float * base; int64_t ldb; float * y; int64_t ldy; };
 
 template <bool PLAN>
 static void lora_two_steps(const LoraSet & l, const LoraWs & w, const LoraCall & c, hipStream_t s) {
     const LoraAdapter * ads = (const LoraAdapter *) l.dev;
-    const int64_t k_split = ((l.a_ld + w.splits - 1) / w.splits + 511) / 512 * 512;
-    const unsigned gx = (unsigned) (PLAN ? w.max_tiles : c.T), splits = (unsigned) ((l.a_ld + k_split - 1) / k_split);
+    const int64_t k_split = ((l.a_ld + w.splits - 1) / w.splits + 31) / 32 * 32;      // the last ones may be empty
+    const int n_z = (l.u_ld + LORA_RC - 1) / LORA_RC;
     const auto shrink = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(gx, splits, (unsigned) ((l.u_ld + LORA_RC - 1) / LORA_RC)), dim3(256), 0, s, ads, l.n, c.ids, w.tiles, w.n_tiles, w.perm, c.x, c.ldx, l.n_in, l.a_ld, c.T, k_split, w.u, l.u_ld);
+        hipLaunchKernelGGL(kernel, dim3((unsigned) ((PLAN ? w.max_tiles : c.T) * n_z * w.splits)), dim3(256), 0, s, ads, l.n, c.ids, w.tiles, w.n_tiles, w.perm, c.x, c.ldx, l.n_in, l.a_ld, c.T, w.splits, k_split, n_z, w.u, l.u_ld);
     };
-    if (c.vx) shrink(lora_shrink_kernel<PLAN, true>); else shrink(lora_shrink_kernel<PLAN, false>);
+    shrink(lora_shrink_kernel<PLAN>);
     const unsigned n_col = (unsigned) ((l.n_out + 255) / 256);
     const auto expand = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned) (PLAN ? w.max_etiles : c.T) * n_col), dim3(256), (size_t) (16 * (l.u_ld + 4)) * 4, s,
-                           ads, l.n, c.ids, w.etiles, w.n_tiles + 1, w.perm, w.u, l.u_ld, (int) splits, c.T, l.n_out, c.base, c.ldb, c.y, c.ldy);
+                           ads, l.n, c.ids, w.etiles, w.n_tiles + 1, w.perm, w.u, l.u_ld, w.splits, c.T, l.n_out, c.base, c.ldb, c.y, c.ldy);
     };
     expand(lora_expand_kernel<PLAN>);
 }
@@ -622,10 +651,7 @@ static void lora_two_steps(const LoraSet & l, const LoraWs & w, const LoraCall &
 static void lora_launch(const LoraSet & l, const LoraWs & w, const LoraCall & c, hipStream_t s) {
     // one launch while every workgroup can read all of A in about the time of a launch: 128 KB of F16 7.5 us, two launches 10.8 us
     if (c.T <= 4 && (int64_t) l.u_ld * l.a_ld * (l.any_f32 ? 4 : 2) <= (256 << 10)) {
-        const auto fused = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3((unsigned) c.T, (unsigned) ((l.n_out + 511) / 512)), dim3(512), 0, s, (const LoraAdapter *) l.dev, l.n, c.ids, c.x, c.ldx, l.n_in, l.a_ld, l.n_out, c.base, c.ldb, c.y, c.ldy);
-        };
-        if (c.vx) fused(lora_fused_kernel<true>); else fused(lora_fused_kernel<false>);
+        hipLaunchKernelGGL(lora_fused_kernel, dim3((unsigned) c.T, (unsigned) ((l.n_out + 511) / 512)), dim3(512), 0, s, (const LoraAdapter *) l.dev, l.n, c.ids, c.x, c.ldx, l.n_in, l.a_ld, l.n_out, c.base, c.ldb, c.y, c.ldy);
     } else if (c.T <= 64) lora_two_steps<false>(l, w, c, s);
     else {
         hipLaunchKernelGGL(lora_plan_kernel, dim3(1), dim3(1024), (size_t) (l.n + 1) * 8, s, c.ids, c.T, l.n, w.perm, w.tiles, w.etiles, w.et, w.n_tiles);
@@ -648,8 +674,7 @@ static int sdh_lora_apply_impl(const sdh_lora * h, const int32_t * ids, const fl
     if (rc != SDH_OK) return rc;
     const LoraWs w = lora_ws(l, T, (uint8_t *) ws);
     if (ws_bytes < w.bytes) { set_error("%s: the workspace holds %lld bytes, %lld are needed", who, (long long) ws_bytes, (long long) w.bytes); return SDH_ERR_INVALID; }
-    const bool vx = aligned(x, 16) && ldx % 4 == 0;
-    lora_launch(l, w, LoraCall{ids, x, ldx, T, base, ldb, y, ldy, vx}, (hipStream_t) stream);
+    lora_launch(l, w, LoraCall{ids, x, ldx, T, base, ldb, y, ldy}, (hipStream_t) stream);
     SDH_HIP_CHECK(hipGetLastError());
     return SDH_OK;
 }
