@@ -54,6 +54,7 @@ struct LoraSet {
 };
 
 constexpr int LT = 32;                     // tokens per tile of the shrink kernel
+constexpr int ET = 16;                     // ... of the expand kernel
 constexpr int LORA_RC = 32;                // ranks per workgroup of the shrink kernel
 
 struct LoraTile { int adapter, start, count, pad; };       // adapter -1: none
@@ -61,15 +62,14 @@ struct LoraTile { int adapter, start, count, pad; };       // adapter -1: none
 // the caller's workspace
 struct LoraWs {
     int * perm; LoraTile * tiles; LoraTile * etiles; int * n_tiles; float * u;
-    int64_t max_tiles, max_etiles; int splits, et; int64_t bytes;
+    int64_t max_tiles, max_etiles; int splits; int64_t bytes;
 };
 
 static LoraWs lora_ws(const LoraSet & l, int64_t T, uint8_t * base) {
     LoraWs w{};
     auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
-    w.et = 16;
     w.max_tiles = (T + LT - 1) / LT + std::min<int64_t>(T, l.n + 1);
-    w.max_etiles = (T + w.et - 1) / w.et + std::min<int64_t>(T, l.n + 1);
+    w.max_etiles = (T + ET - 1) / ET + std::min<int64_t>(T, l.n + 1);
     // K splits of the shrink step: about four workgroups per CU, at least 256 columns each; a power of two, so that from 8 on a split
     // stays on one XCD (round-robin dispatch) with its slice of A for all tiles
     const int64_t tiles = (T + LT - 1) / LT;
@@ -85,25 +85,25 @@ static LoraWs lora_ws(const LoraSet & l, int64_t T, uint8_t * base) {
 }
 
 // ---- tokens sorted by adapter, cut into tiles -----------------------------------------------------------------------
-// One workgroup: count, scan, scatter. The place of a token inside its adapter's run depends on the order of the atomics; no
+// One workgroup: count, scan, tiles, scatter. The place of a token inside its adapter's run depends on the order of the atomics; no
 // result depends on the place.
 __global__ __launch_bounds__(1024)
-void lora_plan_kernel(const int * __restrict__ ids, int64_t T, int n, int * __restrict__ perm, LoraTile * __restrict__ tiles, LoraTile * __restrict__ etiles, int et, int * __restrict__ n_tiles) {
+void lora_plan_kernel(const int * __restrict__ ids, int64_t T, int n, int * __restrict__ perm, LoraTile * __restrict__ tiles, LoraTile * __restrict__ etiles, int * __restrict__ n_tiles) {
     extern __shared__ int lds[];
-    int * cnt = lds, * off = lds + (n + 1);                  // bin n: no adapter
+    int * run = lds, * toff = lds + (n + 2), * eoff = lds + 2 * (n + 2);     // per adapter (bin n: none): tokens, then first place; first tiles
     __shared__ int wsum[3][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int b = tid; b <= n; b += 1024) cnt[b] = 0;
+    for (int b = tid; b <= n + 1; b += 1024) run[b] = 0;
     __syncthreads();
     auto bin = [&](int64_t t) { const int a = t < T && ids ? ids[t] : 0; return t >= T ? -1 : (unsigned) a < (unsigned) n ? a : n; };
     // adds the wave's tokens to the counters of their adapters, one LDS atomic per adapter -> this lane's place
-    auto count_in = [&](int b, int * counter) {
+    auto count_in = [&](int b) {
         int place = 0;
         for (unsigned long long left = __ballot(b >= 0); left;) {
             const int first = __ffsll(left) - 1, one = __shfl(b, first, 64);
             const unsigned long long m = __ballot(b == one);
             int at = 0;
-            if (lane == first) at = atomicAdd(&counter[one], __popcll(m));
+            if (lane == first) at = atomicAdd(&run[one], __popcll(m));
             at = __shfl(at, first, 64);
             if (b == one) place = at + __popcll(m & ((1ull << lane) - 1));
             left &= ~m;
@@ -114,13 +114,13 @@ void lora_plan_kernel(const int * __restrict__ ids, int64_t T, int n, int * __re
     for (int64_t t = tid; t < t_end; t += 4096) {
         const int b[4] = {bin(t), bin(t + 1024), bin(t + 2048), bin(t + 3072)};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) count_in(b[i], cnt);
+        for (int i = 0; i < 4; ++i) count_in(b[i]);
     }
     __syncthreads();
     // exclusive sums of the counts and of both tile counts, a contiguous share of the bins per thread
     const int per = (n + 1 + 1023) / 1024, b0 = min(n + 1, tid * per), b1 = min(n + 1, b0 + per);
     int v[3] = {0, 0, 0}, in[3];
-    for (int b = b0; b < b1; ++b) { v[0] += cnt[b]; v[1] += (cnt[b] + LT - 1) / LT; v[2] += (cnt[b] + et - 1) / et; }
+    for (int b = b0; b < b1; ++b) { v[0] += run[b]; v[1] += (run[b] + LT - 1) / LT; v[2] += (run[b] + ET - 1) / ET; }
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
         in[i] = v[i];
@@ -134,18 +134,29 @@ void lora_plan_kernel(const int * __restrict__ ids, int64_t T, int n, int * __re
         for (int w = 0; w < wave; ++w) v[i] += wsum[i][w];
     }
     for (int b = b0; b < b1; ++b) {
-        off[b] = v[0];
-        for (int j = 0; j < cnt[b]; j += LT) tiles[v[1]++] = LoraTile{b < n ? b : -1, v[0] + j, min(LT, cnt[b] - j), 0};
-        for (int j = 0; j < cnt[b]; j += et) etiles[v[2]++] = LoraTile{b < n ? b : -1, v[0] + j, min(et, cnt[b] - j), 0};
-        v[0] += cnt[b];
+        const int c = run[b];
+        run[b] = v[0]; toff[b] = v[1]; eoff[b] = v[2];
+        v[0] += c; v[1] += (c + LT - 1) / LT; v[2] += (c + ET - 1) / ET;
     }
-    if (tid == 1023) { n_tiles[0] = v[1]; n_tiles[1] = v[2]; }
+    if (tid == 1023) { run[n + 1] = v[0]; toff[n + 1] = n_tiles[0] = v[1]; eoff[n + 1] = n_tiles[1] = v[2]; }
+    __syncthreads();
+    // every tile finds its adapter in the sums
+    const auto fill = [&](const int * first, LoraTile * out, int size) {
+        for (int i = tid; i < first[n + 1]; i += 1024) {
+            int lo = 0, hi = n;                             // the last adapter whose first tile is not past i
+            while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (first[mid] <= i) lo = mid; else hi = mid - 1; }
+            const int at = run[lo] + (i - first[lo]) * size;
+            out[i] = LoraTile{lo < n ? lo : -1, at, min(size, run[lo + 1] - at), 0};
+        }
+    };
+    fill(toff, tiles, LT);
+    fill(eoff, etiles, ET);
     __syncthreads();
     for (int64_t t = tid; t < t_end; t += 4096) {
         const int b[4] = {bin(t), bin(t + 1024), bin(t + 2048), bin(t + 3072)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int place = count_in(b[i], off);
+            const int place = count_in(b[i]);
             if (b[i] >= 0) perm[place] = (int) (t + 1024 * i);
         }
     }
@@ -403,7 +414,7 @@ void lora_expand_kernel(const LoraAdapter * __restrict__ ads, int n, const int *
                         const int * __restrict__ perm, const float * __restrict__ u, int u_ld, int splits, int64_t T, int64_t n_out,
                         const float * base, int64_t ldb, float * y, int64_t ldy) {
     extern __shared__ __align__(16) float us[];             // [16][r_ld + 4]
-    __shared__ int lists[4][PLAN ? LT : 64];
+    __shared__ int lists[4][PLAN ? ET : 64];
     // neighbouring workgroups take neighbouring columns of the same tokens
     const int n_col = (int) ((n_out + 255) >> 8), at = (int) (blockIdx.x / (unsigned) n_col), col = (int) (blockIdx.x % (unsigned) n_col);
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
@@ -654,7 +665,7 @@ static void lora_launch(const LoraSet & l, const LoraWs & w, const LoraCall & c,
         hipLaunchKernelGGL(lora_fused_kernel, dim3((unsigned) c.T, (unsigned) ((l.n_out + 511) / 512)), dim3(512), 0, s, (const LoraAdapter *) l.dev, l.n, c.ids, c.x, c.ldx, l.n_in, l.a_ld, l.n_out, c.base, c.ldb, c.y, c.ldy);
     } else if (c.T <= 64) lora_two_steps<false>(l, w, c, s);
     else {
-        hipLaunchKernelGGL(lora_plan_kernel, dim3(1), dim3(1024), (size_t) (l.n + 1) * 8, s, c.ids, c.T, l.n, w.perm, w.tiles, w.etiles, w.et, w.n_tiles);
+        hipLaunchKernelGGL(lora_plan_kernel, dim3(1), dim3(1024), (size_t) (l.n + 2) * 12, s, c.ids, c.T, l.n, w.perm, w.tiles, w.etiles, w.n_tiles);
         lora_two_steps<true>(l, w, c, s);
     }
 }
