@@ -93,56 +93,68 @@ __global__ __launch_bounds__(256) void dense_few_kernel(const DenseArgs a) {
 }
 
 // 32 tokens x 32 rows per workgroup: still the stream of the weight. The waves split K in groups of four blocks (128 bytes, a whole
-// line of a row) and are joined in LDS at the end; every fragment goes from memory to registers, the next group's before the present
-// one is multiplied, so that a CU has 64 KB in flight without a barrier anywhere in the loop.
+// line of a row) and are joined in LDS at the end; the next group is asked for before the present one is multiplied, without a
+// barrier anywhere in the loop.
+//   loads      128 consecutive bytes of 8 rows per instruction, turned into fragments in a corner of LDS of the wave's own (16-byte
+//              chunks at chunk ^ ((row >> 1) & 7): no bank twice; LDS works in order within a wave). Fragments straight from memory put
+//              neighbouring lanes into different rows, a cache access per lane: 27.4 us against 22.1 for 11 tokens x 14336 -> 4096
+//              (2.8 TB/s), 39 against 23 for 32 tokens.
 //   fragments  v_mfma_i32_32x32x32_i8: lane = row (or token) lane & 31, the 16 bytes of half lane >> 5 of the block; the result has
 //              token 8 (i / 4) + 4 (lane >> 5) + i % 4 in register i and row lane & 31.
 //   scales     four of a row as one 8-byte load (whatever its alignment; one by one they took as long as the weight); the tokens' are
-//              transposed through LDS (each wave its own corner; LDS works in order within a wave).
+//              transposed through LDS.
 //   tail       the last group of a row is its last four blocks, with scales of zero for those that an earlier group has taken.
-// 11 tokens x 14336 -> 4096: 28 us (2.2 TB/s); 16-row tiles with 8-byte fragments took 43 us, 16 waves 31 us, 64 tokens per workgroup
-// 35 us (60 against 38 us at 64 tokens).
 __global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
     constexpr int NW = 8;
+    __shared__ v4i turn[NW][2][256];                             // per wave: 32 rows of the weight, 32 of x
     __shared__ __align__(16) float dxs[NW][4][32];
-    __shared__ float part[NW][32][33];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 31, h = lane >> 5;
+    static_assert(sizeof(turn) >= NW * 32 * 33 * 4, "room for the join");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 31, h = lane >> 5, lr = lane >> 3, lc = lane & 7;
     const int o0 = (int) blockIdx.x * 32;
-    const int64_t t0 = (int64_t) blockIdx.y * 32, orow = min(o0 + m, a.n_out - 1), trow = min(t0 + m, a.T - 1);
-    const int8_t * wp = a.wq + orow * a.nblk * 32 + 16 * h;
-    const __half * dwp = a.wd + orow * a.nblk;
-    const int8_t * xp = a.xq + trow * a.ldq + 16 * h;
-    const float * dxp = a.xd + trow * a.ldd + 2 * h;
+    const int64_t t0 = (int64_t) blockIdx.y * 32;
+    const int8_t * wp[4], * xp[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        wp[i] = a.wq + (int64_t) min(o0 + 8 * i + lr, a.n_out - 1) * a.nblk * 32 + 16 * lc;
+        xp[i] = a.xq + min(t0 + 8 * i + lr, a.T - 1) * a.ldq + 16 * lc;
+    }
+    const __half * dwp = a.wd + (int64_t) min(o0 + m, a.n_out - 1) * a.nblk;
+    const float * dxp = a.xd + min(t0 + m, a.T - 1) * a.ldd + 2 * h;
+    const int st = lr * 8 + (lc ^ (lr >> 1)), key = (m >> 1) & 7;       // rows 8 i + lr: 8 more rows flip bit 2 of the key
     float acc[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-    v4i wf[4], xf[4];
+    v4i wn[4], xn[4];
     __half dw[4];
     float dx[2];
     auto load = [&](int b0) {
         const int bs = min(b0, a.nblk - 4);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) wf[k] = *reinterpret_cast<const v4i *>(wp + (int64_t) (bs + k) * 32);
+        for (int i = 0; i < 4; ++i) wn[i] = *reinterpret_cast<const v4i *>(wp[i] + (int64_t) bs * 32);
         __builtin_memcpy(dw, dwp + bs, 8);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) xf[k] = *reinterpret_cast<const v4i *>(xp + (int64_t) (bs + k) * 32);
+        for (int i = 0; i < 4; ++i) xn[i] = *reinterpret_cast<const v4i *>(xp[i] + (int64_t) bs * 32);
         __builtin_memcpy(dx, dxp + bs, 8);
     };
     load(4 * wave);
     for (int b0 = 4 * wave; b0 < a.nblk; b0 += 4 * NW) {
         const int bs = min(b0, a.nblk - 4);
-        v4i wc[4], xc[4];
         float dc[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { wc[k] = wf[k]; xc[k] = xf[k]; dc[k] = bs + k >= b0 ? __half2float(dw[k]) : 0.0f; }
+        for (int i = 0; i < 4; ++i) {
+            turn[wave][0][64 * i + (i & 1 ? st ^ 4 : st)] = wn[i];
+            turn[wave][1][64 * i + (i & 1 ? st ^ 4 : st)] = xn[i];
+            dc[i] = bs + i >= b0 ? __half2float(dw[i]) : 0.0f;
+        }
         dxs[wave][2 * h][m] = dx[0];
         dxs[wave][2 * h + 1][m] = dx[1];
         load(b0 + 4 * NW);                                       // past the end: in bounds and not used
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
+            const int at = m * 8 + ((2 * k + h) ^ key);
             v16i z = {};
-            z = __builtin_amdgcn_mfma_i32_32x32x32_i8(xc[k], wc[k], z, 0, 0, 0);
+            z = __builtin_amdgcn_mfma_i32_32x32x32_i8(turn[wave][1][at], turn[wave][0][at], z, 0, 0, 0);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const float4 d = *reinterpret_cast<const float4 *>(&dxs[wave][k][8 * q + 4 * h]);
@@ -154,15 +166,17 @@ __global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
         }
         __builtin_amdgcn_wave_barrier();
     }
+    __syncthreads();
+    float * part = reinterpret_cast<float *>(turn);              // [NW][32][33]
 #pragma unroll
-    for (int i = 0; i < 16; ++i) part[wave][8 * (i / 4) + 4 * h + (i & 3)][m] = acc[i];
+    for (int i = 0; i < 16; ++i) part[(wave * 32 + 8 * (i / 4) + 4 * h + (i & 3)) * 33 + m] = acc[i];
     __syncthreads();
     for (int e = threadIdx.x; e < 1024; e += 64 * NW) {
         const int t = e >> 5, c = e & 31;
         if (t0 + t < a.T && o0 + c < a.n_out) {
             float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) v += part[w][t][c];
+            for (int w = 0; w < NW; ++w) v += part[(w * 32 + t) * 33 + c];
             a.y[(t0 + t) * a.ldy + o0 + c] = v;
         }
     }
@@ -314,15 +328,15 @@ static void launch_mfma(const DenseArgs & a, hipStream_t s) {
 static int launch_dense(const DenseArgs & all, hipStream_t s) {
     // Which form, from 3 tokens on: us per 128 bytes of K, by the rounds in which the workgroups fill the CUs (r = workgroups per CU,
     // rounded up), fitted to nine shapes between 1152 and 14336 at 33 to 2048 tokens:
-    //   32 x 32 (mid) 0.34 r + 0.1;  64 x 64, two waves per tile 0.66 r + 0.16;  64 x 128 1.0 r + 0.2;  128 x 128 1.85 r - 0.2, 2.35 at least
-    // 14336 -> 4096, us at 64 / 128 / 256 / 512 / 2048 tokens: mid 38 / 73 / 143 / 283 / 1122, 64 x 64 94 / 93 / 93 / 151 / 655,
-    // 64 x 128 134 / 133 / 133 / 134 / 467, 128 x 128 249 / 263 / 261 / 259 / 403; 4096 -> 14336: 50 / 86 / 165 / 327 / 1304,
+    //   32 x 32 (mid) 0.19 r + 0.05;  64 x 64, two waves per tile 0.66 r + 0.16;  64 x 128 1.0 r + 0.2;  128 x 128 1.85 r - 0.2, 2.35 at least
+    // 14336 -> 4096, us at 64 / 128 / 256 / 512 / 2048 tokens: mid 23 / 42 / 79 / 153 / 595, 64 x 64 94 / 93 / 93 / 151 / 655,
+    // 64 x 128 134 / 133 / 133 / 134 / 467, 128 x 128 249 / 263 / 261 / 259 / 403; 4096 -> 14336: 30 / 49 / 94 / 184 / 730,
     // 30 / 44 / 83 / 145 / 649, 41 / 41 / 65 / 124 / 485, 73 / 76 / 77 / 112 / 421.
     auto rounds = [&](int bm, int bn) {
         const int64_t wg = ((all.T + bm - 1) / bm) * ((all.n_out + bn - 1) / bn), cu = lib().num_cu;
         return (double) ((wg + cu - 1) / cu);
     };
-    const double cost[4] = {0.34 * rounds(32, 32) + 0.1, 0.66 * rounds(64, 64) + 0.16, 1.0 * rounds(64, 128) + 0.2, std::max(2.35, 1.85 * rounds(128, 128) - 0.2)};
+    const double cost[4] = {0.19 * rounds(32, 32) + 0.05, 0.66 * rounds(64, 64) + 0.16, 1.0 * rounds(64, 128) + 0.2, std::max(2.35, 1.85 * rounds(128, 128) - 0.2)};
     const int form = (int) (std::min_element(cost, cost + 4) - cost);
     // a launch has fewer than 2^32 threads, 65536 token tiles in its second dimension: tokens in chunks for very many of them
     const int64_t n_pan = (all.n_out + 63) / 64, chunk = std::max<int64_t>(1, std::min<int64_t>(1024, (1 << 21) / n_pan)) * 128;
@@ -330,8 +344,8 @@ static int launch_dense(const DenseArgs & all, hipStream_t s) {
         DenseArgs a = all;
         a.T = std::min(chunk, all.T - t0);
         a.xq += t0 * a.ldq; a.xd += t0 * a.ldd; a.y += t0 * a.ldy;
-        // one and two tokens: 12.1 / 15.2 us for 4096 -> 14336 (mid 19); up to 8 where mid would have less than a workgroup for every
-        // fourth CU and long rows (6912 -> 1152, 3 / 8 tokens: 7.3 / 8.6 us, mid 12.7 / 13.6); fewer than four blocks: no group for mid
+        // one and two tokens: 12.1 / 15.2 us for 4096 -> 14336 (mid 16.4); up to 8 where mid would have less than a workgroup for every
+        // fourth CU and long rows (6912 -> 1152, 3 / 8 tokens: 7.3 / 8.6 us, mid 12.1); fewer than four blocks: no group for mid
         const bool narrow = all.T <= 8 && a.nblk >= 128 && a.n_out <= 8 * lib().num_cu;
         if (all.T == 1)       { if (a.nblk >= 96) launch_few<1, 2, 4>(a, s); else launch_few<1, 2, 2>(a, s); }
         else if (all.T == 2 || narrow || a.nblk < 4) launch_few<2, 2, 4>(a, s);
