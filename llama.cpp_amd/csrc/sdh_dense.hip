@@ -186,8 +186,11 @@ __global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
 // wave owns 32 tokens x 32 NN rows; with KS = 2 two waves share them, each with every other block, joined at the end.
 //
 // What bounds it is the vector pipe: a 32x32x32 MFMA takes 32 cycles and leaves 16 integers per lane, each of which costs a
-// conversion, the product of its two scales and a fused multiply-add (48 instructions of 4 cycles, packed F32 being off). At 2048
-// tokens x 4096 -> 14336 the vector pipe issues in 85 % of the cycles, the matrix pipe in 11 %, without LDS conflicts.
+// conversion, the product of its two scales and a fused multiply-add (48 instructions of 4 cycles, packed F32 being off; 53 with the
+// rest). At 2048 tokens x 4096 -> 14336 (423 us, 569 TOP/s) the vector pipe issues in 85 % of the cycles and the matrix pipe in the
+// others, without LDS conflicts: the two do not overlap here. So products of the scales by v_mfma_f32_32x32x2_f32 (64 cycles for the
+// 16 instructions that they save, 436 us) gain nothing; nor would F16 operands, whose results need no conversion (two MFMAs of 32
+// cycles and the operands' own conversions).
 //   waves      four per SIMD: a wave waits for LDS, MFMA and conversions in turn (four waves of 64 x 64 in the place of eight of 32 x 64:
 //              559 us against 463).
 //   LDS        16-byte chunks of a row at chunk ^ ((row >> 1) & 7): the 16 rows of a fragment read hit all 64 banks once.
