@@ -35,6 +35,7 @@ __device__ __forceinline__ float4 load4(const float * p, int i, int n) {
     if constexpr (VEC && NT) { const v4f v = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(p + i)); return make_float4(v.x, v.y, v.z, v.w); }
     if constexpr (VEC) return *reinterpret_cast<const float4 *>(p + i);
     float4 v;
+    if (i + 4 <= n) { __builtin_memcpy(&v, p + i, 16); return v; }          // 4-byte aligned: still one load
     v.x = p[i];
     v.y = i + 1 < n ? p[i + 1] : 0.0f; v.z = i + 2 < n ? p[i + 2] : 0.0f; v.w = i + 3 < n ? p[i + 3] : 0.0f;
     return v;
@@ -43,10 +44,10 @@ template <bool VEC, bool NT = false>
 __device__ __forceinline__ void store4(float * p, int i, int n, float4 v) {
     if constexpr (VEC && NT) { __builtin_nontemporal_store(v4f{v.x, v.y, v.z, v.w}, reinterpret_cast<v4f *>(p + i)); return; }
     if constexpr (VEC) { *reinterpret_cast<float4 *>(p + i) = v; return; }
+    if (i + 4 <= n) { __builtin_memcpy(p + i, &v, 16); return; }
     p[i] = v.x;
     if (i + 1 < n) p[i + 1] = v.y;
     if (i + 2 < n) p[i + 2] = v.z;
-    if (i + 3 < n) p[i + 3] = v.w;
 }
 
 // magnitude bits of a double: ordered as unsigned integers, every NaN above infinity, so a maximum keeps a NaN
