@@ -456,12 +456,15 @@ def llama_seeddelta_mul_mat_base_block(x, w_ref, base_d1, base_d2, base_d3, base
 class SeedDeltaContext:
     """Mirror of ``llama_seeddelta_context`` (src/llama-seeddelta.h:27-38): dense-weight key ->
     device payload, filled with the acceptance rules of ``try_add_seeddelta``
-    (src/llama-context.cpp:145-286; enforced inside sdh_weight_create)."""
+    (src/llama-context.cpp:145-286; enforced inside sdh_weight_create), and of the rest of ``build_lora_mm``
+    (src/llama-graph.cpp:672-746) on the device: the weights that stay dense and the adapters of either."""
 
     def __init__(self, enabled: bool = True, gap_tol: float = 0.02):
         self.enabled = enabled
         self.gap_tol = gap_tol          # stored and never read, as in the reference
         self.weights: dict = {}
+        self.dense: dict = {}
+        self.adapters: dict = {}
 
     def try_add(self, key, payload: Payload) -> bool:
         try:
@@ -469,6 +472,20 @@ class SeedDeltaContext:
             return True
         except SeedDeltaError:
             return False               # reference: LLAMA_LOG_WARN + keep the dense path
+
+    def add_dense(self, key, W: np.ndarray):
+        """The dense weight of a key that has no payload (or whose payload was refused): raw Q8_0 rows (n_out, n_in / 32 * 34)."""
+        from . import scan
+        if W.dtype != np.uint8:
+            raise SeedDeltaError(f"add_dense: raw Q8_0 rows (uint8), got {W.dtype}")
+        if _inited_device is None:
+            init(0)
+        self.dense[key] = scan.DenseWeight(W)
+
+    def add_adapters(self, key, adapters):
+        """The adapters of a key: (A (r, n_in), B (n_out, r), scale) each, numbered in order; tokens name theirs by number."""
+        from . import sublayer
+        self.adapters[key] = sublayer.LoraSet(adapters)
 
     def find(self, key) -> Optional[SeedDeltaWeight]:
         return self.weights.get(key)
@@ -479,3 +496,25 @@ class SeedDeltaContext:
             return None
         w = self.find(key)
         return None if w is None else w.forward_host(x)
+
+    def workspace_bytes(self, key, T: int) -> int:
+        """Bytes of workspace (16-byte aligned device memory) that mul_mat_device takes for the key's adapters."""
+        s = self.adapters.get(key)
+        return 0 if s is None else s.workspace_bytes(T)
+
+    def mul_mat_device(self, key, x_ptr: int, ldx: int, T: int, y_ptr: int, ldy: int, x8=None, ids_ptr: int = 0,
+                       ws_ptr: int = 0, ws_bytes: int = 0, flags: int = 0, stream: int = 0) -> bool:
+        """build_lora_mm whole, on device buffers: the key's payload (from x), else its dense weight (from x8, the same activations in
+        8 bits as sublayer.rms_norm_device writes them beside x), then the adapters of the tokens' `ids` added in place (read from x;
+        none registered, or no ids: none added). False: the key has neither payload nor dense weight, nothing was done."""
+        w, d, s = self.find(key) if self.enabled else None, self.dense.get(key), self.adapters.get(key)
+        if w is None and d is None:
+            return False
+        from . import sublayer
+        if w is not None:
+            w.forward_device(x_ptr, ldx, T, y_ptr, ldy, flags, stream)
+        else:
+            sublayer.dense_forward_q8_device(d, x8, T, y_ptr, ldy, stream)
+        if s is not None and ids_ptr:
+            s.apply_device(ids_ptr, x_ptr, ldx, T, y_ptr, ldy, base_ptr=y_ptr, ldb=ldy, ws_ptr=ws_ptr, ws_bytes=ws_bytes, stream=stream)
+        return True

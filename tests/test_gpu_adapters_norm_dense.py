@@ -460,6 +460,57 @@ def test_lora_refusals(hip):
 
 
 # ---- streams and graphs ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("T", [1, 6, 100])
+def test_context_runs_build_lora_mm_on_the_device(hip, T):
+    """SeedDeltaContext.mul_mat_device: a payload, a dense weight and a key without either, with and without adapters; the results
+    are those of the calls it is made of, bit for bit."""
+    n, n_out = 256, 512
+    ctx = hip.SeedDeltaContext()
+    p, W, ads = make_payload(n, n_out, scheme="coo", K=16, base=True, seed=1), make_dense(n, n_out, "q8_0", 2), make_adapters(n, n_out, [8, 20], ["h", "f"])
+    assert ctx.try_add("up", p)
+    ctx.add_dense("gate", W)
+    with pytest.raises(hip.SeedDeltaError):
+        ctx.add_dense("gate16", make_dense(n, n_out, "f16"))
+    for k in ("up", "gate"):
+        ctx.add_adapters(k, ads)
+    x = torch.randn(T, n, device="cuda")
+    q, d, ids = torch.empty(T, n, dtype=torch.int8, device="cuda"), torch.empty(T, n // 32, device="cuda"), dev(some_ids(T, 2, "gaps", T).astype(np.int32))
+    x8 = sublayer.Q8View(q.data_ptr(), n, d.data_ptr(), n // 32)
+    sublayer.q8_quantize_device(x.data_ptr(), n, n, T, x8)
+    ws = torch.empty(ctx.workspace_bytes("up", T), dtype=torch.uint8, device="cuda")
+    assert ctx.workspace_bytes("down", T) == 0
+    assert not ctx.mul_mat_device("down", x.data_ptr(), n, T, 0, n_out)
+    w, dw, s = hip.SeedDeltaWeight(p), scan.DenseWeight(W), sublayer.LoraSet(ads)
+    for key in ("up", "gate"):
+        for with_ids in (False, True):
+            got, want = torch.empty(T, n_out, device="cuda"), torch.empty(T, n_out, device="cuda")
+            i = ids.data_ptr() if with_ids else 0
+            assert ctx.mul_mat_device(key, x.data_ptr(), n, T, got.data_ptr(), n_out, x8=x8, ids_ptr=i, ws_ptr=ws.data_ptr(), ws_bytes=ws.numel())
+            if key == "up":
+                w.forward_device(x.data_ptr(), n, T, want.data_ptr(), n_out)
+            else:
+                sublayer.dense_forward_q8_device(dw, x8, T, want.data_ptr(), n_out)
+            if with_ids:
+                s.apply_device(i, x.data_ptr(), n, T, want.data_ptr(), n_out, base_ptr=want.data_ptr(), ldb=n_out, ws_ptr=ws.data_ptr(), ws_bytes=ws.numel())
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), (key, with_ids)
+    ctx.enabled = False                                   # payloads off: "up" has no dense weight to go to
+    assert not ctx.mul_mat_device("up", x.data_ptr(), n, T, 0, n_out)
+    for v in (w, dw, s):
+        v.close()
+
+
+def test_norm_more_rows_than_one_launch(hip):
+    """Over 2^21 rows: the launch is cut."""
+    T, n = (1 << 21) + 5, 4
+    x = torch.randn(T, n, device="cuda")
+    y = torch.empty_like(x)
+    sublayer.rms_norm_device(x.data_ptr(), n, n, T, eps=EPS, y_ptr=y.data_ptr(), ldy=n)
+    torch.cuda.synchronize()
+    z = x.double() / torch.sqrt((x.double() ** 2).mean(1, keepdim=True) + float(np.float32(EPS)))
+    assert torch.all((y - z).abs() <= (U + 1e-12) * z.abs())
+
+
 @pytest.mark.parametrize("T", [1, 9, 80])
 def test_operators_captured_and_replayed(hip, T):
     """The four calls recorded into one graph as their very first call, replayed with changing inputs and ids, eager work on the same
