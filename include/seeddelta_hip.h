@@ -331,7 +331,8 @@ int sdh_q8_quantize(const float * x, int64_t ldx, int64_t n, int64_t n_tokens, c
 /* sdh_lora_* — low-rank adapters of many requests beside one projection [n_in -> n_out] (SeedDelta or dense):
  *   y[:,t] = base[:,t] + scale_a * B_a (A_a x[:,t]),  a = ids[t]
  * the graph of build_lora_mm (ggml_mul_mat(b, ggml_mul_mat(a, x)), ggml_scale, ggml_add) with the adapter chosen per token.
- * A set holds 1 .. SDH_LORA_MAX_ADAPTERS adapters of ranks 1 .. SDH_LORA_MAX_RANK, each of its own rank and type (F16 or F32). */
+ * A set holds 1 .. SDH_LORA_MAX_ADAPTERS adapters of ranks 1 .. SDH_LORA_MAX_RANK, each of its own rank and type (F16 or F32);
+ * n_in and n_out up to 2^24. */
 #define SDH_LORA_MAX_ADAPTERS 4096
 #define SDH_LORA_MAX_RANK     512
 typedef struct sdh_lora sdh_lora;    /* opaque: the device-resident adapters of one projection */

@@ -341,8 +341,8 @@ static int launch_dense(const DenseArgs & all, hipStream_t s) {
     };
     const double cost[4] = {0.19 * rounds(32, 32) + 0.05, 0.66 * rounds(64, 64) + 0.16, 1.0 * rounds(64, 128) + 0.2, std::max(2.35, 1.85 * rounds(128, 128) - 0.2)};
     const int form = (int) (std::min_element(cost, cost + 4) - cost);
-    // a launch has fewer than 2^32 threads, 65536 token tiles in its second dimension: tokens in chunks for very many of them
-    const int64_t n_pan = (all.n_out + 63) / 64, chunk = std::max<int64_t>(1, std::min<int64_t>(1024, (1 << 21) / n_pan)) * 128;
+    // a launch has fewer than 2^32 threads, 65535 workgroups in its second dimension: tokens in chunks for very many of them
+    const int64_t n_pan = (all.n_out + 63) / 64, chunk = std::max<int64_t>(1, std::min<int64_t>(1000, (1 << 21) / n_pan)) * 128;
     for (int64_t t0 = 0; t0 < all.T; t0 += chunk) {
         DenseArgs a = all;
         a.T = std::min(chunk, all.T - t0);

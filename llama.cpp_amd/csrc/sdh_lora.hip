@@ -31,20 +31,6 @@ struct LoraAdapter {
     int rank, r_ld, f32;   // r_ld: 8, or rank rounded up to 16
 };
 
-inline int64_t lora_a_at(int64_t k, int r, int r_ld, int64_t a_ld, bool f32) {
-    const int rw = r_ld == 8 ? 8 : 16, h = (int) (k >> 4) & 1, g = (int) (k >> 2) & 3, q = (int) k & 3;
-    const int64_t block = ((r / rw) * (a_ld / 32) + (k >> 5)) * rw * 32;
-    const int lane = g * rw + r % rw;
-    return block + (f32 ? h * rw * 16 + lane * 4 + q : lane * 8 + h * 4 + q);
-}
-
-inline int64_t lora_b_at(int64_t o, int r, int r_ld) {
-    const int64_t tile = (o >> 4) * 16 * r_ld;
-    const int row = (int) (o & 15);
-    if (r_ld == 8) return tile + (((r >> 1) * 16 + row) << 1) + (r & 1);
-    return tile + (r >> 4) * 256 + ((((r & 15) >> 2) * 16 + row) << 2) + (r & 3);
-}
-
 struct LoraSet {
     int64_t n_in = 0, n_out = 0, a_ld = 0;
     int n = 0, u_ld = 0;                   // adapters; row pitch of u: the largest r_ld
@@ -574,8 +560,34 @@ static std::vector<uint8_t> lora_rows(const sdh_tensor & t, bool f32) {
     return out;
 }
 
+// rows of A [rank][n_in] into fragment order (LoraAdapter), E: the element
+template <typename E>
+static void lora_pack_a(const E * rows, int rank, int r_ld, int64_t n_in, int64_t a_ld, E * out) {
+    const int rw = r_ld == 8 ? 8 : 16;
+    const bool f32 = sizeof(E) == 4;
+    for (int r = 0; r < rank; ++r)
+        for (int64_t k0 = 0; k0 < n_in; k0 += 32) {
+            E * block = out + (r / rw) * a_ld * rw + k0 * rw;
+            for (int i = 0; i < 8; ++i) {                   // four columns stay neighbours: half h = i >> 2 of the block, lane group g = i & 3
+                const int64_t k = k0 + 4 * i, n = std::min<int64_t>(4, n_in - k);
+                const int lane = (i & 3) * rw + r % rw, h = i >> 2;
+                if (n > 0) memcpy(block + (f32 ? h * rw * 16 + lane * 4 : lane * 8 + h * 4), rows + r * n_in + k, n == 4 ? 4 * sizeof(E) : (size_t) n * sizeof(E));
+            }
+        }
+}
+// rows of B [n_out][rank]
+template <typename E>
+static void lora_pack_b(const E * rows, int rank, int r_ld, int64_t n_out, E * out) {
+    const int kq = r_ld == 8 ? 2 : 4;                       // ranks of a lane
+    for (int64_t o = 0; o < n_out; ++o) {
+        E * tile = out + (o >> 4) * 16 * r_ld + (o & 15) * kq;
+        for (int r = 0; r < rank; r += kq)
+            memcpy(tile + (r / (4 * kq)) * 256 + (r / kq & 3) * 16 * kq, rows + o * rank + r, r + kq <= rank ? (size_t) kq * sizeof(E) : (size_t) (rank - r) * sizeof(E));
+    }
+}
+
 static int lora_create(int64_t n_in, int64_t n_out, const sdh_lora_desc * d, int n, LoraSet ** out) {
-    if (n_in < 1 || n_out < 1 || n_in > INT32_MAX / 2 || n_out > INT32_MAX / 2) { set_error("sdh_lora_create: bad dims n_in=%lld n_out=%lld", (long long) n_in, (long long) n_out); return SDH_ERR_INVALID; }
+    if (n_in < 1 || n_out < 1 || n_in > (1 << 24) || n_out > (1 << 24)) { set_error("sdh_lora_create: bad dims n_in=%lld n_out=%lld", (long long) n_in, (long long) n_out); return SDH_ERR_INVALID; }
     if (n < 1 || n > SDH_LORA_MAX_ADAPTERS) { set_error("sdh_lora_create: %d adapters (1 .. %d)", n, SDH_LORA_MAX_ADAPTERS); return SDH_ERR_INVALID; }
     LoraSet l;
     l.n_in = n_in; l.n_out = n_out; l.n = n;
@@ -612,15 +624,13 @@ static int lora_create(int64_t n_in, int64_t n_out, const sdh_lora_desc * d, int
         a.a = l.dev + at_a[(size_t) i]; a.b = l.dev + at_b[(size_t) i];
         std::vector<uint8_t> rows = lora_rows(d[i].a, a.f32 != 0);
         buf.assign((size_t) (a.r_ld * l.a_ld) * es, 0);
-        for (int r = 0; r < a.rank; ++r)
-            for (int64_t k = 0; k < n_in; k += 4)           // four columns stay neighbours in either fragment form
-                memcpy(&buf[(size_t) lora_a_at(k, r, a.r_ld, l.a_ld, a.f32 != 0) * es], &rows[(size_t) (r * n_in + k) * es], (size_t) std::min<int64_t>(4, n_in - k) * es);
+        if (a.f32) lora_pack_a((const float *) rows.data(), a.rank, a.r_ld, n_in, l.a_ld, (float *) buf.data());
+        else       lora_pack_a((const uint16_t *) rows.data(), a.rank, a.r_ld, n_in, l.a_ld, (uint16_t *) buf.data());
         SDH_HIP_CHECK(upload(at_a[(size_t) i], buf.size()));
         rows = lora_rows(d[i].b, a.f32 != 0);
         buf.assign((size_t) b_rows * (size_t) a.r_ld * es, 0);
-        for (int64_t o = 0; o < n_out; ++o)
-            for (int r = 0; r < a.rank; r += 2)             // pairs of ranks stay neighbours in either fragment form
-                memcpy(&buf[(size_t) lora_b_at(o, r, a.r_ld) * es], &rows[(size_t) (o * a.rank + r) * es], (size_t) std::min(2, a.rank - r) * es);
+        if (a.f32) lora_pack_b((const float *) rows.data(), a.rank, a.r_ld, n_out, (float *) buf.data());
+        else       lora_pack_b((const uint16_t *) rows.data(), a.rank, a.r_ld, n_out, (uint16_t *) buf.data());
         SDH_HIP_CHECK(upload(at_b[(size_t) i], buf.size()));
     }
     buf.resize(tab.size() * sizeof(LoraAdapter));
@@ -670,22 +680,34 @@ static void lora_launch(const LoraSet & l, const LoraWs & w, const LoraCall & c,
     }
 }
 
+// Tokens per pass: a launch has fewer than 2^32 threads, 256 for every tile and 256 columns of y
+static int64_t lora_chunk(const LoraSet & l, int64_t T) {
+    const int64_t most = (1 << 24) / ((l.n_out + 255) / 256 + 1) - 1;            // tiles, at least 250
+    int64_t c = std::min<int64_t>(T, 1 << 20);
+    while (c > 64 && (c + ET - 1) / ET + std::min<int64_t>(c, l.n + 1) > most) c = c / 2;
+    return c;
+}
+
 static int sdh_lora_apply_impl(const sdh_lora * h, const int32_t * ids, const float * x, int64_t ldx, int64_t T,
                                const float * base, int64_t ldb, float * y, int64_t ldy, void * ws, int64_t ws_bytes, void * stream) {
     static const char * who = "sdh_lora_apply";
     if (T == 0) return ready_on_device(who);
     if (!h || !x || !y || !ws) { set_error("%s: null argument", who); return SDH_ERR_INVALID; }
     const LoraSet & l = *reinterpret_cast<const LoraSet *>(h);
-    if (T < 0 || T > INT32_MAX / 2 || ldx < l.n_in || ldy < l.n_out || (base && ldb < l.n_out) || (base == y && ldb != ldy)) {
+    if (T < 0 || T > INT32_MAX / 2 || ldx < l.n_in || ldy < l.n_out || (base && ldb < l.n_out) || (base == y && ldb != ldy) || y == x) {
         set_error("%s: bad shape: T=%lld ldx=%lld (n_in=%lld) ldb=%lld ldy=%lld (n_out=%lld)", who, (long long) T, (long long) ldx, (long long) l.n_in, (long long) ldb, (long long) ldy, (long long) l.n_out);
         return SDH_ERR_INVALID;
     }
     if (!aligned(ids, 4) || !aligned(x, 4) || !aligned(base, 4) || !aligned(y, 4) || !aligned(ws, 16)) { set_error("%s: pointers need 4-byte alignment, the workspace 16", who); return SDH_ERR_INVALID; }
     const int rc = ready_on_device(who);
     if (rc != SDH_OK) return rc;
-    const LoraWs w = lora_ws(l, T, (uint8_t *) ws);
-    if (ws_bytes < w.bytes) { set_error("%s: the workspace holds %lld bytes, %lld are needed", who, (long long) ws_bytes, (long long) w.bytes); return SDH_ERR_INVALID; }
-    lora_launch(l, w, LoraCall{ids, x, ldx, T, base, ldb, y, ldy}, (hipStream_t) stream);
+    const int64_t need = sdh_lora_workspace_bytes(h, T);
+    if (ws_bytes < need) { set_error("%s: the workspace holds %lld bytes, %lld are needed", who, (long long) ws_bytes, (long long) need); return SDH_ERR_INVALID; }
+    const int64_t chunk = lora_chunk(l, T);
+    for (int64_t t0 = 0; t0 < T; t0 += chunk) {
+        const int64_t n = std::min(chunk, T - t0);
+        lora_launch(l, lora_ws(l, n, (uint8_t *) ws), LoraCall{ids ? ids + t0 : nullptr, x + t0 * ldx, ldx, n, base ? base + t0 * ldb : nullptr, ldb, y + t0 * ldy, ldy}, (hipStream_t) stream);
+    }
     SDH_HIP_CHECK(hipGetLastError());
     return SDH_OK;
 }
@@ -710,7 +732,10 @@ extern "C" int64_t sdh_lora_bytes(const sdh_lora * h) { return h ? reinterpret_c
 
 extern "C" int64_t sdh_lora_workspace_bytes(const sdh_lora * h, int64_t T) {
     if (!h || T < 0 || T > INT32_MAX / 2) { set_error("sdh_lora_workspace_bytes: bad argument"); return SDH_ERR_INVALID; }
-    return T == 0 ? 0 : lora_ws(*reinterpret_cast<const LoraSet *>(h), T, nullptr).bytes;
+    if (T == 0) return 0;
+    const LoraSet & l = *reinterpret_cast<const LoraSet *>(h);
+    const int64_t chunk = lora_chunk(l, T), last = T % chunk;
+    return std::max(lora_ws(l, chunk, nullptr).bytes, last ? lora_ws(l, last, nullptr).bytes : 0);
 }
 
 extern "C" int sdh_lora_apply(const sdh_lora * l, const int32_t * ids, const float * x, int64_t ldx, int64_t n_tokens,

@@ -439,6 +439,22 @@ def test_lora_strided_host_views(hip):
     check_lora([(a[:12], b, 0.5), (a[:7].astype(np.float32), np.ascontiguousarray(b[:, :7]), 1.0)], np.array([0, 1, 1, 0, -1]), 5)
 
 
+def test_lora_more_tokens_than_one_pass(hip):
+    """Over 2^20 tokens the call takes them in passes; the workspace it asks for covers each."""
+    T = (1 << 20) + 700
+    rng = np.random.default_rng(0)
+    ads = make_adapters(3, 4, [2, 9], ["h", "f"])
+    ids = rng.integers(-1, 3, T)
+    ids[-700:] = 1
+    check_lora(ads, ids, T, x=rng.standard_normal((T, 3)).astype(np.float32))
+
+
+def test_lora_wide_output(hip):
+    """A million columns: few tokens a pass."""
+    ads = make_adapters(4, 1 << 20, [3, 1], ["f", "h"])
+    check_lora(ads, some_ids(70, 2, "gaps", 1), 70)
+
+
 def test_lora_refusals(hip):
     ads = make_adapters(64, 48, [8], ["h"])
     s = sublayer.LoraSet(ads)
@@ -448,7 +464,7 @@ def test_lora_refusals(hip):
     ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
     good = dict(ids_ptr=ids.data_ptr(), x_ptr=x.data_ptr(), ldx=64, T=4, y_ptr=y.data_ptr(), ldy=48, base_ptr=0, ldb=0, ws_ptr=ws.data_ptr(), ws_bytes=n)
     for k in (dict(x_ptr=0), dict(y_ptr=0), dict(ws_ptr=0), dict(ws_bytes=n - 1), dict(ws_ptr=ws.data_ptr() + 8), dict(ldx=63), dict(ldy=47), dict(T=-1),
-              dict(base_ptr=y.data_ptr(), ldb=49, ldy=48), dict(base_ptr=x.data_ptr(), ldb=47), dict(ids_ptr=ids.data_ptr() + 2), dict(x_ptr=x.data_ptr() + 1)):
+              dict(base_ptr=y.data_ptr(), ldb=49, ldy=48), dict(base_ptr=x.data_ptr(), ldb=47), dict(ids_ptr=ids.data_ptr() + 2), dict(x_ptr=x.data_ptr() + 1), dict(x_ptr=y.data_ptr(), ldx=64)):
         with pytest.raises(hip.SeedDeltaError, match=r"\(-1\)"):
             s.apply_device(**{**good, **k})
     with pytest.raises(hip.SeedDeltaError):

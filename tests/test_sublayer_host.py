@@ -79,6 +79,13 @@ def test_adapter_sets_taken_up_to_the_device(monkeypatch):
             sublayer.LoraSet(adapters)
 
 
+def test_adapter_sets_have_a_largest_size():
+    lib, d = sd.load_library(), (sd.SdhLoraDesc * 1)()
+    h = C.c_void_p()
+    for n_in, n_out in ((0, 48), (32, 0), (-1, 48), ((1 << 24) + 1, 48), (32, (1 << 24) + 1)):
+        assert lib.sdh_lora_create(n_in, n_out, d, 1, C.byref(h)) == -1 and b"dims" in lib.sdh_last_error()
+
+
 def test_lora_entry_points_without_a_set():
     lib = sd.load_library()
     assert lib.sdh_lora_bytes(None) == -1 and lib.sdh_lora_workspace_bytes(None, 4) == -1
