@@ -57,7 +57,8 @@ static LoraWs lora_ws(const LoraSet & l, int64_t T, uint8_t * base) {
     w.max_tiles = (T + LT - 1) / LT + std::min<int64_t>(T, l.n + 1);
     w.max_etiles = (T + ET - 1) / ET + std::min<int64_t>(T, l.n + 1);
     // K splits of the shrink step: about four workgroups per CU, at least 256 columns each; a power of two, so that from 8 on a split
-    // stays on one XCD (round-robin dispatch) with its slice of A for all tiles
+    // stays on one XCD (round-robin dispatch) with its slice of A for all tiles. At most 16, which the expand step adds up: with 8 it
+    // is 1.2 us faster and this one 5 slower (512 tokens at rank 64)
     const int64_t tiles = (T + LT - 1) / LT;
     for (w.splits = 1; w.splits < 16 && 2 * w.splits * tiles <= 1024 && l.a_ld / (2 * w.splits) >= 256;) w.splits *= 2;
     int64_t at = 0;
@@ -213,7 +214,7 @@ __device__ __forceinline__ int lora_tokens(const LoraTile * tiles, const int * n
 // 28 us for the 512 tokens below): a wave loads 128 consecutive bytes of 8 rows per instruction and turns them in a corner of LDS of
 // its own (16-byte chunks of a row at chunk ^ ((row >> 1) & 7): no bank twice; LDS works in order within a wave, so no barrier).
 // A is stored as its fragments are.
-constexpr int SU = 2;                                       // steps in flight per wave
+constexpr int SU = 1;                                       // steps in flight per wave; two: 24.2 us against 20.4 for 512 tokens at rank 64
 
 // NS: groups of 16 tokens, NJ: fragments of A. Steps k, k + 128, ... below k_end; CHECK: some columns of a step may lie past n_in.
 template <typename W, int NS, int NJ, bool CHECK>
@@ -320,8 +321,7 @@ __global__ __launch_bounds__(256, 3)
 void lora_shrink_kernel(const LoraAdapter * __restrict__ ads, int n, const int * __restrict__ ids, const LoraTile * __restrict__ tiles, const int * __restrict__ n_tiles,
                         const int * __restrict__ perm, const float * __restrict__ x, int64_t ldx, int64_t n_in, int64_t a_ld, int64_t T, int splits, int64_t k_split, int n_z,
                         float * __restrict__ u, int u_ld) {
-    __shared__ v4f lds[4 * SU * 256];
-    static_assert(sizeof(lds) >= 4 * LT * (LORA_RC + 1) * 4, "room for the join");
+    __shared__ v4f lds[std::max(4 * SU * 256, LT * (LORA_RC + 1))];          // the waves' corners, then the join
     __shared__ int lists[4][64];
     int * list = lists[threadIdx.x >> 6];
     // the split is the fastest index, then the ranks: all workgroups of a split on one XCD (8 splits and more), those that read the
