@@ -346,8 +346,8 @@ typedef struct sdh_lora_desc {
 int     sdh_lora_create(int64_t n_in, int64_t n_out, const sdh_lora_desc * adapters, int n_adapters, sdh_lora ** out);
 void    sdh_lora_destroy(sdh_lora * l);                       /* waits for the device */
 int64_t sdh_lora_bytes(const sdh_lora * l);                   /* the adapters' weights as stored */
-/* Bytes of the caller's workspace for sdh_lora_apply with n_tokens (16-byte aligned; contents need not be kept or cleared;
- * calls that may overlap — two streams, two graphs in flight — take one each). */
+/* Bytes of the caller's workspace for sdh_lora_apply with up to n_tokens (16-byte aligned; contents need not be kept or
+ * cleared; calls that may overlap — two streams, two graphs in flight — take one each). */
 int64_t sdh_lora_workspace_bytes(const sdh_lora * l, int64_t n_tokens);
 /* ids: int32 [n_tokens] on the device, read by the kernels (a captured graph sees the ids of the replay); anything outside
  * [0, n_adapters) means no adapter: that token's y is its base. ids NULL: every token has adapter 0. Tokens may have their

@@ -42,6 +42,8 @@ struct LoraSet {
 constexpr int LT = 32;                     // tokens per tile of the shrink kernel
 constexpr int ET = 16;                     // ... of the expand kernel
 constexpr int LORA_RC = 32;                // ranks per workgroup of the shrink kernel
+constexpr int LORA_SPLITS = 16;            // its most splits of the columns
+constexpr int64_t LORA_WGS = 1024;         // no more splits where tiles times splits would pass this
 
 struct LoraTile { int adapter, start, count, pad; };       // adapter -1: none
 
@@ -60,7 +62,7 @@ static LoraWs lora_ws(const LoraSet & l, int64_t T, uint8_t * base) {
     // stays on one XCD (round-robin dispatch) with its slice of A for all tiles. At most 16, which the expand step adds up: with 8 it
     // is 1.2 us faster and this one 5 slower (512 tokens at rank 64)
     const int64_t tiles = (T + LT - 1) / LT;
-    for (w.splits = 1; w.splits < 16 && 2 * w.splits * tiles <= 1024 && l.a_ld / (2 * w.splits) >= 256;) w.splits *= 2;
+    for (w.splits = 1; w.splits < LORA_SPLITS && 2 * w.splits * tiles <= LORA_WGS && l.a_ld / (2 * w.splits) >= 256;) w.splits *= 2;
     int64_t at = 0;
     w.perm = (int *) (base + at);         at += up(T * 4);
     w.tiles = (LoraTile *) (base + at);   at += up(w.max_tiles * (int64_t) sizeof(LoraTile));
@@ -680,10 +682,10 @@ static void lora_launch(const LoraSet & l, const LoraWs & w, const LoraCall & c,
     }
 }
 
-// Tokens per pass: a launch has fewer than 2^32 threads, 256 for every tile and 256 columns of y
-static int64_t lora_chunk(const LoraSet & l, int64_t T) {
+// The most tokens of a pass: a launch has fewer than 2^32 threads, 256 for every tile and 256 columns of y
+static int64_t lora_chunk(const LoraSet & l) {
     const int64_t most = (1 << 24) / ((l.n_out + 255) / 256 + 1) - 1;            // tiles, at least 250
-    int64_t c = std::min<int64_t>(T, 1 << 20);
+    int64_t c = 1 << 20;
     while (c > 64 && (c + ET - 1) / ET + std::min<int64_t>(c, l.n + 1) > most) c = c / 2;
     return c;
 }
@@ -703,7 +705,7 @@ static int sdh_lora_apply_impl(const sdh_lora * h, const int32_t * ids, const fl
     if (rc != SDH_OK) return rc;
     const int64_t need = sdh_lora_workspace_bytes(h, T);
     if (ws_bytes < need) { set_error("%s: the workspace holds %lld bytes, %lld are needed", who, (long long) ws_bytes, (long long) need); return SDH_ERR_INVALID; }
-    const int64_t chunk = lora_chunk(l, T);
+    const int64_t chunk = lora_chunk(l);
     for (int64_t t0 = 0; t0 < T; t0 += chunk) {
         const int64_t n = std::min(chunk, T - t0);
         lora_launch(l, lora_ws(l, n, (uint8_t *) ws), LoraCall{ids ? ids + t0 : nullptr, x + t0 * ldx, ldx, n, base ? base + t0 * ldb : nullptr, ldb, y + t0 * ldy, ldy}, (hipStream_t) stream);
@@ -734,8 +736,11 @@ extern "C" int64_t sdh_lora_workspace_bytes(const sdh_lora * h, int64_t T) {
     if (!h || T < 0 || T > INT32_MAX / 2) { set_error("sdh_lora_workspace_bytes: bad argument"); return SDH_ERR_INVALID; }
     if (T == 0) return 0;
     const LoraSet & l = *reinterpret_cast<const LoraSet *>(h);
-    const int64_t chunk = lora_chunk(l, T), last = T % chunk;
-    return std::max(lora_ws(l, chunk, nullptr).bytes, last ? lora_ws(l, last, nullptr).bytes : 0);
+    // what any number of tokens up to T needs: fewer tokens can have more splits, so the most tokens of each number of splits count
+    const int64_t most = std::min(T, lora_chunk(l));
+    int64_t bytes = lora_ws(l, most, nullptr).bytes;
+    for (int64_t splits = 2; splits <= LORA_SPLITS; splits *= 2) bytes = std::max(bytes, lora_ws(l, std::min(most, LORA_WGS / splits * LT), nullptr).bytes);
+    return bytes;
 }
 
 extern "C" int sdh_lora_apply(const sdh_lora * l, const int32_t * ids, const float * x, int64_t ldx, int64_t n_tokens,

@@ -449,6 +449,20 @@ def test_lora_more_tokens_than_one_pass(hip):
     check_lora(ads, ids, T, x=rng.standard_normal((T, 3)).astype(np.float32))
 
 
+def test_lora_workspace_of_the_most_tokens_serves_fewer(hip):
+    s = sublayer.LoraSet(make_adapters(4096, 64, [16, 8], ["h", "h"]))
+    counts = sorted({max(1, c + d) for e in range(0, 22) for c in [1 << e] for d in (-1, 0, 1)} | {3000, 5000, 3 << 20})
+    need = [s.workspace_bytes(T) for T in counts]
+    assert need == sorted(need)
+    T, most = 2048, 2049                                    # the shorter call has twice the splits
+    x = torch.randn(T, 4096, device="cuda")
+    y = torch.zeros(T, 64, device="cuda")
+    ws = torch.empty(s.workspace_bytes(most), dtype=torch.uint8, device="cuda")
+    s.apply_device(0, x.data_ptr(), 4096, T, y.data_ptr(), 64, ws_ptr=ws.data_ptr(), ws_bytes=ws.numel())
+    torch.cuda.synchronize()
+    assert torch.isfinite(y).all() and (y != 0).any(dim=1).all()
+
+
 def test_lora_wide_output(hip):
     """A million columns: few tokens a pass."""
     ads = make_adapters(4, 1 << 20, [3, 1], ["f", "h"])
