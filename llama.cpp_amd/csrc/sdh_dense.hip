@@ -56,12 +56,13 @@ __global__ __launch_bounds__(256) void dense_few_kernel(const DenseArgs a) {
         float dw[U][R];
         int c[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {                         // chunks past the end: the last one, with a scale of zero
+        for (int u = 0; u < U; ++u) {                         // even lanes count; chunks past the end: the last one, both scales zero (one may be infinite)
             c[u] = min(c0 + 64 * u, n_ch - 1);
+            const int counts = c0 + 64 * u < n_ch && !(lane & 1) ? -1 : 0;      // as a mask: a choice would make the load conditional (16.4 us for one token)
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 w[u][r] = __builtin_nontemporal_load(reinterpret_cast<const v4i *>(wp[r] + (int64_t) c[u] * 16));
-                dw[u][r] = __half2float(dp[r][c[u] >> 1]);
+                dw[u][r] = __int_as_float(__float_as_int(__half2float(dp[r][c[u] >> 1])) & counts);
             }
         }
 #pragma unroll
@@ -70,7 +71,7 @@ __global__ __launch_bounds__(256) void dense_few_kernel(const DenseArgs a) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const v4i x = *reinterpret_cast<const v4i *>(a.xq + tt * a.ldq + (int64_t) c[u] * 16);
-                const float dx = c0 + 64 * u < n_ch && !(lane & 1) ? a.xd[tt * a.ldd + (c[u] >> 1)] : 0.0f;     // even lanes count
+                const float dx = c0 + 64 * u < n_ch && !(lane & 1) ? a.xd[tt * a.ldd + (c[u] >> 1)] : 0.0f;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     int s = 0;
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(256) void dense_few_kernel(const DenseArgs a) {
 //              token 8 (i / 4) + 4 (lane >> 5) + i % 4 in register i and row lane & 31.
 //   scales     four of a row as one 8-byte load (whatever its alignment; one by one they took as long as the weight); the tokens' are
 //              transposed through LDS.
-//   tail       the last group of a row is its last four blocks, with scales of zero for those that an earlier group has taken.
+//   tail       the last group of a row is its last four blocks, with both scales zero (one may be infinite) for those that an earlier group has taken.
 __global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
     constexpr int NW = 8;
     __shared__ v4i turn[NW][2][256];                             // per wave: 32 rows of the weight, 32 of x
@@ -146,8 +147,8 @@ __global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
             turn[wave][1][64 * i + (i & 1 ? st ^ 4 : st)] = xn[i];
             dc[i] = bs + i >= b0 ? __half2float(dw[i]) : 0.0f;
         }
-        dxs[wave][2 * h][m] = dx[0];
-        dxs[wave][2 * h + 1][m] = dx[1];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) dxs[wave][2 * h + i][m] = bs + 2 * h + i >= b0 ? dx[i] : 0.0f;
         load(b0 + 4 * NW);                                       // past the end: in bounds and not used
         __builtin_amdgcn_wave_barrier();
 #pragma unroll

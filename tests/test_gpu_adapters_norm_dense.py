@@ -270,6 +270,33 @@ def test_dense_scale_that_is_not_finite_stays_in_its_row(hip, T):
     w.close()
 
 
+@pytest.mark.parametrize("T", [1, 2, 4, 40, 200])
+@pytest.mark.parametrize("n_in", [96, 320, 1056])
+def test_dense_infinite_scales_stay_infinite(hip, n_in, T):
+    """An infinite scale, of the weight or of x, meets no zero that the formula does not have: the output is infinite and not NaN."""
+    W, q, d = dense_case(n_in, 200, T, 6)
+    nb = n_in // 32
+    blk = W.reshape(200, nb, 34)
+    for o, b, v in ((0, nb - 1, 5), (3, max(0, nb - 3), 251), (199, 0, 5), (70, nb // 2, 5)):
+        blk[o, b, :2] = np.frombuffer(np.float16(np.inf).tobytes(), np.uint8)
+        blk[o, b, 2:] = v                                # all 5, or all -5
+    q[:] = np.maximum(np.abs(q), 1)                      # no sum of these blocks is zero
+    blk[:, max(0, nb - 3), 2:][blk[:, max(0, nb - 3), 2:] == 0] = 1
+    for b, t in ((nb - 1, 0), (max(0, nb - 3), T - 1)):
+        d[t, b] = np.inf
+    w, qd, dd, y = scan.DenseWeight(W), dev(q), dev(d), Out(T, 200)
+    sublayer.dense_forward_q8_device(w, sublayer.Q8View(qd.data_ptr(), n_in, dd.data_ptr(), nb), T, y.ptr, y.ld)
+    got = y.get()
+    with np.errstate(invalid="ignore"):
+        want, mag = dense_ref(W, q, d)
+    for value in (np.inf, -np.inf):
+        assert np.array_equal(got == value, want == value)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.isinf(want).any()
+    fin = np.isfinite(want)
+    assert np.all(np.abs(got - np.where(fin, want, 0))[fin] <= ((nb + 10) * U * mag)[fin])
+    w.close()
+
+
 def test_dense_refusals(hip):
     q, d, y = torch.zeros(4, 64, dtype=torch.int8, device="cuda"), torch.zeros(4, 2, device="cuda"), torch.zeros(4, 48, device="cuda")
     w = scan.DenseWeight(make_dense(64, 48, "q8_0"))
