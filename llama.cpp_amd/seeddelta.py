@@ -510,6 +510,9 @@ class SeedDeltaContext:
         w, d, s = self.find(key) if self.enabled else None, self.dense.get(key), self.adapters.get(key)
         if w is None and d is None:
             return False
+        at = w if w is not None else d
+        if s is not None and (s.n_in, s.n_out) != (at.n_in, at.n_out):
+            raise SeedDeltaError(f"mul_mat_device: {key}: adapters of {s.n_in} -> {s.n_out} beside a weight of {at.n_in} -> {at.n_out}")
         from . import sublayer
         if w is not None:
             w.forward_device(x_ptr, ldx, T, y_ptr, ldy, flags, stream)

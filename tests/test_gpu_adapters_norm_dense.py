@@ -557,6 +557,17 @@ def test_context_runs_build_lora_mm_on_the_device(hip, T):
         v.close()
 
 
+@pytest.mark.parametrize("dims", [(512, 512), (128, 512), (256, 544)])
+def test_context_refuses_adapters_of_another_projection(hip, dims):
+    ctx = hip.SeedDeltaContext()
+    ctx.add_dense("up", make_dense(256, 512, "q8_0", 2))
+    ctx.add_adapters("up", make_adapters(*dims, [8], ["h"]))
+    x, y = torch.zeros(2, 512, device="cuda"), torch.full((2, 544), 7.0, device="cuda")
+    with pytest.raises(hip.SeedDeltaError, match="adapters of"):
+        ctx.mul_mat_device("up", x.data_ptr(), 512, 2, y.data_ptr(), 544)
+    assert torch.all(y == 7.0)
+
+
 def test_norm_more_rows_than_one_launch(hip):
     """Over 2^21 rows: the launch is cut."""
     T, n = (1 << 21) + 5, 4
