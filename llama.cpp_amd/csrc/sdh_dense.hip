@@ -15,6 +15,7 @@ namespace sdh {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
+typedef float v32f __attribute__((ext_vector_type(32)));
 
 struct DenseArgs {
     const int8_t * wq; const __half * wd;      // [n_out][n_in], [n_out][nblk]
@@ -198,17 +199,24 @@ __global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
 //   scales     [block][row]: a lane reads the four tokens of a register group as one broadcast.
 //   workgroups XCD k (round-robin dispatch) takes the row panels k, k + 8, ... with all their token tiles: a panel of the weight
 //              comes from memory once and stays in that XCD's L2.
+// 16 bytes per lane from memory straight to LDS: the wave's 1 KB from `to` (the same in all lanes) on, in the order of its lanes
+__device__ __forceinline__ void to_lds(const int8_t * from, int8_t * to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned *) from, (__attribute__((address_space(3))) unsigned *) to, 16, 0, 0);
+}
+
 template <int BM, int BN, int NN, int KS>
 __global__ __launch_bounds__(BM * BN / 16 / NN * KS, 4) void dense_mfma_kernel(const DenseArgs a, int n_tt) {
     constexpr int NT = BM * BN / 16 / NN * KS;                      // threads
     constexpr int XL = BM * 8 / NT, WL = BN * 8 / NT;               // 16-byte loads per thread and stage
     constexpr int XS = (4 * BM + NT - 1) / NT, WS = (4 * BN + NT - 1) / NT;      // scales per thread and stage
-    constexpr int D = BM == 128 ? 1 : 2;                            // stages asked for ahead of the one in use (128: no registers for two)
+    constexpr int D = BM == 128 ? 1 : 2, NSTG = D + 1;              // stages asked for ahead of the one in use; stages of quants in LDS
     static_assert(NT * XL == BM * 8 && NT * WL == BN * 8, "whole loads");
-    __shared__ __align__(16) int8_t xs[2][BM * 128];
-    __shared__ __align__(16) int8_t ws[2][BN * 128];
-    __shared__ __align__(16) float dxs[2][4 * BM];
-    __shared__ __half dws[2][4 * BN];
+    // one array: with several the compiler waits for loads on their way to the next stage before it reads the present one
+    __shared__ __align__(16) int8_t lds[NSTG * (BM + BN) * 128 + 2 * 4 * (BM + BN) * 4];
+    int8_t (* const xs)[BM * 128] = reinterpret_cast<int8_t (*)[BM * 128]>(lds);
+    int8_t (* const ws)[BN * 128] = reinterpret_cast<int8_t (*)[BN * 128]>(lds + NSTG * BM * 128);
+    float (* const dxs)[4 * BM] = reinterpret_cast<float (*)[4 * BM]>(lds + NSTG * (BM + BN) * 128);
+    float (* const dws)[4 * BN] = reinterpret_cast<float (*)[4 * BN]>(lds + NSTG * (BM + BN) * 128 + 2 * 4 * BM * 4);
     const int id = (int) blockIdx.x, seq = id >> 3;
     const int o_tile = ((seq / n_tt) * 8 + (id & 7)) * BN;
     const int64_t t_tile = (int64_t) (seq % n_tt) * BM;
@@ -216,7 +224,8 @@ __global__ __launch_bounds__(BM * BN / 16 / NN * KS, 4) void dense_mfma_kernel(c
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 31, h = lane >> 5;
     const int wt = (wave % (BM / 32)) * 32, wo = (wave / (BM / 32)) % (BN / 32 / NN) * 32 * NN, ks = KS == 1 ? 0 : wave / (BM * BN / 1024 / NN);
     const int64_t n_in = (int64_t) a.nblk * 32;
-    const int lr = tid >> 3, lc = tid & 7;                          // staging: rows lr + NT / 8 i, chunk lc
+    const int lr = tid >> 3, lc = (tid & 7) ^ ((lr >> 1) & 7);      // staging: rows lr + NT / 8 i (the same key), chunk lc into slot tid & 7
+    const int dst = __builtin_amdgcn_readfirstlane(wave) * 1024;
     const int8_t * xp[XL], * wp[WL];
 #pragma unroll
     for (int i = 0; i < XL; ++i) xp[i] = a.xq + min(t_tile + lr + NT / 8 * i, a.T - 1) * a.ldq;
@@ -224,75 +233,79 @@ __global__ __launch_bounds__(BM * BN / 16 / NN * KS, 4) void dense_mfma_kernel(c
     for (int i = 0; i < WL; ++i) wp[i] = a.wq + (int64_t) min(o_tile + lr + NT / 8 * i, a.n_out - 1) * n_in;
     const float * dxp = a.xd + min(t_tile + tid % BM, a.T - 1) * a.ldd;               // scale e of a stage: row e % BM (BN), block e / BM (BN)
     const __half * dwp = a.wd + (int64_t) min(o_tile + tid % BN, a.n_out - 1) * a.nblk;
-    const int st_off = lr * 128 + ((lc ^ ((lr >> 1) & 7)) << 4);    // rows 16 apart have the same key
 
-    struct Stage { v4i x[XL], w[WL]; float dx[XS]; __half dw[WS]; } pre[D];
-    auto load = [&](int b0, Stage & r) {
-        const int cb = min(b0 + (lc >> 1), a.nblk - 1);             // blocks past the end: the last one, with scales of zero
-        const int64_t off = (int64_t) cb * 32 + (lc & 1) * 16;
+    struct Scales { float dx[XS]; __half dw[WS]; } pre[D];
+    auto load = [&](int b0, int st, Scales & r) {
 #pragma unroll
-        for (int i = 0; i < XL; ++i) r.x[i] = *reinterpret_cast<const v4i *>(xp[i] + off);
+        for (int k = 0; k < XS; ++k) r.dx[k] = dxp[min(b0 + ((tid + NT * k) / BM & 3), a.nblk - 1)];
 #pragma unroll
-        for (int i = 0; i < WL; ++i) r.w[i] = *reinterpret_cast<const v4i *>(wp[i] + off);
+        for (int k = 0; k < WS; ++k) r.dw[k] = dwp[min(b0 + ((tid + NT * k) / BN & 3), a.nblk - 1)];
+        asm volatile("" ::: "memory");                              // the quants' loads are the last ones of a stage
+        const int64_t off = (int64_t) min(b0 + (lc >> 1), a.nblk - 1) * 32 + (lc & 1) * 16;       // blocks past the end: the last one, with scales of zero
 #pragma unroll
-        for (int k = 0; k < XS; ++k) { const int b = b0 + ((tid + NT * k) / BM & 3); r.dx[k] = dxp[min(b, a.nblk - 1)]; if (b >= a.nblk) r.dx[k] = 0.0f; }
+        for (int i = 0; i < XL; ++i) to_lds(xp[i] + off, &xs[st][dst + i * 16 * NT]);
 #pragma unroll
-        for (int k = 0; k < WS; ++k) { const int b = b0 + ((tid + NT * k) / BN & 3); r.dw[k] = dwp[min(b, a.nblk - 1)]; if (b >= a.nblk) r.dw[k] = __half(0.0f); }
+        for (int i = 0; i < WL; ++i) to_lds(wp[i] + off, &ws[st][dst + i * 16 * NT]);
     };
-    auto store = [&](int st, const Stage & r) {
+    auto store = [&](int b0, int st, const Scales & r) {            // the choices stand here: at the load they would wait for it
 #pragma unroll
-        for (int i = 0; i < XL; ++i) *reinterpret_cast<v4i *>(&xs[st][st_off + i * 16 * NT]) = r.x[i];
+        for (int k = 0; k < XS; ++k) if (tid + NT * k < 4 * BM) dxs[st][tid + NT * k] = b0 + ((tid + NT * k) / BM & 3) < a.nblk ? r.dx[k] : 0.0f;
 #pragma unroll
-        for (int i = 0; i < WL; ++i) *reinterpret_cast<v4i *>(&ws[st][st_off + i * 16 * NT]) = r.w[i];
-#pragma unroll
-        for (int k = 0; k < XS; ++k) if (tid + NT * k < 4 * BM) dxs[st][tid + NT * k] = r.dx[k];
-#pragma unroll
-        for (int k = 0; k < WS; ++k) if (tid + NT * k < 4 * BN) dws[st][tid + NT * k] = r.dw[k];
+        for (int k = 0; k < WS; ++k) if (tid + NT * k < 4 * BN) dws[st][tid + NT * k] = b0 + ((tid + NT * k) / BN & 3) < a.nblk ? __half2float(r.dw[k]) : 0.0f;
     };
     float acc[NN][16];
 #pragma unroll
     for (int j = 0; j < NN; ++j)
 #pragma unroll
         for (int q = 0; q < 16; ++q) acc[j][q] = 0.0f;
-    const int n_step = (a.nblk + 3) / 4, key = (m >> 1) & 7;        // tiles start at multiples of 32 rows: the key is the lane's
-    load(0, pre[0]);
-    store(0, pre[0]);
+    const int n_step = (a.nblk + 3) / 4, c0 = (((2 * ks + h) ^ ((m >> 1) & 7)) << 4);        // tiles start at multiples of 32 rows: the key is the lane's
+    load(0, 0, pre[0]);
+    store(0, 0, pre[0]);
 #pragma unroll
-    for (int d = 1; d < D; ++d) load(4 * d, pre[d - 1]);
+    for (int d = 1; d < D; ++d) load(4 * d, d, pre[d - 1]);
+    int cur = 0, nxt = D;                                           // the stage in use, the one to fill
     for (int s0 = 0; s0 < n_step; s0 += D)
 #pragma unroll
-    for (int d = 0; d < D; ++d) {                                   // stage s + 1 is in pre[d], stage s + D goes to pre[(d + D - 1) % D]
+    for (int d = 0; d < D; ++d) {                                   // scales of stage s + 1 are in pre[d], those of s + D go to pre[(d + D - 1) % D]
         const int s = s0 + d;
         if (s >= n_step) break;
-        __syncthreads();
+        // all loads but those of the D - 1 stages after this one have arrived
+        if constexpr (D == 1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else                  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(XL + WL) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
         const int st = s & 1;
-        load(4 * (s + D), pre[(d + D - 1) % D]);                    // past the end: in bounds and not stored
-#pragma unroll 1                                                    // or every MFMA of the step is started first, and registers spill
-        for (int k = ks; k < 4; k += KS) {
-            const int ch = ((2 * k + h) ^ key) << 4;
-            const v4i xf = *reinterpret_cast<const v4i *>(&xs[st][(wt + m) * 128 + ch]);
-            v4i wf[NN];
-            float dw[NN];
-            v16i z[NN];
+        load(4 * (s + D), nxt, pre[(d + D - 1) % D]);               // past the end: in bounds and not used
+        // products of the scales, two 32 x 32 outer products an instruction: NN == 2 the wave's two tiles, else two of its blocks
+        constexpr int KP = NN == 2 ? 1 : 2;                         // blocks per step of the loop
+        static_assert(NN * KP == 2, "two outer products");
+        // chunk 2 k + h of row m is at (h ^ key) * 16 with its bits 5 and 6 flipped by k
+        const int8_t * const xa = &xs[cur][(wt + m) * 128], * const wa = &ws[cur][(wo + m) * 128];
+        const float * const dxa = &dxs[st][ks * BM + wt + m + (NN == 2 ? 0 : h * KS * BM)], * const dwa = &dws[st][ks * BN + wo + (NN == 2 ? lane : m + h * KS * BN)];
 #pragma unroll
-            for (int j = 0; j < NN; ++j) { wf[j] = *reinterpret_cast<const v4i *>(&ws[st][(wo + 32 * j + m) * 128 + ch]); dw[j] = __half2float(dws[st][k * BN + wo + 32 * j + m]); }
+        for (int k = 0; k < 4; k += KP * KS) {
+            v32f dd = {};
+            dd = __builtin_amdgcn_mfma_f32_32x32x1f32(dxa[k * BM], dwa[k * BN], dd, 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < NN; ++j) {
-                const v16i zero = {};
-                z[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf, wf[j], zero, 0, 0, 0);
+            for (int p = 0; p < 2; ++p) {
+                const int at = c0 ^ ((NN == 2 ? k : k + KS * p) << 5), j = NN == 2 ? p : 0;
+                const v4i xf = *reinterpret_cast<const v4i *>(xa + at);
+                const v4i wf = *reinterpret_cast<const v4i *>(wa + 32 * j * 128 + at);
+                v16i z = {};
+                z = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf, wf, z, 0, 0, 0);
+#pragma unroll
+                for (int q = 0; q < 16; ++q) acc[j][q] = fmaf((float) z[q], dd[16 * p + q], acc[j][q]);
             }
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4 d4 = *reinterpret_cast<const float4 *>(&dxs[st][k * BM + wt + 8 * g + 4 * h]);
-                const float dx[4] = {d4.x, d4.y, d4.z, d4.w};
+            for (int j = 0; j < NN; ++j)                            // one pair after the other, or every MFMA of the step is started first and registers spill
 #pragma unroll
-                for (int j = 0; j < NN; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) acc[j][4 * g + q] = fmaf((float) z[j][4 * g + q], dx[q] * dw[j], acc[j][4 * g + q]);
-            }
+                for (int q = 0; q < 16; ++q) asm volatile("" : "+v"(acc[j][q]) :: "memory");
         }
-        if (s + 1 < n_step) store(st ^ 1, pre[d]);
+        if (s + 1 < n_step) store(4 * (s + 1), st ^ 1, pre[d]);
+        cur = cur == NSTG - 1 ? 0 : cur + 1;
+        nxt = nxt == NSTG - 1 ? 0 : nxt + 1;
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                // nothing is still on its way to LDS when it changes its use, or its owner
     if constexpr (KS == 2) {                                        // 4 KB per pair of waves: as much as the stages of x hold
         static_assert(KS == 1 || (NN == 1 && BM * BN * 4 <= 2 * BM * 128), "room for the second halves");
         float * red = reinterpret_cast<float *>(xs) + (wave % (NT / 128)) * 1024 + lane;
