@@ -3,8 +3,10 @@
 // The integer sum of a block of 32 is exact (at most 32 * 127 * 128 < 2^20); the two scales multiply it once in F32 and the
 // blocks are summed in F32.
 //
-//   dense_few_kernel   one or two tokens: bound by the stream of the weight; v_dot4_i32_i8.
-//   dense_mid_kernel   a batch: 32 x 32 tiles of v_mfma_i32_32x32x32_i8, whose K is exactly one block, straight from memory.
+//   dense_few_kernel   one token (two of very many rows): bound by the stream of the weight; v_dot4_i32_i8.
+//   dense_thin_kernel, dense_mid_kernel
+//                      a batch: 16 rows of v_mfma_i32_16x16x32_i8 or 32 x 32 tiles of v_mfma_i32_32x32x32_i8, whose K is exactly one
+//                      block, straight from memory.
 //   dense_mfma_kernel  a prompt: tiles of 64 x 64 to 128 x 128 through LDS, bound by the vector pipe (the scales).
 #include "sdh_internal.h"
 
@@ -184,6 +186,99 @@ __global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
     }
 }
 
+// The same with 16 rows and 16 TT tokens per workgroup: twice the workgroups, so that a weight of some thousand rows reaches every CU
+// (11 tokens x 14336 -> 4096: 11.8 us, 5.3 TB/s, with tiles of 32 x 32 on half of the CUs 22.4; 16 waves instead of 8: 13.5).
+//   fragments  v_mfma_i32_16x16x32_i8: lane = row (or token) lane & 15, the 8 bytes lane >> 4 of the block; the result has token
+//              4 (lane >> 4) + i in register i and row lane & 15.
+template <int TT>
+__global__ __launch_bounds__(512, TT == 1 ? 8 : 4) void dense_thin_kernel(const DenseArgs a) {
+    constexpr int NW = 8;
+    __shared__ v4i turn[NW][1 + TT][128];                        // per wave: 16 rows of the weight, 16 TT of x
+    __shared__ __align__(16) float dxs[NW][4][16 * TT];
+    static_assert(sizeof(turn) >= NW * 16 * TT * 17 * 4, "room for the join");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4, lr = lane >> 3, lc = lane & 7;
+    const int o0 = (int) blockIdx.x * 16;
+    const int64_t t0 = (int64_t) blockIdx.y * (16 * TT);
+    const int8_t * wp[2], * xp[2 * TT];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) wp[i] = a.wq + (int64_t) min(o0 + 8 * i + lr, a.n_out - 1) * a.nblk * 32 + 16 * lc;
+#pragma unroll
+    for (int i = 0; i < 2 * TT; ++i) xp[i] = a.xq + min(t0 + 8 * i + lr, a.T - 1) * a.ldq + 16 * lc;
+    const __half * dwp = a.wd + (int64_t) min(o0 + m, a.n_out - 1) * a.nblk;
+    const int dxt = TT == 2 ? lane & 31 : m, dxb = TT == 2 ? 2 * (lane >> 5) : g;         // this lane's token and first block (TT: as many)
+    const float * dxp = a.xd + min(t0 + dxt, a.T - 1) * a.ldd + dxb;
+    const int st = lr * 8 + (lc ^ (lr >> 1)), key = (m >> 1) & 7;       // rows 8 i + lr: 8 more rows flip bit 2 of the key
+    float acc[TT][4];
+#pragma unroll
+    for (int j = 0; j < TT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+    v4i wn[2], xn[2 * TT];
+    __half dw[4];
+    float dx[TT];
+    auto load = [&](int b0) {
+        const int bs = min(b0, a.nblk - 4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) wn[i] = *reinterpret_cast<const v4i *>(wp[i] + (int64_t) bs * 32);
+        __builtin_memcpy(dw, dwp + bs, 8);
+#pragma unroll
+        for (int i = 0; i < 2 * TT; ++i) xn[i] = *reinterpret_cast<const v4i *>(xp[i] + (int64_t) bs * 32);
+        __builtin_memcpy(dx, dxp + bs, 4 * TT);
+    };
+    load(4 * wave);
+    for (int b0 = 4 * wave; b0 < a.nblk; b0 += 4 * NW) {
+        const int bs = min(b0, a.nblk - 4);
+        float dc[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) turn[wave][0][64 * i + (i & 1 ? st ^ 4 : st)] = wn[i];
+#pragma unroll
+        for (int i = 0; i < 2 * TT; ++i) turn[wave][1 + i / 2][64 * (i & 1) + (i & 1 ? st ^ 4 : st)] = xn[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dc[i] = bs + i >= b0 ? __half2float(dw[i]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < TT; ++i) dxs[wave][dxb + i][dxt] = bs + dxb + i >= b0 ? dx[i] : 0.0f;
+        load(b0 + 4 * NW);                                       // past the end: in bounds and not used
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int at = 2 * (m * 8 + ((2 * k + (g >> 1)) ^ key)) + (g & 1);         // 8 bytes
+            const long w = reinterpret_cast<const long *>(turn[wave][0])[at];
+#pragma unroll
+            for (int j = 0; j < TT; ++j) {
+                v4i z = {};
+                z = __builtin_amdgcn_mfma_i32_16x16x32_i8(reinterpret_cast<const long *>(turn[wave][1 + j])[at], w, z, 0, 0, 0);
+                const float4 d = *reinterpret_cast<const float4 *>(&dxs[wave][k][16 * j + 4 * g]);
+                acc[j][0] = fmaf((float) z[0], d.x * dc[k], acc[j][0]);
+                acc[j][1] = fmaf((float) z[1], d.y * dc[k], acc[j][1]);
+                acc[j][2] = fmaf((float) z[2], d.z * dc[k], acc[j][2]);
+                acc[j][3] = fmaf((float) z[3], d.w * dc[k], acc[j][3]);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    float * part = reinterpret_cast<float *>(turn);              // [NW][16 TT][17]
+#pragma unroll
+    for (int j = 0; j < TT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[(wave * 16 * TT + 16 * j + 4 * g + i) * 17 + m] = acc[j][i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 256 * TT; e += 64 * NW) {
+        const int t = e >> 4, c = e & 15;
+        if (t0 + t < a.T && o0 + c < a.n_out) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) v += part[(w * 16 * TT + t) * 17 + c];
+            a.y[(t0 + t) * a.ldy + o0 + c] = v;
+        }
+    }
+}
+
+template <int TT>
+static void launch_thin(const DenseArgs & a, hipStream_t s) {
+    hipLaunchKernelGGL(dense_thin_kernel<TT>, dim3((unsigned) ((a.n_out + 15) / 16), (unsigned) ((a.T + 16 * TT - 1) / (16 * TT))), dim3(512), 0, s, a);
+}
+
 // Many tokens: BM tokens x BN rows per workgroup, both operands through LDS in steps of four blocks (128 bytes a row), two stages. A
 // wave owns 32 tokens x 32 NN rows; with KS = 2 two waves share them, each with every other block, joined at the end.
 //
@@ -343,32 +438,37 @@ static void launch_mfma(const DenseArgs & a, hipStream_t s) {
 }
 
 static int launch_dense(const DenseArgs & all, hipStream_t s) {
-    // Which form, from 3 tokens on: us per 128 bytes of K, by the rounds in which the workgroups fill the CUs (r = workgroups per CU,
-    // rounded up), fitted to nine shapes between 1152 and 14336 at 33 to 2048 tokens:
-    //   32 x 32 (mid) 0.19 r + 0.05;  64 x 64, two waves per tile 0.66 r + 0.16;  64 x 128 1.0 r + 0.2;  128 x 128 1.85 r - 0.2, 2.35 at least
-    // 14336 -> 4096, us at 64 / 128 / 256 / 512 / 2048 tokens: mid 23 / 42 / 79 / 153 / 595, 64 x 64 94 / 93 / 93 / 151 / 655,
-    // 64 x 128 134 / 133 / 133 / 134 / 467, 128 x 128 249 / 263 / 261 / 259 / 403; 4096 -> 14336: 30 / 49 / 94 / 184 / 730,
-    // 30 / 44 / 83 / 145 / 649, 41 / 41 / 65 / 124 / 485, 73 / 76 / 77 / 112 / 421.
+    // Which form, from 2 tokens on: us per 128 bytes of K, by the rounds in which the workgroups fill the CUs (r = workgroups per CU,
+    // rounded up), fitted to eight shapes between 1152 and 28672 at 2 to 2048 tokens:
+    //   16 rows (thin) x 16 tokens 0.115 r, x 32 0.145 r;  32 x 32 (mid) 0.21 r + 0.03;  64 x 64, two waves per tile 0.63 r + 0.06;
+    //   64 x 128 0.96 r, 1.17 at least;  128 x 128 1.6 r, 2 at least
+    // 14336 -> 4096, us at 11 / 32 / 64 / 256 / 512 / 2048 tokens: thin 11.8 / 17.3 / 32 / - / - / -, mid 22.5 / 23.0 / 23.2 / 79 / 156 / 642,
+    // 64 x 64 - / 77 / 83 / 82 / 141 / 601, 64 x 128 - / 122 / 132 / 132 / 133 / 430, 128 x 128 - / 199 / 207 / 222 / 223 / 357;
+    // 4096 -> 14336: 18.7 / 21.4 / 35 / - / - / -, 16.8 / 18.3 / 30 / 96 / 183 / 723, - / 23 / 26 / 80 / 139 / 591, - / 34 / 38 / 60 / 111 / 434,
+    // - / 58 / 60 / 67 / 99 / 364.
     auto rounds = [&](int bm, int bn) {
         const int64_t wg = ((all.T + bm - 1) / bm) * ((all.n_out + bn - 1) / bn), cu = lib().num_cu;
         return (double) ((wg + cu - 1) / cu);
     };
-    const double cost[4] = {0.19 * rounds(32, 32) + 0.05, 0.66 * rounds(64, 64) + 0.16, 1.0 * rounds(64, 128) + 0.2, std::max(2.35, 1.85 * rounds(128, 128) - 0.2)};
-    const int form = (int) (std::min_element(cost, cost + 4) - cost);
+    const double thin = rounds(16, 16);
+    const double cost[6] = {0.115 * thin, 0.145 * rounds(32, 16), 0.21 * rounds(32, 32) + 0.03, 0.63 * rounds(64, 64) + 0.06,
+                            std::max(1.17, 0.96 * rounds(64, 128)), std::max(2.0, 1.6 * rounds(128, 128))};
+    const int form = (int) (std::min_element(cost, cost + 6) - cost);
     // a launch has fewer than 2^32 threads, 65535 workgroups in its second dimension: tokens in chunks for very many of them
     const int64_t n_pan = (all.n_out + 63) / 64, chunk = std::max<int64_t>(1, std::min<int64_t>(1000, (1 << 21) / n_pan)) * 128;
     for (int64_t t0 = 0; t0 < all.T; t0 += chunk) {
         DenseArgs a = all;
         a.T = std::min(chunk, all.T - t0);
         a.xq += t0 * a.ldq; a.xd += t0 * a.ldd; a.y += t0 * a.ldy;
-        // one and two tokens: 12.1 / 15.2 us for 4096 -> 14336 (mid 16.4); up to 8 where mid would have less than a workgroup for every
-        // fourth CU and long rows (6912 -> 1152, 3 / 8 tokens: 7.3 / 8.6 us, mid 12.1); fewer than four blocks: no group for mid
-        const bool narrow = all.T <= 8 && a.nblk >= 128 && a.n_out <= 8 * lib().num_cu;
+        // one token: 4096 -> 14336 11.6 us (thin 16.5), 14336 -> 4096 13.3 (11.5); two tokens of very many rows: 15.0 us (thin 17.1, mid
+        // 16.9), else thin (14336 -> 4096: 16.5 us, thin 11.2); fewer than four blocks: no group for the others
         if (all.T == 1)       { if (a.nblk >= 96) launch_few<1, 2, 4>(a, s); else launch_few<1, 2, 2>(a, s); }
-        else if (all.T == 2 || narrow || a.nblk < 4) launch_few<2, 2, 4>(a, s);
-        else if (form == 0) hipLaunchKernelGGL(dense_mid_kernel, dim3((unsigned) ((a.n_out + 31) / 32), (unsigned) ((a.T + 31) / 32)), dim3(512), 0, s, a);
-        else if (form == 1) launch_mfma<64, 64, 1, 2>(a, s);
-        else if (form == 2) launch_mfma<64, 128, 1, 1>(a, s);
+        else if ((all.T == 2 && thin >= 4) || a.nblk < 4) launch_few<2, 2, 4>(a, s);
+        else if (form == 0) launch_thin<1>(a, s);
+        else if (form == 1) launch_thin<2>(a, s);
+        else if (form == 2) hipLaunchKernelGGL(dense_mid_kernel, dim3((unsigned) ((a.n_out + 31) / 32), (unsigned) ((a.T + 31) / 32)), dim3(512), 0, s, a);
+        else if (form == 3) launch_mfma<64, 64, 1, 2>(a, s);
+        else if (form == 4) launch_mfma<64, 128, 1, 1>(a, s);
         else                launch_mfma<128, 128, 2, 1>(a, s);
     }
     SDH_HIP_CHECK(hipGetLastError());
