@@ -7,7 +7,7 @@
 //   dense_thin_kernel, dense_mid_kernel
 //                      a batch: 16 rows of v_mfma_i32_16x16x32_i8 or 32 x 32 tiles of v_mfma_i32_32x32x32_i8, whose K is exactly one
 //                      block, straight from memory.
-//   dense_mfma_kernel  a prompt: tiles of 64 x 64 to 128 x 128 through LDS, bound by the vector pipe (the scales).
+//   dense_mfma_kernel  a prompt: tiles of 64 x 64 to 128 x 128 through LDS, bound by the vector pipe (integers to F32).
 #include "sdh_internal.h"
 
 #include <algorithm>
@@ -279,39 +279,44 @@ static void launch_thin(const DenseArgs & a, hipStream_t s) {
     hipLaunchKernelGGL(dense_thin_kernel<TT>, dim3((unsigned) ((a.n_out + 15) / 16), (unsigned) ((a.T + 16 * TT - 1) / (16 * TT))), dim3(512), 0, s, a);
 }
 
-// Many tokens: BM tokens x BN rows per workgroup, both operands through LDS in steps of four blocks (128 bytes a row), two stages. A
-// wave owns 32 tokens x 32 NN rows; with KS = 2 two waves share them, each with every other block, joined at the end.
+// Many tokens: BM tokens x BN rows per workgroup, both operands through LDS in steps of SB blocks, two stages. A wave owns 32 tokens x
+// 32 NN rows; with KS = 2 two waves share them, each with every other block, joined at the end.
 //
-// What bounds it is the vector pipe: a 32x32x32 MFMA takes 32 cycles and leaves 16 integers per lane, each of which costs a
-// conversion, the product of its two scales and a fused multiply-add (48 instructions of 4 cycles, packed F32 being off; 53 with the
-// rest). At 2048 tokens x 4096 -> 14336 (423 us, 569 TOP/s) the vector pipe issues in 85 % of the cycles and the matrix pipe in the
-// others, without LDS conflicts: the two do not overlap here. So products of the scales by v_mfma_f32_32x32x2_f32 (64 cycles for the
-// 16 instructions that they save, 436 us) gain nothing; nor would F16 operands, whose results need no conversion (two MFMAs of 32
-// cycles and the operands' own conversions).
+// What bounds it is the vector pipe, to whose time that of the matrix pipe adds (both together issue in every cycle): a 32x32x32 MFMA
+// takes 32 cycles and leaves 16 integers per lane, each of which costs a conversion and a fused multiply-add (packed F32 being off).
+// The products of the scales come from v_mfma_f32_32x32x1_2b_f32, two tiles in 64 cycles (32 vector instructions of 4 cycles
+// otherwise); a step's addresses are one operation each, and the operands' way through registers is left out (loads to LDS), so two
+// tiles take 128 cycles of the matrix pipe and 66 vector instructions. 2048 tokens x 4096 -> 14336: 356 us, 675 TOP/s (products by
+// vector instructions, operands through registers: 424 us).
 //   waves      four per SIMD: a wave waits for LDS, MFMA and conversions in turn (four waves of 64 x 64 in the place of eight of 32 x 64:
 //              559 us against 463).
-//   LDS        16-byte chunks of a row at chunk ^ ((row >> 1) & 7): the 16 rows of a fragment read hit all 64 banks once.
-//   scales     [block][row]: a lane reads the four tokens of a register group as one broadcast.
+//   steps      four blocks (128 bytes a row); eight for 64 x 64, which has half the work between two barriers (512 tokens x 2560 ->
+//              10240: 50 us against 78, with four and two stages ahead 62).
+//   LDS        16-byte chunks of a row at chunk ^ ((row >> 1) & 7), or ^ (row & 15) for 256 bytes a row: the 16 rows of a fragment read
+//              hit all 64 banks once.
+//   scales     [block][row], a lane's row of the product's operand.
 //   workgroups XCD k (round-robin dispatch) takes the row panels k, k + 8, ... with all their token tiles: a panel of the weight
 //              comes from memory once and stays in that XCD's L2.
+
 // 16 bytes per lane from memory straight to LDS: the wave's 1 KB from `to` (the same in all lanes) on, in the order of its lanes
 __device__ __forceinline__ void to_lds(const int8_t * from, int8_t * to) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned *) from, (__attribute__((address_space(3))) unsigned *) to, 16, 0, 0);
 }
 
-template <int BM, int BN, int NN, int KS>
+template <int BM, int BN, int NN, int KS, int SB>
 __global__ __launch_bounds__(BM * BN / 16 / NN * KS, 4) void dense_mfma_kernel(const DenseArgs a, int n_tt) {
     constexpr int NT = BM * BN / 16 / NN * KS;                      // threads
-    constexpr int XL = BM * 8 / NT, WL = BN * 8 / NT;               // 16-byte loads per thread and stage
-    constexpr int XS = (4 * BM + NT - 1) / NT, WS = (4 * BN + NT - 1) / NT;      // scales per thread and stage
-    constexpr int D = BM == 128 ? 1 : 2, NSTG = D + 1;              // stages asked for ahead of the one in use; stages of quants in LDS
-    static_assert(NT * XL == BM * 8 && NT * WL == BN * 8, "whole loads");
+    constexpr int CH = 2 * SB, RB = 16 * CH;                        // chunks and bytes of a row in a stage
+    constexpr int XL = BM * CH / NT, WL = BN * CH / NT;             // 16-byte loads per thread and stage
+    constexpr int XS = (SB * BM + NT - 1) / NT, WS = (SB * BN + NT - 1) / NT;    // scales per thread and stage
+    constexpr int KP = 2 / NN;                                      // blocks per pair of products
+    static_assert(NT * XL == BM * CH && NT * WL == BN * CH && NT / CH % 16 == 0 && KP * NN == 2 && SB % (KP * KS) == 0, "whole loads, whole pairs");
     // one array: with several the compiler waits for loads on their way to the next stage before it reads the present one
-    __shared__ __align__(16) int8_t lds[NSTG * (BM + BN) * 128 + 2 * 4 * (BM + BN) * 4];
-    int8_t (* const xs)[BM * 128] = reinterpret_cast<int8_t (*)[BM * 128]>(lds);
-    int8_t (* const ws)[BN * 128] = reinterpret_cast<int8_t (*)[BN * 128]>(lds + NSTG * BM * 128);
-    float (* const dxs)[4 * BM] = reinterpret_cast<float (*)[4 * BM]>(lds + NSTG * (BM + BN) * 128);
-    float (* const dws)[4 * BN] = reinterpret_cast<float (*)[4 * BN]>(lds + NSTG * (BM + BN) * 128 + 2 * 4 * BM * 4);
+    __shared__ __align__(16) int8_t lds[2 * (BM + BN) * (RB + 4 * SB)];
+    int8_t (* const xs)[BM * RB] = reinterpret_cast<int8_t (*)[BM * RB]>(lds);
+    int8_t (* const ws)[BN * RB] = reinterpret_cast<int8_t (*)[BN * RB]>(lds + 2 * BM * RB);
+    float (* const dxs)[SB * BM] = reinterpret_cast<float (*)[SB * BM]>(lds + 2 * (BM + BN) * RB);
+    float (* const dws)[SB * BN] = reinterpret_cast<float (*)[SB * BN]>(lds + 2 * (BM + BN) * RB + 2 * SB * BM * 4);
     const int id = (int) blockIdx.x, seq = id >> 3;
     const int o_tile = ((seq / n_tt) * 8 + (id & 7)) * BN;
     const int64_t t_tile = (int64_t) (seq % n_tt) * BM;
@@ -319,73 +324,61 @@ __global__ __launch_bounds__(BM * BN / 16 / NN * KS, 4) void dense_mfma_kernel(c
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 31, h = lane >> 5;
     const int wt = (wave % (BM / 32)) * 32, wo = (wave / (BM / 32)) % (BN / 32 / NN) * 32 * NN, ks = KS == 1 ? 0 : wave / (BM * BN / 1024 / NN);
     const int64_t n_in = (int64_t) a.nblk * 32;
-    const int lr = tid >> 3, lc = (tid & 7) ^ ((lr >> 1) & 7);      // staging: rows lr + NT / 8 i (the same key), chunk lc into slot tid & 7
+    const auto key = [](int row) { return SB == 4 ? (row >> 1) & 7 : row & 15; };
+    const int lr = tid / CH, lc = tid % CH ^ key(lr);               // staging: rows lr + NT / CH i (the same key), chunk lc into slot tid % CH
     const int dst = __builtin_amdgcn_readfirstlane(wave) * 1024;
     const int8_t * xp[XL], * wp[WL];
 #pragma unroll
-    for (int i = 0; i < XL; ++i) xp[i] = a.xq + min(t_tile + lr + NT / 8 * i, a.T - 1) * a.ldq;
+    for (int i = 0; i < XL; ++i) xp[i] = a.xq + min(t_tile + lr + NT / CH * i, a.T - 1) * a.ldq;
 #pragma unroll
-    for (int i = 0; i < WL; ++i) wp[i] = a.wq + (int64_t) min(o_tile + lr + NT / 8 * i, a.n_out - 1) * n_in;
+    for (int i = 0; i < WL; ++i) wp[i] = a.wq + (int64_t) min(o_tile + lr + NT / CH * i, a.n_out - 1) * n_in;
     const float * dxp = a.xd + min(t_tile + tid % BM, a.T - 1) * a.ldd;               // scale e of a stage: row e % BM (BN), block e / BM (BN)
     const __half * dwp = a.wd + (int64_t) min(o_tile + tid % BN, a.n_out - 1) * a.nblk;
-
-    struct Scales { float dx[XS]; __half dw[WS]; } pre[D];
-    auto load = [&](int b0, int st, Scales & r) {
+    float dx[XS];
+    __half dw[WS];
+    auto load = [&](int b0, int st) {
 #pragma unroll
-        for (int k = 0; k < XS; ++k) r.dx[k] = dxp[min(b0 + ((tid + NT * k) / BM & 3), a.nblk - 1)];
+        for (int k = 0; k < XS; ++k) dx[k] = dxp[min(b0 + (tid + NT * k) / BM % SB, a.nblk - 1)];
 #pragma unroll
-        for (int k = 0; k < WS; ++k) r.dw[k] = dwp[min(b0 + ((tid + NT * k) / BN & 3), a.nblk - 1)];
-        asm volatile("" ::: "memory");                              // the quants' loads are the last ones of a stage
+        for (int k = 0; k < WS; ++k) dw[k] = dwp[min(b0 + (tid + NT * k) / BN % SB, a.nblk - 1)];
         const int64_t off = (int64_t) min(b0 + (lc >> 1), a.nblk - 1) * 32 + (lc & 1) * 16;       // blocks past the end: the last one, with scales of zero
 #pragma unroll
         for (int i = 0; i < XL; ++i) to_lds(xp[i] + off, &xs[st][dst + i * 16 * NT]);
 #pragma unroll
         for (int i = 0; i < WL; ++i) to_lds(wp[i] + off, &ws[st][dst + i * 16 * NT]);
     };
-    auto store = [&](int b0, int st, const Scales & r) {            // the choices stand here: at the load they would wait for it
+    auto store = [&](int b0, int st) {                              // the choices stand here: at the load they would wait for it
 #pragma unroll
-        for (int k = 0; k < XS; ++k) if (tid + NT * k < 4 * BM) dxs[st][tid + NT * k] = b0 + ((tid + NT * k) / BM & 3) < a.nblk ? r.dx[k] : 0.0f;
+        for (int k = 0; k < XS; ++k) if (tid + NT * k < SB * BM) dxs[st][tid + NT * k] = b0 + (tid + NT * k) / BM < a.nblk ? dx[k] : 0.0f;
 #pragma unroll
-        for (int k = 0; k < WS; ++k) if (tid + NT * k < 4 * BN) dws[st][tid + NT * k] = b0 + ((tid + NT * k) / BN & 3) < a.nblk ? __half2float(r.dw[k]) : 0.0f;
+        for (int k = 0; k < WS; ++k) if (tid + NT * k < SB * BN) dws[st][tid + NT * k] = b0 + (tid + NT * k) / BN < a.nblk ? __half2float(dw[k]) : 0.0f;
     };
     float acc[NN][16];
 #pragma unroll
     for (int j = 0; j < NN; ++j)
 #pragma unroll
         for (int q = 0; q < 16; ++q) acc[j][q] = 0.0f;
-    const int n_step = (a.nblk + 3) / 4, c0 = (((2 * ks + h) ^ ((m >> 1) & 7)) << 4);        // tiles start at multiples of 32 rows: the key is the lane's
-    load(0, 0, pre[0]);
-    store(0, 0, pre[0]);
-#pragma unroll
-    for (int d = 1; d < D; ++d) load(4 * d, d, pre[d - 1]);
-    int cur = 0, nxt = D;                                           // the stage in use, the one to fill
-    for (int s0 = 0; s0 < n_step; s0 += D)
-#pragma unroll
-    for (int d = 0; d < D; ++d) {                                   // scales of stage s + 1 are in pre[d], those of s + D go to pre[(d + D - 1) % D]
-        const int s = s0 + d;
-        if (s >= n_step) break;
-        // all loads but those of the D - 1 stages after this one have arrived
-        if constexpr (D == 1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        else                  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(XL + WL) : "memory");
+    const int c0 = ((2 * ks + h) ^ key(m)) << 4;                    // tiles start at multiples of 32 rows: the key is the lane's
+    load(0, 0);
+    store(0, 0);
+    for (int b0 = 0, st = 0; b0 < a.nblk; b0 += SB, st ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); // the stage has arrived, this wave's part; after the barrier all of it
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        const int st = s & 1;
-        load(4 * (s + D), nxt, pre[(d + D - 1) % D]);               // past the end: in bounds and not used
-        // products of the scales, two 32 x 32 outer products an instruction: NN == 2 the wave's two tiles, else two of its blocks
-        constexpr int KP = NN == 2 ? 1 : 2;                         // blocks per step of the loop
-        static_assert(NN * KP == 2, "two outer products");
-        // chunk 2 k + h of row m is at (h ^ key) * 16 with its bits 5 and 6 flipped by k
-        const int8_t * const xa = &xs[cur][(wt + m) * 128], * const wa = &ws[cur][(wo + m) * 128];
+        load(b0 + SB, st ^ 1);                                      // past the end: in bounds and not used
+        // chunk 2 k + h of row m is at (h ^ key) * 16 with its bits from 5 on flipped by k
+        const int8_t * const xa = &xs[st][(wt + m) * RB], * const wa = &ws[st][(wo + m) * RB];
         const float * const dxa = &dxs[st][ks * BM + wt + m + (NN == 2 ? 0 : h * KS * BM)], * const dwa = &dws[st][ks * BN + wo + (NN == 2 ? lane : m + h * KS * BN)];
 #pragma unroll
-        for (int k = 0; k < 4; k += KP * KS) {
+        for (int k = 0; k < SB; k += KP * KS) {
+            // products of the scales, two 32 x 32 outer products an instruction: NN == 2 the wave's two tiles, else two of its blocks
             v32f dd = {};
             dd = __builtin_amdgcn_mfma_f32_32x32x1f32(dxa[k * BM], dwa[k * BN], dd, 0, 0, 0);
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const int at = c0 ^ ((NN == 2 ? k : k + KS * p) << 5), j = NN == 2 ? p : 0;
                 const v4i xf = *reinterpret_cast<const v4i *>(xa + at);
-                const v4i wf = *reinterpret_cast<const v4i *>(wa + 32 * j * 128 + at);
+                const v4i wf = *reinterpret_cast<const v4i *>(wa + 32 * j * RB + at);
                 v16i z = {};
                 z = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf, wf, z, 0, 0, 0);
 #pragma unroll
@@ -396,22 +389,28 @@ __global__ __launch_bounds__(BM * BN / 16 / NN * KS, 4) void dense_mfma_kernel(c
 #pragma unroll
                 for (int q = 0; q < 16; ++q) asm volatile("" : "+v"(acc[j][q]) :: "memory");
         }
-        if (s + 1 < n_step) store(4 * (s + 1), st ^ 1, pre[d]);
-        cur = cur == NSTG - 1 ? 0 : cur + 1;
-        nxt = nxt == NSTG - 1 ? 0 : nxt + 1;
+        if (b0 + SB < a.nblk) store(b0 + SB, st ^ 1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                // nothing is still on its way to LDS when it changes its use, or its owner
-    if constexpr (KS == 2) {                                        // 4 KB per pair of waves: as much as the stages of x hold
-        static_assert(KS == 1 || (NN == 1 && BM * BN * 4 <= 2 * BM * 128), "room for the second halves");
-        float * red = reinterpret_cast<float *>(xs) + (wave % (NT / 128)) * 1024 + lane;
+    if constexpr (KS > 1) {                                         // the waves that share a tile: 4 KB of each tile and wave but the first
+        constexpr int TW = NT / 64 / KS;                            // waves per part
+        static_assert((KS - 1) * TW * NN * 4096 <= 2 * (BM + BN) * RB, "room for the parts");
+        float * red = reinterpret_cast<float *>(lds) + wave % TW * NN * 1024 + lane;
         __syncthreads();
-        if (ks)
+        if (ks) {
 #pragma unroll
-            for (int q = 0; q < 16; ++q) red[64 * q] = acc[0][q];
+            for (int j = 0; j < NN; ++j)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) red[((ks - 1) * TW * NN + j) * 1024 + 64 * q] = acc[j][q];
+        }
         __syncthreads();
         if (ks) return;
 #pragma unroll
-        for (int q = 0; q < 16; ++q) acc[0][q] += red[64 * q];
+        for (int i = 0; i < KS - 1; ++i)
+#pragma unroll
+            for (int j = 0; j < NN; ++j)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) acc[j][q] += red[(i * TW * NN + j) * 1024 + 64 * q];
     }
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
@@ -431,28 +430,28 @@ static void launch_few(const DenseArgs & a, hipStream_t s) {
     hipLaunchKernelGGL((dense_few_kernel<TT, R, U>), dim3((unsigned) ((a.n_out + 4 * R - 1) / (4 * R)), (unsigned) ((a.T + TT - 1) / TT)), dim3(256), 0, s, a);
 }
 
-template <int BM, int BN, int NN, int KS>
+template <int BM, int BN, int NN, int KS, int SB>
 static void launch_mfma(const DenseArgs & a, hipStream_t s) {
     const int n_tt = (int) ((a.T + BM - 1) / BM), n_pan = (a.n_out + BN - 1) / BN;
-    hipLaunchKernelGGL((dense_mfma_kernel<BM, BN, NN, KS>), dim3((unsigned) ((n_pan + 7) / 8 * 8 * n_tt)), dim3(BM * BN / 16 / NN * KS), 0, s, a, n_tt);
+    hipLaunchKernelGGL((dense_mfma_kernel<BM, BN, NN, KS, SB>), dim3((unsigned) ((n_pan + 7) / 8 * 8 * n_tt)), dim3(BM * BN / 16 / NN * KS), 0, s, a, n_tt);
 }
 
 static int launch_dense(const DenseArgs & all, hipStream_t s) {
     // Which form, from 2 tokens on: us per 128 bytes of K, by the rounds in which the workgroups fill the CUs (r = workgroups per CU,
     // rounded up), fitted to eight shapes between 1152 and 28672 at 2 to 2048 tokens:
-    //   16 rows (thin) x 16 tokens 0.115 r, x 32 0.145 r;  32 x 32 (mid) 0.21 r + 0.03;  64 x 64, two waves per tile 0.63 r + 0.06;
-    //   64 x 128 0.96 r, 1.17 at least;  128 x 128 1.6 r, 2 at least
+    //   16 rows (thin) x 16 tokens 0.115 r, x 32 0.145 r;  32 x 32 (mid) 0.21 r + 0.03;  64 x 64, two waves per tile 0.46 r + 0.1;
+    //   64 x 128 0.92 r, 1.05 at least;  128 x 128 1.54 r, 1.85 at least
     // 14336 -> 4096, us at 11 / 32 / 64 / 256 / 512 / 2048 tokens: thin 11.8 / 17.3 / 32 / - / - / -, mid 22.5 / 23.0 / 23.2 / 79 / 156 / 642,
-    // 64 x 64 - / 77 / 83 / 82 / 141 / 601, 64 x 128 - / 122 / 132 / 132 / 133 / 430, 128 x 128 - / 199 / 207 / 222 / 223 / 357;
-    // 4096 -> 14336: 18.7 / 21.4 / 35 / - / - / -, 16.8 / 18.3 / 30 / 96 / 183 / 723, - / 23 / 26 / 80 / 139 / 591, - / 34 / 38 / 60 / 111 / 434,
-    // - / 58 / 60 / 67 / 99 / 364.
+    // 64 x 64 - / - / 65 / 66 / 103 / 447, 64 x 128 - / - / 120 / 114 / 116 / 425, 128 x 128 - / - / 189 / 205 / 205 / 340;
+    // 4096 -> 14336: 18.7 / 21.4 / 35 / - / - / -, 16.8 / 18.3 / 30 / 96 / 183 / 723, - / - / 23 / 57 / 103 / 465, - / - / 38 / 55 / 104 / 426,
+    // - / - / 55 / 61 / 94 / 348.
     auto rounds = [&](int bm, int bn) {
         const int64_t wg = ((all.T + bm - 1) / bm) * ((all.n_out + bn - 1) / bn), cu = lib().num_cu;
         return (double) ((wg + cu - 1) / cu);
     };
     const double thin = rounds(16, 16);
-    const double cost[6] = {0.115 * thin, 0.145 * rounds(32, 16), 0.21 * rounds(32, 32) + 0.03, 0.63 * rounds(64, 64) + 0.06,
-                            std::max(1.17, 0.96 * rounds(64, 128)), std::max(2.0, 1.6 * rounds(128, 128))};
+    const double cost[6] = {0.115 * thin, 0.145 * rounds(32, 16), 0.21 * rounds(32, 32) + 0.03, 0.46 * rounds(64, 64) + 0.1,
+                            std::max(1.05, 0.92 * rounds(64, 128)), std::max(1.85, 1.54 * rounds(128, 128))};
     const int form = (int) (std::min_element(cost, cost + 6) - cost);
     // a launch has fewer than 2^32 threads, 65535 workgroups in its second dimension: tokens in chunks for very many of them
     const int64_t n_pan = (all.n_out + 63) / 64, chunk = std::max<int64_t>(1, std::min<int64_t>(1000, (1 << 21) / n_pan)) * 128;
@@ -467,9 +466,9 @@ static int launch_dense(const DenseArgs & all, hipStream_t s) {
         else if (form == 0) launch_thin<1>(a, s);
         else if (form == 1) launch_thin<2>(a, s);
         else if (form == 2) hipLaunchKernelGGL(dense_mid_kernel, dim3((unsigned) ((a.n_out + 31) / 32), (unsigned) ((a.T + 31) / 32)), dim3(512), 0, s, a);
-        else if (form == 3) launch_mfma<64, 64, 1, 2>(a, s);
-        else if (form == 4) launch_mfma<64, 128, 1, 1>(a, s);
-        else                launch_mfma<128, 128, 2, 1>(a, s);
+        else if (form == 3) launch_mfma<64, 64, 1, 2, 8>(a, s);
+        else if (form == 4) launch_mfma<64, 128, 1, 1, 4>(a, s);
+        else                launch_mfma<128, 128, 2, 1, 4>(a, s);
     }
     SDH_HIP_CHECK(hipGetLastError());
     return SDH_OK;
