@@ -186,8 +186,9 @@ __device__ __forceinline__ v4f load4x(const float * p, int64_t k, int64_t n) {
 }
 
 // ---- the tokens of a workgroup --------------------------------------------------------------------------------------
-// PLAN: tile `at` of the plan. Otherwise all tokens of the adapter of token `at`, if that is the first of them. -> the tokens in `list` (a row of LDS of each wave's own: LDS works in order within a wave, no barrier), their number (0:
-// nothing to do here) and the adapter (-1: none)
+// PLAN: tile `at` of the plan. Otherwise (up to 64 tokens) all tokens of one adapter: with fewer adapters than tokens of adapter `at` (n:
+// none), else of the adapter of token `at`, if that is the first of them. -> the tokens in `list` (a row of LDS of each wave's own: LDS
+// works in order within a wave, no barrier), their number (0: nothing to do here) and the adapter (-1: none)
 template <bool PLAN>
 __device__ __forceinline__ int lora_tokens(const LoraTile * tiles, const int * n_tiles, const int * perm, const int * ids, int T, int n, int at, int * list, int * adapter) {
     const int lane = threadIdx.x & 63;
@@ -198,14 +199,14 @@ __device__ __forceinline__ int lora_tokens(const LoraTile * tiles, const int * n
         *adapter = tile.adapter;
         return tile.count;
     }
-    const int t = at;
     int a = lane < T ? (ids ? ids[lane] : 0) : -2;          // -2: no token
     if (lane < T && (unsigned) a >= (unsigned) n) a = -1;
-    const int mine = __shfl(a, t, 64);
+    const bool by_adapter = n + 1 < T;
+    const int mine = by_adapter ? (at < n ? at : -1) : __builtin_amdgcn_readfirstlane(__shfl(a, at, 64));
     const unsigned long long m = __ballot(a == mine);
-    if (m & ((1ull << t) - 1)) return 0;
-    if (a == mine) list[__popcll(m & ((1ull << lane) - 1))] = lane;
     *adapter = mine;
+    if (!by_adapter && (m & ((1ull << at) - 1))) return 0;
+    if (a == mine) list[__popcll(m & ((1ull << lane) - 1))] = lane;
     return __popcll(m);
 }
 
@@ -331,9 +332,8 @@ void lora_shrink_kernel(const LoraAdapter * __restrict__ ads, int n, const int *
     const int split = (int) (blockIdx.x % (unsigned) splits), rest = (int) (blockIdx.x / (unsigned) splits), rc = rest % n_z * LORA_RC;
     int a = -1;
     const int count = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, rest / n_z, list, &a);
-    if (!count || a < 0) return;
-    const LoraAdapter ad = ads[a];
-    if (rc >= ad.rank) return;
+    const LoraAdapter ad = ads[max(a, 0)];                  // on its way beside the ids where `a` does not come from them
+    if (!count || a < 0 || rc >= ad.rank) return;
     const int64_t k0 = split * k_split, k1 = min(a_ld, k0 + k_split);
     float * us = u + split * T * u_ld;
     for (int t0 = 0; t0 < count; t0 += LT) {
@@ -409,10 +409,9 @@ void lora_expand_kernel(const LoraAdapter * __restrict__ ads, int n, const int *
     int * list = lists[wave];
     int a = -1;
     const int all = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, at, list, &a);
+    const LoraAdapter ad = ads[max(a, 0)];
     if (!all || (a < 0 && base == y)) return;
     ExpandWave e{list, all, us, 0, 0, n_out, base, ldb, y, ldy};
-    LoraAdapter ad{};
-    if (a >= 0) ad = ads[a];
     e.us_ld = ad.r_ld + 4;                                  // 16-byte rows that start on different banks
     const int n4 = ad.r_ld >> 2;
 #pragma unroll 1
@@ -659,13 +658,14 @@ static void lora_two_steps(const LoraSet & l, const LoraWs & w, const LoraCall &
     const LoraAdapter * ads = (const LoraAdapter *) l.dev;
     const int64_t k_split = ((l.a_ld + w.splits - 1) / w.splits + 31) / 32 * 32;      // the last ones may be empty
     const int n_z = (l.u_ld + LORA_RC - 1) / LORA_RC;
+    const int64_t few = std::min<int64_t>(c.T, l.n + 1);                              // lora_tokens: by token or by adapter
     const auto shrink = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned) ((PLAN ? w.max_tiles : c.T) * n_z * w.splits)), dim3(256), 0, s, ads, l.n, c.ids, w.tiles, w.n_tiles, w.perm, c.x, c.ldx, l.n_in, l.a_ld, c.T, w.splits, k_split, n_z, w.u, l.u_ld);
+        hipLaunchKernelGGL(kernel, dim3((unsigned) ((PLAN ? w.max_tiles : few) * n_z * w.splits)), dim3(256), 0, s, ads, l.n, c.ids, w.tiles, w.n_tiles, w.perm, c.x, c.ldx, l.n_in, l.a_ld, c.T, w.splits, k_split, n_z, w.u, l.u_ld);
     };
     shrink(lora_shrink_kernel<PLAN>);
     const unsigned n_col = (unsigned) ((l.n_out + 255) / 256);
     const auto expand = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned) (PLAN ? w.max_etiles : c.T) * n_col), dim3(256), (size_t) (16 * (l.u_ld + 4)) * 4, s,
+        hipLaunchKernelGGL(kernel, dim3((unsigned) (PLAN ? w.max_etiles : few) * n_col), dim3(256), (size_t) (16 * (l.u_ld + 4)) * 4, s,
                            ads, l.n, c.ids, w.etiles, w.n_tiles + 1, w.perm, w.u, l.u_ld, w.splits, c.T, l.n_out, c.base, c.ldb, c.y, c.ldy);
     };
     expand(lora_expand_kernel<PLAN>);
