@@ -99,11 +99,14 @@ void lora_plan_kernel(const int * __restrict__ ids, int64_t T, int n, int * __re
         }
         return place;
     };
-    const int64_t t_end = (T + 4095) / 4096 * 4096;         // four ids in flight per thread; all lanes take part
+    // four ids in flight per thread; all lanes take part
+    const int64_t t_end = (T + 4095) / 4096 * 4096;
+    int bk[4], at[4];
     for (int64_t t = tid; t < t_end; t += 4096) {
-        const int b[4] = {bin(t), bin(t + 1024), bin(t + 2048), bin(t + 3072)};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) count_in(b[i]);
+        for (int i = 0; i < 4; ++i) bk[i] = bin(t + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) at[i] = count_in(bk[i]);
     }
     __syncthreads();
     // exclusive sums of the counts and of both tile counts, a contiguous share of the bins per thread
@@ -141,6 +144,11 @@ void lora_plan_kernel(const int * __restrict__ ids, int64_t T, int n, int * __re
     fill(toff, tiles, LT);
     fill(eoff, etiles, ET);
     __syncthreads();
+    if (t_end <= 4096) {                                    // every thread still has its tokens and their places in the runs
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (bk[i] >= 0) perm[run[bk[i]] + at[i]] = tid + 1024 * i;
+        return;
+    }
     for (int64_t t = tid; t < t_end; t += 4096) {
         const int b[4] = {bin(t), bin(t + 1024), bin(t + 2048), bin(t + 3072)};
 #pragma unroll
