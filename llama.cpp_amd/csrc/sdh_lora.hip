@@ -43,7 +43,7 @@ constexpr int LT = 32;                     // tokens per tile of the shrink kern
 constexpr int ET = 16;                     // ... of the expand kernel
 constexpr int LORA_RC = 32;                // ranks per workgroup of the shrink kernel
 constexpr int LORA_SPLITS = 16;            // its most splits of the columns
-constexpr int64_t LORA_WGS = 1024;         // no more splits where tiles times splits would pass this
+constexpr int64_t LORA_WGS = 384;          // no more splits where tiles times splits would pass this
 
 struct LoraTile { int adapter, start, count, pad; };       // adapter -1: none
 
@@ -58,9 +58,10 @@ static LoraWs lora_ws(const LoraSet & l, int64_t T, uint8_t * base) {
     auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
     w.max_tiles = (T + LT - 1) / LT + std::min<int64_t>(T, l.n + 1);
     w.max_etiles = (T + ET - 1) / ET + std::min<int64_t>(T, l.n + 1);
-    // K splits of the shrink step: about four workgroups per CU, at least 256 columns each; a power of two, so that from 8 on a split
-    // stays on one XCD (round-robin dispatch) with its slice of A for all tiles. At most 16, which the expand step adds up: with 8 it
-    // is 1.2 us faster and this one 5 slower (512 tokens at rank 64)
+    // K splits of the shrink step: a workgroup per CU and more, at least 256 columns each; a power of two, so that from 8 on a split
+    // stays on one XCD (round-robin dispatch) with its slice of A for all tiles. Not more than that needs, as the expand step adds them
+    // up: 4096 tokens at rank 16, 2 splits 123 us, 8 (1056 workgroups) 129; 512 tokens at rank 64, 8 instead of 16 makes the expand step
+    // 1.2 us faster and this one 5 slower
     const int64_t tiles = (T + LT - 1) / LT;
     for (w.splits = 1; w.splits < LORA_SPLITS && 2 * w.splits * tiles <= LORA_WGS && l.a_ld / (2 * w.splits) >= 256;) w.splits *= 2;
     int64_t at = 0;
