@@ -48,7 +48,7 @@ typedef enum sdh_status {
 typedef enum sdh_type {
     SDH_TYPE_F32  = 0,   /* GGML_TYPE_F32  */
     SDH_TYPE_F16  = 1,   /* GGML_TYPE_F16  */
-    SDH_TYPE_Q8_0 = 8,   /* GGML_TYPE_Q8_0 (dense weights for the scan only) */
+    SDH_TYPE_Q8_0 = 8,   /* GGML_TYPE_Q8_0 (dense weights)  */
     SDH_TYPE_I16  = 25,  /* GGML_TYPE_I16  */
     SDH_TYPE_I32  = 26   /* GGML_TYPE_I32  */
 } sdh_type;

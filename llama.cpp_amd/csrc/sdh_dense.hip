@@ -30,7 +30,7 @@ struct DenseArgs {
 
 // A wave owns R rows; chunk c of 16 bytes (half a block) of a row belongs to lane c & 63, so a load instruction takes 1 KB of
 // consecutive bytes, U of them per row in flight; neighbouring lanes join their halves of a block as integers. The tokens' chunks
-// come from the cache; no LDS, no barrier. One token x 4096 -> 14336: 12.1 us, 5.2 TB/s (58.7 MB, a large copy moves 4.9 TB/s);
+// come from the cache; no LDS, no barrier. One token x 4096 -> 14336: 11.6 us, 5.4 TB/s (62.4 MB; torch's copy of a large tensor 4.95);
 // a block per lane, two loads 32 bytes apart, took 22.8 us, four rows per wave 13.3 to 13.9 us, one row 10.5 us without the
 // exchange of halves against 10.6 for two.
 template <int TT, int R, int U>
@@ -101,13 +101,14 @@ __global__ __launch_bounds__(256) void dense_few_kernel(const DenseArgs a) {
 // barrier anywhere in the loop.
 //   loads      128 consecutive bytes of 8 rows per instruction, turned into fragments in a corner of LDS of the wave's own (16-byte
 //              chunks at chunk ^ ((row >> 1) & 7): no bank twice; LDS works in order within a wave). Fragments straight from memory put
-//              neighbouring lanes into different rows, a cache access per lane: 27.4 us against 22.1 for 11 tokens x 14336 -> 4096
-//              (2.8 TB/s), 39 against 23 for 32 tokens.
+//              neighbouring lanes into different rows, a cache access per lane: 27.4 us against 22.1 for 11 tokens x 14336 -> 4096,
+//              39 against 23 for 32 tokens.
 //   fragments  v_mfma_i32_32x32x32_i8: lane = row (or token) lane & 31, the 16 bytes of half lane >> 5 of the block; the result has
 //              token 8 (i / 4) + 4 (lane >> 5) + i % 4 in register i and row lane & 31.
 //   scales     four of a row as one 8-byte load (whatever its alignment; one by one they took as long as the weight); the tokens' are
 //              transposed through LDS.
-//   tail       the last group of a row is its last four blocks, with both scales zero (one may be infinite) for those that an earlier group has taken.
+//   tail       the last group of a row is its last four blocks, with both scales zero (one may be infinite) for those that an earlier
+//              group has taken.
 __global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
     constexpr int NW = 8;
     __shared__ v4i turn[NW][2][256];                             // per wave: 32 rows of the weight, 32 of x
@@ -187,7 +188,8 @@ __global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
 }
 
 // The same with 16 rows and 16 TT tokens per workgroup: twice the workgroups, so that a weight of some thousand rows reaches every CU
-// (11 tokens x 14336 -> 4096: 11.8 us, 5.3 TB/s, with tiles of 32 x 32 on half of the CUs 22.4; 16 waves instead of 8: 13.5).
+// (11 tokens x 14336 -> 4096: 11.8 us, 5.3 TB/s, with tiles of 32 x 32 on half of the CUs 22.4; 16 waves instead of 8: 13.5). With three
+// or four workgroups per CU at once (4096 -> 14336) 18.7 us, tiles of 32 x 32 16.8; starting each workgroup at another column 20.5.
 //   fragments  v_mfma_i32_16x16x32_i8: lane = row (or token) lane & 15, the 8 bytes lane >> 4 of the block; the result has token
 //              4 (lane >> 4) + i in register i and row lane & 15.
 template <int TT>

@@ -7,6 +7,11 @@
 //   more              lora_plan_kernel sorts the tokens by adapter and cuts them into tiles.
 // One to four tokens of small adapters take one launch (lora_fused_kernel) in which every workgroup forms u for itself.
 //
+// Kernel times (plan + shrink + expand), and what bounds them: 1 token, rank 16, 4096 -> 14336: 6.3 us (one launch and its chain of
+// loads: id, record, A, B). 48 tokens, 32 adapters of rank 32 and less: 5.9 + 11.1 us (the same chains; 22 MB). 512 tokens, rank 64 in
+// F32, 14336 -> 4096: 4.9 + 20 + 13 us (the products alone are 2 x 6 us at the rate of a large F32 product; x comes from the caches
+// twice, once per 32 ranks). 4096 tokens, rank 16, 4096 -> 14336: 7.6 + 23 + 96 us; the last one is 470 MB of base and y, 4.9 TB/s.
+//
 // Everything is F32: v_mfma_f32_16x16x4_f32 does 2048 operations in 32 cycles, and both steps move far more bytes than that costs
 // (8 bytes of y per 2 * rank operations, 4 of x per 2 * rank). Which k an MFMA takes is free as long as both operands agree: lane
 // group g = lane >> 4 holds consecutive columns and MFMA j multiplies its j-th, so every operand load is a vector.
@@ -21,9 +26,9 @@ namespace sdh {
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 // A in the order of the shrink kernel's fragments: per 16 ranks (8 up to rank 8), per 32 columns, lane' = 16 (or 8) * group + rank with
-// columns 4 group .. and 16 + 4 group ..: eight consecutive halves, or four floats in each of two halves of the block. B in the order of the expand kernel's fragments: per 16 output rows, per 16 ranks,
-// [lane][4] with row lane & 15 and ranks 4 (lane >> 4) ..; up to rank 8 one [lane][2] with ranks 2 (lane >> 4) ... Whatever lies past
-// n_in, n_out or `rank` is zero.
+// columns 4 group .. and 16 + 4 group ..: eight consecutive halves, or four floats in each of two halves of the block. B in the order of
+// the expand kernel's fragments: per 16 output rows, per 16 ranks, [lane][4] with row lane & 15 and ranks 4 (lane >> 4) ..; up to
+// rank 8 one [lane][2] with ranks 2 (lane >> 4) ... Whatever lies past n_in, n_out or `rank` is zero.
 struct LoraAdapter {
     const void * a;
     const void * b;
@@ -222,8 +227,8 @@ __device__ __forceinline__ int lora_tokens(const LoraTile * tiles, const int * n
 // ---- u[split][token][r] = sum over the split's columns of A[r][k] x[token][k] -------------------------------------------
 // A workgroup: one tile, LORA_RC ranks, one split of the columns; its four waves take steps of 32 columns in turn and are joined in
 // LDS. 16x16x4 operands: row / column lane & 15, k = lane >> 4; in a step lane group g holds columns 4 g .. 4 g + 3 and 16 + 4 g ...
-// Fragments of x read from memory would put neighbouring lanes into different rows, a cache access per lane (what bounded this step:
-// 28 us for the 512 tokens below): a wave loads 128 consecutive bytes of 8 rows per instruction and turns them in a corner of LDS of
+// Fragments of x read from memory would put neighbouring lanes into different rows, a cache access per lane (28 us against 20 for 512
+// tokens of rank 64): a wave loads 128 consecutive bytes of 8 rows per instruction and turns them in a corner of LDS of
 // its own (16-byte chunks of a row at chunk ^ ((row >> 1) & 7): no bank twice; LDS works in order within a wave, so no barrier).
 // A is stored as its fragments are.
 constexpr int SU = 1;                                       // steps in flight per wave; two: 24.2 us against 20.4 for 512 tokens at rank 64
@@ -355,7 +360,8 @@ void lora_shrink_kernel(const LoraAdapter * __restrict__ ads, int n, const int *
 // A wave owns 64 columns (four fragments of 16) and takes its tokens 16 at a time. u is the A operand, so the result has token
 // 4 (lane >> 4) + i in register i and column lane & 15: a load or store of base and y takes 64 consecutive bytes of 4 tokens, four
 // cache accesses. (The other way round a lane has four columns and an instruction moves 16 bytes per lane, but neighbouring lanes
-// are in different rows, which costs an access per lane: 107 us against 92 for the 4096 tokens below.)
+// are in different rows, which costs an access per lane: 106 us against 100 for 4096 tokens x 4096 -> 14336. Asking for B before u and the
+// base gains nothing: 13.0 us against 12.5 for 48 tokens.)
 struct ExpandWave {
     const int * list; int count;           // tokens
     const float * us; int us_ld;           // scale * u of them, in LDS
@@ -681,8 +687,9 @@ static void lora_two_steps(const LoraSet & l, const LoraWs & w, const LoraCall &
 }
 
 static void lora_launch(const LoraSet & l, const LoraWs & w, const LoraCall & c, hipStream_t s) {
-    // one launch while every workgroup can read all of A in about the time of a launch: 128 KB of F16 7.5 us, two launches 10.8 us
-    if (c.T <= 4 && (int64_t) l.u_ld * l.a_ld * (l.any_f32 ? 4 : 2) <= (256 << 10)) {
+    // one launch while every workgroup can read all of A in about the time of a launch: 1 and 4 tokens in a replayed graph, A of 128 KB
+    // 5.5 and 5.7 us (two launches 8.9 and 9.0), 256 KB 9.1 and 11.4 (9.8), 512 KB 20.2 (10.7 and 11.0)
+    if (c.T <= 4 && (int64_t) l.u_ld * l.a_ld * (l.any_f32 ? 4 : 2) <= (192 << 10)) {
         hipLaunchKernelGGL(lora_fused_kernel, dim3((unsigned) c.T, (unsigned) ((l.n_out + 511) / 512)), dim3(512), 0, s, (const LoraAdapter *) l.dev, l.n, c.ids, c.x, c.ldx, l.n_in, l.a_ld, l.n_out, c.base, c.ldb, c.y, c.ldy);
     } else if (c.T <= 64) lora_two_steps<false>(l, w, c, s);
     else {

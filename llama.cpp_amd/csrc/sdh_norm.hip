@@ -3,7 +3,7 @@
 //   s = x + res,  z = s * w / sqrt(mean(s^2) + eps),  per 32 values d = max|z| / 127, q = rint(z / d).
 //
 // One workgroup per token, the row in registers between the sum of squares and the outputs: every input is read once and the memory
-// bounds it. 8192 rows of 4096 with residual and 8-bit output: 84.6 us, 5.2 TB/s (a large copy: 4.9). A lane holds 4 consecutive
+// bounds it. 8192 rows of 4096 with residual and 8-bit output: 78.1 us, 5.6 TB/s (torch's copy of a large tensor: 4.95). A lane holds 4 consecutive
 // values per step, so eight neighbouring lanes hold a block of 32 and its maximum is three lane exchanges.
 //
 // Arithmetic: s is rounded to F32 (the next layer reads it); from there on everything is in double and rounded once per output.
@@ -29,7 +29,7 @@ struct NormArgs {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 
-// NT: past the L2 (rows that are more than it holds together): 84.6 us against 93.8 for the prompt below
+// NT: past the caches (rows that are more than the L2 holds together): 78.1 us against 92.8 for the prompt above
 template <bool VEC, bool NT = false>
 __device__ __forceinline__ float4 load4(const float * p, int i, int n) {
     if constexpr (VEC && NT) { const v4f v = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(p + i)); return make_float4(v.x, v.y, v.z, v.w); }
@@ -170,7 +170,7 @@ static int launch_norm(const NormArgs & all, int64_t T, hipStream_t s) {
     const bool vec = all.n % 4 == 0 && ok(all.x, all.ldx) && ok(all.res, all.ldr) && ok(all.sum, all.lds) && ok(all.y, all.ldy) && ok(all.w, 0);
     const int q4 = (all.n + 3) / 4;
     // few rows: as many threads as there are groups of four values (one row of 4096: 4.8 us); many: four groups a thread, four
-    // workgroups of 256 for one of 1024 (8192 rows of 4096: 93.8 us against 99.6)
+    // workgroups of 256 for one of 1024 (8192 rows of 4096: 78.1 us against 90.4)
     const int nv = q4 > 4096 ? 0 : q4 > 2048 || (T > 2 * lib().num_cu && q4 >= 1024) ? 4 : q4 > 1024 ? 2 : 1;
     const bool nt = (int64_t) 4 * all.n * T > (32 << 20);
     constexpr int64_t CHUNK = 1 << 21;                      // a launch has fewer than 2^32 threads
