@@ -4,7 +4,7 @@
 // (lora_expand_kernel, K = rank). Tokens are taken by adapter, 32 at a time, so an adapter is read once per 32 of its tokens in
 // whatever order they stand. ids live on the device (a captured graph sees the ids of the replay), so the sorting does too:
 //   up to 64 tokens   a wave sees all ids at once: the first token of an adapter does the work of all of them (no launch for it);
-//   more              lora_plan_kernel sorts the tokens by adapter and cuts them into tiles.
+//   more              lora_plan_kernel sorts the tokens by adapter and cuts them into tiles (no ids, one adapter: nothing to sort).
 // One to four tokens of small adapters take one launch (lora_fused_kernel) in which every workgroup forms u for itself.
 //
 // Kernel times (plan + shrink + expand), and what bounds them: 1 token, rank 16, 4096 -> 14336: 6.3 us (one launch and its chain of
@@ -200,13 +200,19 @@ __device__ __forceinline__ v4f load4x(const float * p, int64_t k, int64_t n) {
 }
 
 // ---- the tokens of a workgroup --------------------------------------------------------------------------------------
-// PLAN: tile `at` of the plan. Otherwise (up to 64 tokens) all tokens of one adapter: with fewer adapters than tokens of adapter `at` (n:
+// PLAN: tile `at` of the plan, without ids of `size` tokens of adapter 0. Otherwise (up to 64 tokens) all tokens of one adapter: with fewer adapters than tokens of adapter `at` (n:
 // none), else of the adapter of token `at`, if that is the first of them. -> the tokens in `list` (a row of LDS of each wave's own: LDS
 // works in order within a wave, no barrier), their number (0: nothing to do here) and the adapter (-1: none)
 template <bool PLAN>
-__device__ __forceinline__ int lora_tokens(const LoraTile * tiles, const int * n_tiles, const int * perm, const int * ids, int T, int n, int at, int * list, int * adapter) {
+__device__ __forceinline__ int lora_tokens(const LoraTile * tiles, const int * n_tiles, const int * perm, const int * ids, int T, int n, int at, int size, int * list, int * adapter) {
     const int lane = threadIdx.x & 63;
     if constexpr (PLAN) {
+        if (!ids) {                                         // all tokens in their order
+            const int start = at * size, count = max(0, min(size, T - start));
+            for (int i = lane; i < count; i += 64) list[i] = start + i;
+            *adapter = 0;
+            return count;
+        }
         const LoraTile tile = tiles[at];
         if (at >= *n_tiles) return 0;
         for (int i = lane; i < tile.count; i += 64) list[i] = perm[tile.start + i];
@@ -345,7 +351,7 @@ void lora_shrink_kernel(const LoraAdapter * __restrict__ ads, int n, const int *
     // same columns of x one after the other
     const int split = (int) (blockIdx.x % (unsigned) splits), rest = (int) (blockIdx.x / (unsigned) splits), rc = rest % n_z * LORA_RC;
     int a = -1;
-    const int count = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, rest / n_z, list, &a);
+    const int count = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, rest / n_z, LT, list, &a);
     const LoraAdapter ad = ads[max(a, 0)];                  // on its way beside the ids where `a` does not come from them
     if (!count || a < 0 || rc >= ad.rank) return;
     const int64_t k0 = split * k_split, k1 = min(a_ld, k0 + k_split);
@@ -423,7 +429,7 @@ void lora_expand_kernel(const LoraAdapter * __restrict__ ads, int n, const int *
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
     int * list = lists[wave];
     int a = -1;
-    const int all = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, at, list, &a);
+    const int all = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, at, ET, list, &a);
     const LoraAdapter ad = ads[max(a, 0)];
     if (!all || (a < 0 && base == y)) return;
     ExpandWave e{list, all, us, 0, 0, n_out, base, ldb, y, ldy};
@@ -673,14 +679,16 @@ static void lora_two_steps(const LoraSet & l, const LoraWs & w, const LoraCall &
     const LoraAdapter * ads = (const LoraAdapter *) l.dev;
     const int64_t k_split = ((l.a_ld + w.splits - 1) / w.splits + 31) / 32 * 32;      // the last ones may be empty
     const int n_z = (l.u_ld + LORA_RC - 1) / LORA_RC;
-    const int64_t few = std::min<int64_t>(c.T, l.n + 1);                              // lora_tokens: by token or by adapter
+    const auto along = [&](int size, int64_t planned) {                               // workgroups along the tokens, as lora_tokens deals them
+        return !PLAN ? std::min<int64_t>(c.T, l.n + 1) : c.ids ? planned : (c.T + size - 1) / size;
+    };
     const auto shrink = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned) ((PLAN ? w.max_tiles : few) * n_z * w.splits)), dim3(256), 0, s, ads, l.n, c.ids, w.tiles, w.n_tiles, w.perm, c.x, c.ldx, l.n_in, l.a_ld, c.T, w.splits, k_split, n_z, w.u, l.u_ld);
+        hipLaunchKernelGGL(kernel, dim3((unsigned) (along(LT, w.max_tiles) * n_z * w.splits)), dim3(256), 0, s, ads, l.n, c.ids, w.tiles, w.n_tiles, w.perm, c.x, c.ldx, l.n_in, l.a_ld, c.T, w.splits, k_split, n_z, w.u, l.u_ld);
     };
     shrink(lora_shrink_kernel<PLAN>);
     const unsigned n_col = (unsigned) ((l.n_out + 255) / 256);
     const auto expand = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned) (PLAN ? w.max_etiles : few) * n_col), dim3(256), (size_t) (16 * (l.u_ld + 4)) * 4, s,
+        hipLaunchKernelGGL(kernel, dim3((unsigned) along(ET, w.max_etiles) * n_col), dim3(256), (size_t) (16 * (l.u_ld + 4)) * 4, s,
                            ads, l.n, c.ids, w.etiles, w.n_tiles + 1, w.perm, w.u, l.u_ld, w.splits, c.T, l.n_out, c.base, c.ldb, c.y, c.ldy);
     };
     expand(lora_expand_kernel<PLAN>);
@@ -693,7 +701,7 @@ static void lora_launch(const LoraSet & l, const LoraWs & w, const LoraCall & c,
         hipLaunchKernelGGL(lora_fused_kernel, dim3((unsigned) c.T, (unsigned) ((l.n_out + 511) / 512)), dim3(512), 0, s, (const LoraAdapter *) l.dev, l.n, c.ids, c.x, c.ldx, l.n_in, l.a_ld, l.n_out, c.base, c.ldb, c.y, c.ldy);
     } else if (c.T <= 64) lora_two_steps<false>(l, w, c, s);
     else {
-        hipLaunchKernelGGL(lora_plan_kernel, dim3(1), dim3(1024), (size_t) (l.n + 2) * 12, s, c.ids, c.T, l.n, w.perm, w.tiles, w.etiles, w.n_tiles);
+        if (c.ids) hipLaunchKernelGGL(lora_plan_kernel, dim3(1), dim3(1024), (size_t) (l.n + 2) * 12, s, c.ids, c.T, l.n, w.perm, w.tiles, w.etiles, w.n_tiles);
         lora_two_steps<true>(l, w, c, s);
     }
 }

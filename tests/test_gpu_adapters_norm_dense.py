@@ -416,6 +416,12 @@ def test_lora_all_none_and_null_ids(hip, T):
     check_lora(ads, None, T)
 
 
+@pytest.mark.parametrize("T", [66, 96, 511, 2000])
+@pytest.mark.parametrize("base", ["apart", "in place", None])
+def test_lora_one_adapter_for_all_tokens(hip, T, base):
+    check_lora(make_adapters(200, 300, [20, 8], ["f", "h"]), None, T, base=base, pad=1, shift=1)
+
+
 @pytest.mark.parametrize("T", [1, 40, 64, 200])
 def test_lora_many_adapters(hip, T):
     n = 4096 if T != 40 else 1000
