@@ -284,12 +284,12 @@ static void launch_thin(const DenseArgs & a, hipStream_t s) {
 // Many tokens: BM tokens x BN rows per workgroup, both operands through LDS in steps of SB blocks, two stages. A wave owns 32 tokens x
 // 32 NN rows; with KS = 2 two waves share them, each with every other block, joined at the end.
 //
-// What bounds it is the vector pipe, to whose time that of the matrix pipe adds (both together issue in every cycle): a 32x32x32 MFMA
-// takes 32 cycles and leaves 16 integers per lane, each of which costs a conversion and a fused multiply-add (packed F32 being off).
-// The products of the scales come from v_mfma_f32_32x32x1_2b_f32, two tiles in 64 cycles (32 vector instructions of 4 cycles
-// otherwise); a step's addresses are one operation each, and the operands' way through registers is left out (loads to LDS), so two
-// tiles take 128 cycles of the matrix pipe and 66 vector instructions. 2048 tokens x 4096 -> 14336: 356 us, 675 TOP/s (products by
-// vector instructions, operands through registers: 424 us).
+// What bounds it is the vector pipe, to whose time that of the matrix pipe adds (562,000 + 229,000 of 743,000 busy cycles per SIMD for
+// 2048 tokens x 4096 -> 14336: 356 us, 675 TOP/s): a 32x32x32 MFMA takes 32 cycles and leaves 16 integers per lane, each of which costs
+// a conversion and a fused multiply-add (packed F32 being off). The products of the scales come from v_mfma_f32_32x32x1_2b_f32, two
+// tiles in 64 cycles (32 vector instructions of 4 cycles otherwise); a step's addresses are one operation each, and the operands' way
+// through registers is left out (loads to LDS), so two tiles take 128 cycles of the matrix pipe and 72 vector instructions, 288 cycles
+// (products by vector instructions and operands through registers: 424 us).
 //   waves      four per SIMD: a wave waits for LDS, MFMA and conversions in turn (four waves of 64 x 64 in the place of eight of 32 x 64:
 //              559 us against 463).
 //   steps      four blocks (128 bytes a row); eight for 64 x 64, which has half the work between two barriers (512 tokens x 2560 ->
