@@ -297,6 +297,40 @@ def test_dense_infinite_scales_stay_infinite(hip, n_in, T):
     w.close()
 
 
+# enough workgroups for each form to be the cheapest one: two tokens of many rows, 32 x 32, 64 x 64, 64 x 128 and 128 x 128 tiles
+FORMS = [(160, 13000, 2), (416, 5000, 70), (1056, 2900, 300), (160, 5000, 700), (288, 4500, 1500), (32, 2900, 300), (64, 4500, 1500)]
+
+
+@pytest.mark.parametrize("n_in, n_out, T", FORMS)
+@pytest.mark.parametrize("pad, shift", [(0, 0), (1, 1)])
+def test_dense_many_workgroups(hip, n_in, n_out, T, pad, shift):
+    run_dense(n_in, n_out, T, seed=n_in, pad=pad, shift=shift)
+
+
+@pytest.mark.parametrize("n_in, n_out, T", FORMS[:5])
+def test_dense_many_workgroups_infinite_scales(hip, n_in, n_out, T):
+    """In the first and the last block, where steps end: infinite outputs stay infinite, the others what they are."""
+    W, q, d = dense_case(n_in, n_out, T, 8)
+    nb = n_in // 32
+    blk = W.reshape(n_out, nb, 34)
+    q[:] = np.maximum(np.abs(q), 1)
+    for o, b, v in ((0, nb - 1, 5), (n_out - 1, 0, 251), (n_out // 2, nb - 1, 7)):
+        blk[o, b, :2] = np.frombuffer(np.float16(np.inf).tobytes(), np.uint8)
+        blk[o, b, 2:] = v                                # one sign, so no sum of theirs is zero
+    d[T - 1, nb - 1] = np.inf
+    w, qd, dd, y = scan.DenseWeight(W), dev(q), dev(d), Out(T, n_out)
+    sublayer.dense_forward_q8_device(w, sublayer.Q8View(qd.data_ptr(), n_in, dd.data_ptr(), nb), T, y.ptr, y.ld)
+    got = y.get()
+    with np.errstate(invalid="ignore"):
+        want, mag = dense_ref(W, q, d)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.isinf(want[:, 0]).all()
+    for value in (np.inf, -np.inf):
+        assert np.array_equal(got == value, want == value)
+    fin = np.isfinite(want)
+    assert np.all(np.abs(got - np.where(fin, want, 0))[fin] <= ((nb + 10) * U * mag)[fin])
+    w.close()
+
+
 def test_dense_refusals(hip):
     q, d, y = torch.zeros(4, 64, dtype=torch.int8, device="cuda"), torch.zeros(4, 2, device="cuda"), torch.zeros(4, 48, device="cuda")
     w = scan.DenseWeight(make_dense(64, 48, "q8_0"))
