@@ -565,21 +565,22 @@ static int lora_check(const char * what, int i, const sdh_tensor & t, int64_t ne
     return SDH_OK;
 }
 
-// t (F16 / F32, any strides) as contiguous rows, as it is or widened
-static std::vector<uint8_t> lora_rows(const sdh_tensor & t, bool f32) {
+// t (F16 / F32, any strides) as contiguous rows, as it is (in place, or copied to `keep`) or widened
+static const void * lora_rows(const sdh_tensor & t, bool f32, std::vector<uint8_t> & keep) {
     const size_t n0 = (size_t) t.ne[0], n1 = (size_t) t.ne[1], es = f32 ? 4 : 2;
-    std::vector<uint8_t> out(n0 * n1 * es);
+    if ((t.type == SDH_TYPE_F32) == f32 && t.nb[0] == (int64_t) es && t.nb[1] == (int64_t) (n0 * es)) return t.data;
+    keep.resize(n0 * n1 * es);
     if (f32) {
         const std::vector<float> v = tensor_f32(t);
-        memcpy(out.data(), v.data(), out.size());
-        return out;
+        memcpy(keep.data(), v.data(), keep.size());
+        return keep.data();
     }
     for (size_t i1 = 0; i1 < n1; ++i1) {
         const uint8_t * row = (const uint8_t *) t.data + (int64_t) i1 * t.nb[1];
-        if (t.nb[0] == 2) memcpy(out.data() + i1 * n0 * 2, row, n0 * 2);
-        else for (size_t i0 = 0; i0 < n0; ++i0) memcpy(out.data() + (i1 * n0 + i0) * 2, row + (int64_t) i0 * t.nb[0], 2);
+        if (t.nb[0] == 2) memcpy(keep.data() + i1 * n0 * 2, row, n0 * 2);
+        else for (size_t i0 = 0; i0 < n0; ++i0) memcpy(keep.data() + (i1 * n0 + i0) * 2, row + (int64_t) i0 * t.nb[0], 2);
     }
-    return out;
+    return keep.data();
 }
 
 // rows of A [rank][n_in] into fragment order (LoraAdapter), E: the element
@@ -638,21 +639,21 @@ static int lora_create(int64_t n_in, int64_t n_out, const sdh_lora_desc * d, int
     if (const int rc = ready_on_device("sdh_lora_create")) return rc;
     SDH_HIP_CHECK(hipMalloc((void **) &l.dev, total));
     struct Guard { uint8_t * p; ~Guard() { if (p) (void) hipFree(p); } } guard{l.dev};
-    std::vector<uint8_t> buf;
+    std::vector<uint8_t> buf, keep;
     auto upload = [&](size_t at, size_t bytes) { return hipMemcpy(l.dev + at, buf.data(), bytes, hipMemcpyHostToDevice); };
     for (int i = 0; i < n; ++i) {
         LoraAdapter & a = tab[(size_t) i];
         const size_t es = a.f32 ? 4 : 2;
         a.a = l.dev + at_a[(size_t) i]; a.b = l.dev + at_b[(size_t) i];
-        std::vector<uint8_t> rows = lora_rows(d[i].a, a.f32 != 0);
+        const void * rows = lora_rows(d[i].a, a.f32 != 0, keep);
         buf.assign((size_t) (a.r_ld * l.a_ld) * es, 0);
-        if (a.f32) lora_pack_a((const float *) rows.data(), a.rank, a.r_ld, n_in, l.a_ld, (float *) buf.data());
-        else       lora_pack_a((const uint16_t *) rows.data(), a.rank, a.r_ld, n_in, l.a_ld, (uint16_t *) buf.data());
+        if (a.f32) lora_pack_a((const float *) rows, a.rank, a.r_ld, n_in, l.a_ld, (float *) buf.data());
+        else       lora_pack_a((const uint16_t *) rows, a.rank, a.r_ld, n_in, l.a_ld, (uint16_t *) buf.data());
         SDH_HIP_CHECK(upload(at_a[(size_t) i], buf.size()));
-        rows = lora_rows(d[i].b, a.f32 != 0);
+        rows = lora_rows(d[i].b, a.f32 != 0, keep);
         buf.assign((size_t) b_rows * (size_t) a.r_ld * es, 0);
-        if (a.f32) lora_pack_b((const float *) rows.data(), a.rank, a.r_ld, n_out, (float *) buf.data());
-        else       lora_pack_b((const uint16_t *) rows.data(), a.rank, a.r_ld, n_out, (uint16_t *) buf.data());
+        if (a.f32) lora_pack_b((const float *) rows, a.rank, a.r_ld, n_out, (float *) buf.data());
+        else       lora_pack_b((const uint16_t *) rows, a.rank, a.r_ld, n_out, (uint16_t *) buf.data());
         SDH_HIP_CHECK(upload(at_b[(size_t) i], buf.size()));
     }
     buf.resize(tab.size() * sizeof(LoraAdapter));
