@@ -3,10 +3,10 @@
 // The integer sum of a block of 32 is exact (at most 32 * 127 * 128 < 2^20); the two scales multiply it once in F32 and the
 // blocks are summed in F32.
 //
-//   dense_few_kernel   one token (two of very many rows): bound by the stream of the weight; v_dot4_i32_i8.
+//   dense_few_kernel   one token: bound by the stream of the weight; v_dot4_i32_i8.
 //   dense_thin_kernel, dense_mid_kernel
-//                      a batch: 16 rows of v_mfma_i32_16x16x32_i8 or 32 x 32 tiles of v_mfma_i32_32x32x32_i8, whose K is exactly one
-//                      block, straight from memory.
+//                      a batch: 16 to 64 rows of v_mfma_i32_16x16x32_i8 or 32 x 32 tiles of v_mfma_i32_32x32x32_i8, whose K is exactly
+//                      one block, straight from memory.
 //   dense_mfma_kernel  a prompt: tiles of 64 x 64 to 128 x 128 through LDS, bound by the vector pipe (integers to F32).
 #include "sdh_internal.h"
 
@@ -187,42 +187,49 @@ __global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
     }
 }
 
-// The same with 16 rows and 16 TT tokens per workgroup: twice the workgroups, so that a weight of some thousand rows reaches every CU
-// (11 tokens x 14336 -> 4096: 11.8 us, 5.3 TB/s, with tiles of 32 x 32 on half of the CUs 22.4; 16 waves instead of 8: 13.5). With three
-// or four workgroups per CU at once (4096 -> 14336) 18.7 us, tiles of 32 x 32 16.8; starting each workgroup at another column 20.5.
+// The same with 16 RR rows and 16 TT tokens per workgroup, for two things that 32 x 32 tiles do badly: a weight of some thousand rows
+// leaves CUs without work (RR = 1: 11 tokens x 14336 -> 4096 11.7 us, 5.4 TB/s, against 22.5), and one of very many rows reads x so often
+// that its way from the L2 counts as much as the weight (RR = 4, one workgroup per CU: 11 tokens x 4096 -> 14336 13.2 us against 16.8, 18.7
+// with RR = 1). RR = 3 where that fills the CUs better. 16 waves instead of 8 gain nothing (13.5 us for the former), nor does starting
+// each workgroup at another column (20.5 us for the latter: x is then no longer shared in the cache).
 //   fragments  v_mfma_i32_16x16x32_i8: lane = row (or token) lane & 15, the 8 bytes lane >> 4 of the block; the result has token
 //              4 (lane >> 4) + i in register i and row lane & 15.
-template <int TT>
-__global__ __launch_bounds__(512, TT == 1 ? 8 : 4) void dense_thin_kernel(const DenseArgs a) {
+template <int TT, int RR>
+__global__ __launch_bounds__(512, TT * RR == 1 ? 8 : TT + RR <= 4 ? 4 : 2) void dense_thin_kernel(const DenseArgs a) {
     constexpr int NW = 8;
-    __shared__ v4i turn[NW][1 + TT][128];                        // per wave: 16 rows of the weight, 16 TT of x
+    __shared__ v4i turn[NW][RR + TT][128];                       // per wave: 16 RR rows of the weight, 16 TT of x
     __shared__ __align__(16) float dxs[NW][4][16 * TT];
-    static_assert(sizeof(turn) >= NW * 16 * TT * 17 * 4, "room for the join");
+    static_assert(sizeof(turn) >= NW * 16 * TT * (16 * RR + 1) * 4, "room for the join");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4, lr = lane >> 3, lc = lane & 7;
-    const int o0 = (int) blockIdx.x * 16;
+    const int o0 = (int) blockIdx.x * (16 * RR);
     const int64_t t0 = (int64_t) blockIdx.y * (16 * TT);
-    const int8_t * wp[2], * xp[2 * TT];
+    const int8_t * wp[2 * RR], * xp[2 * TT];
+    const __half * dwp[RR];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) wp[i] = a.wq + (int64_t) min(o0 + 8 * i + lr, a.n_out - 1) * a.nblk * 32 + 16 * lc;
+    for (int i = 0; i < 2 * RR; ++i) wp[i] = a.wq + (int64_t) min(o0 + 8 * i + lr, a.n_out - 1) * a.nblk * 32 + 16 * lc;
 #pragma unroll
     for (int i = 0; i < 2 * TT; ++i) xp[i] = a.xq + min(t0 + 8 * i + lr, a.T - 1) * a.ldq + 16 * lc;
-    const __half * dwp = a.wd + (int64_t) min(o0 + m, a.n_out - 1) * a.nblk;
+#pragma unroll
+    for (int r = 0; r < RR; ++r) dwp[r] = a.wd + (int64_t) min(o0 + 16 * r + m, a.n_out - 1) * a.nblk;
     const int dxt = TT == 2 ? lane & 31 : m, dxb = TT == 2 ? 2 * (lane >> 5) : g;         // this lane's token and first block (TT: as many)
     const float * dxp = a.xd + min(t0 + dxt, a.T - 1) * a.ldd + dxb;
     const int st = lr * 8 + (lc ^ (lr >> 1)), key = (m >> 1) & 7;       // rows 8 i + lr: 8 more rows flip bit 2 of the key
-    float acc[TT][4];
+    float acc[RR][TT][4];
 #pragma unroll
-    for (int j = 0; j < TT; ++j)
+    for (int r = 0; r < RR; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
-    v4i wn[2], xn[2 * TT];
-    __half dw[4];
+        for (int j = 0; j < TT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[r][j][i] = 0.0f;
+    v4i wn[2 * RR], xn[2 * TT];
+    __half dw[RR][4];
     float dx[TT];
     auto load = [&](int b0) {
         const int bs = min(b0, a.nblk - 4);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) wn[i] = *reinterpret_cast<const v4i *>(wp[i] + (int64_t) bs * 32);
-        __builtin_memcpy(dw, dwp + bs, 8);
+        for (int i = 0; i < 2 * RR; ++i) wn[i] = *reinterpret_cast<const v4i *>(wp[i] + (int64_t) bs * 32);
+#pragma unroll
+        for (int r = 0; r < RR; ++r) __builtin_memcpy(dw[r], dwp[r] + bs, 8);
 #pragma unroll
         for (int i = 0; i < 2 * TT; ++i) xn[i] = *reinterpret_cast<const v4i *>(xp[i] + (int64_t) bs * 32);
         __builtin_memcpy(dx, dxp + bs, 4 * TT);
@@ -230,13 +237,15 @@ __global__ __launch_bounds__(512, TT == 1 ? 8 : 4) void dense_thin_kernel(const 
     load(4 * wave);
     for (int b0 = 4 * wave; b0 < a.nblk; b0 += 4 * NW) {
         const int bs = min(b0, a.nblk - 4);
-        float dc[4];
+        float dc[RR][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) turn[wave][0][64 * i + (i & 1 ? st ^ 4 : st)] = wn[i];
+        for (int i = 0; i < 2 * RR; ++i) turn[wave][i / 2][64 * (i & 1) + (i & 1 ? st ^ 4 : st)] = wn[i];
 #pragma unroll
-        for (int i = 0; i < 2 * TT; ++i) turn[wave][1 + i / 2][64 * (i & 1) + (i & 1 ? st ^ 4 : st)] = xn[i];
+        for (int i = 0; i < 2 * TT; ++i) turn[wave][RR + i / 2][64 * (i & 1) + (i & 1 ? st ^ 4 : st)] = xn[i];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dc[i] = bs + i >= b0 ? __half2float(dw[i]) : 0.0f;
+        for (int r = 0; r < RR; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dc[r][i] = bs + i >= b0 ? __half2float(dw[r][i]) : 0.0f;
 #pragma unroll
         for (int i = 0; i < TT; ++i) dxs[wave][dxb + i][dxt] = bs + dxb + i >= b0 ? dx[i] : 0.0f;
         load(b0 + 4 * NW);                                       // past the end: in bounds and not used
@@ -244,41 +253,46 @@ __global__ __launch_bounds__(512, TT == 1 ? 8 : 4) void dense_thin_kernel(const 
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int at = 2 * (m * 8 + ((2 * k + (g >> 1)) ^ key)) + (g & 1);         // 8 bytes
-            const long w = reinterpret_cast<const long *>(turn[wave][0])[at];
 #pragma unroll
             for (int j = 0; j < TT; ++j) {
-                v4i z = {};
-                z = __builtin_amdgcn_mfma_i32_16x16x32_i8(reinterpret_cast<const long *>(turn[wave][1 + j])[at], w, z, 0, 0, 0);
+                const long xf = reinterpret_cast<const long *>(turn[wave][RR + j])[at];
                 const float4 d = *reinterpret_cast<const float4 *>(&dxs[wave][k][16 * j + 4 * g]);
-                acc[j][0] = fmaf((float) z[0], d.x * dc[k], acc[j][0]);
-                acc[j][1] = fmaf((float) z[1], d.y * dc[k], acc[j][1]);
-                acc[j][2] = fmaf((float) z[2], d.z * dc[k], acc[j][2]);
-                acc[j][3] = fmaf((float) z[3], d.w * dc[k], acc[j][3]);
+#pragma unroll
+                for (int r = 0; r < RR; ++r) {
+                    v4i z = {};
+                    z = __builtin_amdgcn_mfma_i32_16x16x32_i8(xf, reinterpret_cast<const long *>(turn[wave][r])[at], z, 0, 0, 0);
+                    acc[r][j][0] = fmaf((float) z[0], d.x * dc[r][k], acc[r][j][0]);
+                    acc[r][j][1] = fmaf((float) z[1], d.y * dc[r][k], acc[r][j][1]);
+                    acc[r][j][2] = fmaf((float) z[2], d.z * dc[r][k], acc[r][j][2]);
+                    acc[r][j][3] = fmaf((float) z[3], d.w * dc[r][k], acc[r][j][3]);
+                }
             }
         }
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    float * part = reinterpret_cast<float *>(turn);              // [NW][16 TT][17]
+    float * part = reinterpret_cast<float *>(turn);              // [NW][16 TT][16 RR + 1]
 #pragma unroll
-    for (int j = 0; j < TT; ++j)
+    for (int r = 0; r < RR; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) part[(wave * 16 * TT + 16 * j + 4 * g + i) * 17 + m] = acc[j][i];
+        for (int j = 0; j < TT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[(wave * 16 * TT + 16 * j + 4 * g + i) * (16 * RR + 1) + 16 * r + m] = acc[r][j][i];
     __syncthreads();
-    for (int e = threadIdx.x; e < 256 * TT; e += 64 * NW) {
-        const int t = e >> 4, c = e & 15;
+    for (int e = threadIdx.x; e < 256 * TT * RR; e += 64 * NW) {
+        const int t = e / (16 * RR), c = e % (16 * RR);
         if (t0 + t < a.T && o0 + c < a.n_out) {
             float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) v += part[(w * 16 * TT + t) * 17 + c];
+            for (int w = 0; w < NW; ++w) v += part[(w * 16 * TT + t) * (16 * RR + 1) + c];
             a.y[(t0 + t) * a.ldy + o0 + c] = v;
         }
     }
 }
 
-template <int TT>
+template <int TT, int RR>
 static void launch_thin(const DenseArgs & a, hipStream_t s) {
-    hipLaunchKernelGGL(dense_thin_kernel<TT>, dim3((unsigned) ((a.n_out + 15) / 16), (unsigned) ((a.T + 16 * TT - 1) / (16 * TT))), dim3(512), 0, s, a);
+    hipLaunchKernelGGL((dense_thin_kernel<TT, RR>), dim3((unsigned) ((a.n_out + 16 * RR - 1) / (16 * RR)), (unsigned) ((a.T + 16 * TT - 1) / (16 * TT))), dim3(512), 0, s, a);
 }
 
 // Many tokens: BM tokens x BN rows per workgroup, both operands through LDS in steps of SB blocks, two stages. A wave owns 32 tokens x
@@ -438,39 +452,58 @@ static void launch_mfma(const DenseArgs & a, hipStream_t s) {
     hipLaunchKernelGGL((dense_mfma_kernel<BM, BN, NN, KS, SB>), dim3((unsigned) ((n_pan + 7) / 8 * 8 * n_tt)), dim3(BM * BN / 16 / NN * KS), 0, s, a, n_tt);
 }
 
+static void launch_mid(const DenseArgs & a, hipStream_t s) {
+    hipLaunchKernelGGL(dense_mid_kernel, dim3((unsigned) ((a.n_out + 31) / 32), (unsigned) ((a.T + 31) / 32)), dim3(512), 0, s, a);
+}
+
+// The forms from 2 tokens on: tile of tokens x rows, and its time in us per 128 bytes of K: per round in which the workgroups fill the CUs
+// (workgroups per CU, rounded up), plus `add`, `least` at least. `blocks`: the fewest blocks of a row; before that the start and the end
+// of a large tile count for more than its rounds (48 tokens x 1152 -> 6912: 32 x 64 8.9 us, 32 x 32 6.6). Fitted to nine shapes between 1152 and 28672 at 2 to 2048 tokens (a
+// call's time less 2 us). What the choice is worth, us:
+//   14336 -> 4096    11 tokens  16 x 16 11.7, 16 x 48 23, 16 x 64 29, 32 x 32 22.5;    32 tokens  32 x 16 17, 32 x 32 23, 32 x 64 39;
+//                    64 / 256 / 512 / 2048 tokens  32 x 32 23 / 79 / 156 / 642, 64 x 64 65 / 66 / 103 / 447, 64 x 128 120 / 114 / 116 / 425,
+//                    128 x 128 189 / 205 / 205 / 340
+//   4096 -> 14336    11 tokens  16 x 16 18.7, 16 x 48 18.3, 16 x 64 13.2, 32 x 32 16.8;  32 tokens  32 x 16 21, 32 x 32 18.3, 32 x 48 24, 32 x 64 17.1;
+//                    64 / 256 / 512 / 2048 tokens  32 x 32 30 / 96 / 183 / 723, 64 x 64 23 / 57 / 103 / 465, 64 x 128 38 / 55 / 104 / 426,
+//                    128 x 128 55 / 61 / 94 / 348
+//   2560 -> 10240    16 tokens  16 x 16 8.3, 16 x 48 7.8, 16 x 64 9.0, 32 x 32 10.5;    32 tokens  32 x 16 11.0, 32 x 32 11.7, 32 x 48 10.0, 32 x 64 11.5
+struct DenseForm {
+    int tokens, rows, blocks;
+    double per, add, least;
+    void (*launch)(const DenseArgs &, hipStream_t);
+};
+static const DenseForm dense_forms[] = {
+    {16, 16, 4, 0.115, 0, 0, launch_thin<1, 1>},
+    {16, 48, 64, 0.29, 0, 0, launch_thin<1, 3>},
+    {16, 64, 64, 0.37, 0, 0, launch_thin<1, 4>},
+    {32, 16, 4, 0.145, 0, 0, launch_thin<2, 1>},
+    {32, 32, 4, 0.24, 0, 0, launch_mid},
+    {32, 48, 64, 0.42, 0, 0, launch_thin<2, 3>},
+    {32, 64, 64, 0.47, 0, 0, launch_thin<2, 4>},
+    {64, 64, 4, 0.46, 0.1, 0, launch_mfma<64, 64, 1, 2, 8>},
+    {64, 128, 4, 0.92, 0, 1.05, launch_mfma<64, 128, 1, 1, 4>},
+    {128, 128, 4, 1.54, 0, 1.85, launch_mfma<128, 128, 2, 1, 4>},
+};
+
 static int launch_dense(const DenseArgs & all, hipStream_t s) {
-    // Which form, from 2 tokens on: us per 128 bytes of K, by the rounds in which the workgroups fill the CUs (r = workgroups per CU,
-    // rounded up), fitted to eight shapes between 1152 and 28672 at 2 to 2048 tokens:
-    //   16 rows (thin) x 16 tokens 0.115 r, x 32 0.145 r;  32 x 32 (mid) 0.21 r + 0.03;  64 x 64, two waves per tile 0.46 r + 0.1;
-    //   64 x 128 0.92 r, 1.05 at least;  128 x 128 1.54 r, 1.85 at least
-    // 14336 -> 4096, us at 11 / 32 / 64 / 256 / 512 / 2048 tokens: thin 11.8 / 17.3 / 32 / - / - / -, mid 22.5 / 23.0 / 23.2 / 79 / 156 / 642,
-    // 64 x 64 - / - / 65 / 66 / 103 / 447, 64 x 128 - / - / 120 / 114 / 116 / 425, 128 x 128 - / - / 189 / 205 / 205 / 340;
-    // 4096 -> 14336: 18.7 / 21.4 / 35 / - / - / -, 16.8 / 18.3 / 30 / 96 / 183 / 723, - / - / 23 / 57 / 103 / 465, - / - / 38 / 55 / 104 / 426,
-    // - / - / 55 / 61 / 94 / 348.
-    auto rounds = [&](int bm, int bn) {
-        const int64_t wg = ((all.T + bm - 1) / bm) * ((all.n_out + bn - 1) / bn), cu = lib().num_cu;
-        return (double) ((wg + cu - 1) / cu);
-    };
-    const double thin = rounds(16, 16);
-    const double cost[6] = {0.115 * thin, 0.145 * rounds(32, 16), 0.21 * rounds(32, 32) + 0.03, 0.46 * rounds(64, 64) + 0.1,
-                            std::max(1.05, 0.92 * rounds(64, 128)), std::max(1.85, 1.54 * rounds(128, 128))};
-    const int form = (int) (std::min_element(cost, cost + 6) - cost);
+    const DenseForm * form = nullptr;                       // none with fewer than four blocks
+    double best = 0.0;
+    for (const DenseForm & f : dense_forms) {
+        if (all.nblk < f.blocks) continue;
+        const int64_t wg = ((all.T + f.tokens - 1) / f.tokens) * ((all.n_out + f.rows - 1) / f.rows), cu = lib().num_cu;
+        const double cost = std::max(f.least, f.per * (double) ((wg + cu - 1) / cu) + f.add);
+        if (!form || cost < best) { form = &f; best = cost; }
+    }
     // a launch has fewer than 2^32 threads, 65535 workgroups in its second dimension: tokens in chunks for very many of them
     const int64_t n_pan = (all.n_out + 63) / 64, chunk = std::max<int64_t>(1, std::min<int64_t>(1000, (1 << 21) / n_pan)) * 128;
     for (int64_t t0 = 0; t0 < all.T; t0 += chunk) {
         DenseArgs a = all;
         a.T = std::min(chunk, all.T - t0);
         a.xq += t0 * a.ldq; a.xd += t0 * a.ldd; a.y += t0 * a.ldy;
-        // one token: 4096 -> 14336 11.6 us (thin 16.5), 14336 -> 4096 13.3 (11.5); two tokens of very many rows: 15.0 us (thin 17.1, mid
-        // 16.9), else thin (14336 -> 4096: 16.5 us, thin 11.2); fewer than four blocks: no group for the others
+        // one token: 4096 -> 14336 11.6 us (16 x 64 tiles 12.7), 14336 -> 4096 13.3 (16 x 16 11.5), 6912 -> 1152 5.1 (6.3)
         if (all.T == 1)       { if (a.nblk >= 96) launch_few<1, 2, 4>(a, s); else launch_few<1, 2, 2>(a, s); }
-        else if ((all.T == 2 && thin >= 4) || a.nblk < 4) launch_few<2, 2, 4>(a, s);
-        else if (form == 0) launch_thin<1>(a, s);
-        else if (form == 1) launch_thin<2>(a, s);
-        else if (form == 2) hipLaunchKernelGGL(dense_mid_kernel, dim3((unsigned) ((a.n_out + 31) / 32), (unsigned) ((a.T + 31) / 32)), dim3(512), 0, s, a);
-        else if (form == 3) launch_mfma<64, 64, 1, 2, 8>(a, s);
-        else if (form == 4) launch_mfma<64, 128, 1, 1, 4>(a, s);
-        else                launch_mfma<128, 128, 2, 1, 4>(a, s);
+        else if (form)        form->launch(a, s);
+        else                  launch_few<2, 2, 4>(a, s);
     }
     SDH_HIP_CHECK(hipGetLastError());
     return SDH_OK;

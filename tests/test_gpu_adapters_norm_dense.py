@@ -297,8 +297,10 @@ def test_dense_infinite_scales_stay_infinite(hip, n_in, T):
     w.close()
 
 
-# enough workgroups for each form to be the cheapest one: two tokens of many rows, 32 x 32, 64 x 64, 64 x 128 and 128 x 128 tiles
-FORMS = [(160, 13000, 2), (416, 5000, 70), (1056, 2900, 300), (160, 5000, 700), (288, 4500, 1500), (32, 2900, 300), (64, 4500, 1500)]
+# enough workgroups for each form to be the cheapest one: 16 x 16, 32 x 32, 64 x 64, 64 x 128, 128 x 128 tiles, rows of one and two blocks,
+# tiles of 48 and 64 rows
+FORMS = [(160, 13000, 2), (416, 5000, 70), (1056, 2900, 300), (160, 5000, 700), (288, 4500, 1500), (32, 2900, 300), (64, 4500, 1500),
+         (2080, 10001, 9), (2112, 14003, 16), (2080, 10010, 29), (2112, 14001, 25)]
 
 
 @pytest.mark.parametrize("n_in, n_out, T", FORMS)
@@ -307,7 +309,7 @@ def test_dense_many_workgroups(hip, n_in, n_out, T, pad, shift):
     run_dense(n_in, n_out, T, seed=n_in, pad=pad, shift=shift)
 
 
-@pytest.mark.parametrize("n_in, n_out, T", FORMS[:5])
+@pytest.mark.parametrize("n_in, n_out, T", FORMS[:5] + FORMS[7:])
 def test_dense_many_workgroups_infinite_scales(hip, n_in, n_out, T):
     """In the first and the last block, where steps end: infinite outputs stay infinite, the others what they are."""
     W, q, d = dense_case(n_in, n_out, T, 8)
