@@ -4,7 +4,8 @@
 // (lora_expand_kernel, K = rank). Tokens are taken by adapter, 32 at a time, so an adapter is read once per 32 of its tokens in
 // whatever order they stand. ids live on the device (a captured graph sees the ids of the replay), so the sorting does too:
 //   up to 64 tokens   a wave sees all ids at once: the first token of an adapter does the work of all of them (no launch for it);
-//   more              lora_plan_kernel sorts the tokens by adapter and cuts them into tiles (no ids, one adapter: nothing to sort).
+//   more              of few adapters the same up to 256 tokens; else lora_plan_kernel sorts the tokens by adapter and cuts them into
+//                     tiles (no ids, one adapter: nothing to sort).
 // One to four tokens of small adapters take one launch (lora_fused_kernel) in which every workgroup forms u for itself.
 //
 // Kernel times (plan + shrink + expand), and what bounds them: 1 token, rank 16, 4096 -> 14336: 6.3 us (one launch and its chain of
@@ -48,6 +49,7 @@ constexpr int LT = 32;                     // tokens per tile of the shrink kern
 constexpr int ET = 16;                     // ... of the expand kernel
 constexpr int LORA_RC = 32;                // ranks per workgroup of the shrink kernel
 constexpr int LORA_SPLITS = 16;            // its most splits of the columns
+constexpr int LORA_SCAN_T = 256;           // most tokens that a wave deals from the ids alone
 constexpr int64_t LORA_WGS = 384;          // no more splits where tiles times splits would pass this
 
 struct LoraTile { int adapter, start, count, pad; };       // adapter -1: none
@@ -200,13 +202,19 @@ __device__ __forceinline__ v4f load4x(const float * p, int64_t k, int64_t n) {
 }
 
 // ---- the tokens of a workgroup --------------------------------------------------------------------------------------
-// PLAN: tile `at` of the plan, without ids of `size` tokens of adapter 0. Otherwise (up to 64 tokens) all tokens of one adapter: with fewer adapters than tokens of adapter `at` (n:
-// none), else of the adapter of token `at`, if that is the first of them. -> the tokens in `list` (a row of LDS of each wave's own: LDS
-// works in order within a wave, no barrier), their number (0: nothing to do here) and the adapter (-1: none)
-template <bool PLAN>
+// How the tokens are dealt to workgroups:
+//   LORA_FEW   up to 64 tokens: all tokens of one adapter; with fewer adapters than tokens of adapter `at` (n: none), else of the adapter
+//              of token `at`, if that is the first of them;
+//   LORA_SCAN  up to LORA_SCAN_T tokens of few adapters (n < 64): tile `at` of `size` tokens, found by every wave from the ids. Lane b
+//              counts adapter b (n: none);
+//   LORA_PLAN  tile `at` of the plan, or without ids of `size` tokens of adapter 0.
+// -> the tokens in `list` (a row of LDS of each wave's own: LDS works in order within a wave, no barrier), their number (0: nothing to do
+// here) and the adapter (-1: none)
+enum LoraDeal { LORA_FEW, LORA_SCAN, LORA_PLAN };
+template <LoraDeal DEAL>
 __device__ __forceinline__ int lora_tokens(const LoraTile * tiles, const int * n_tiles, const int * perm, const int * ids, int T, int n, int at, int size, int * list, int * adapter) {
     const int lane = threadIdx.x & 63;
-    if constexpr (PLAN) {
+    if constexpr (DEAL == LORA_PLAN) {
         if (!ids) {                                         // all tokens in their order
             const int start = at * size, count = max(0, min(size, T - start));
             for (int i = lane; i < count; i += 64) list[i] = start + i;
@@ -218,6 +226,40 @@ __device__ __forceinline__ int lora_tokens(const LoraTile * tiles, const int * n
         for (int i = lane; i < tile.count; i += 64) list[i] = perm[tile.start + i];
         *adapter = tile.adapter;
         return tile.count;
+    }
+    if constexpr (DEAL == LORA_SCAN) {
+        constexpr int C = LORA_SCAN_T / 64;
+        int a[C], count = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            a[c] = -1;                                      // no token
+            if (64 * c + lane < T) { a[c] = ids[64 * c + lane]; if ((unsigned) a[c] >= (unsigned) n) a[c] = n; }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            for (unsigned long long left = __ballot(a[c] >= 0); left;) {
+                const int one = __builtin_amdgcn_readlane(a[c], __ffsll(left) - 1);
+                const unsigned long long m = __ballot(a[c] == one);
+                if (lane == one) count += __popcll(m);
+                left &= ~m;
+            }
+        const int n_t = (count + size - 1) / size;
+        int first = n_t;
+        for (int m = 1; m < 64; m <<= 1) { const int up = __shfl_up(first, m, 64); if (lane >= m) first += up; }
+        first -= n_t;
+        const unsigned long long own = __ballot(at >= first && at < first + n_t);
+        if (!own) return 0;
+        const int mine = __ffsll(own) - 1, from = (at - __builtin_amdgcn_readlane(first, mine)) * size;
+        int seen = -from;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const unsigned long long m = __ballot(a[c] == mine);
+            const int i = seen + __popcll(m & ((1ull << lane) - 1));
+            if (a[c] == mine && i >= 0 && i < size) list[i] = 64 * c + lane;
+            seen += __popcll(m);
+        }
+        *adapter = mine < n ? mine : -1;
+        return min(seen, size);
     }
     int a = lane < T ? (ids ? ids[lane] : 0) : -2;          // -2: no token
     if (lane < T && (unsigned) a >= (unsigned) n) a = -1;
@@ -339,7 +381,7 @@ __device__ void shrink_tile(const LoraAdapter & ad, const int * list, int count,
     __syncthreads();
 }
 
-template <bool PLAN>
+template <LoraDeal DEAL>
 __global__ __launch_bounds__(256, 3)
 void lora_shrink_kernel(const LoraAdapter * __restrict__ ads, int n, const int * __restrict__ ids, const LoraTile * __restrict__ tiles, const int * __restrict__ n_tiles,
                         const int * __restrict__ perm, const float * __restrict__ x, int64_t ldx, int64_t n_in, int64_t a_ld, int64_t T, int splits, int64_t k_split, int n_z,
@@ -351,7 +393,7 @@ void lora_shrink_kernel(const LoraAdapter * __restrict__ ads, int n, const int *
     // same columns of x one after the other
     const int split = (int) (blockIdx.x % (unsigned) splits), rest = (int) (blockIdx.x / (unsigned) splits), rc = rest % n_z * LORA_RC;
     int a = -1;
-    const int count = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, rest / n_z, LT, list, &a);
+    const int count = lora_tokens<DEAL>(tiles, n_tiles, perm, ids, (int) T, n, rest / n_z, LT, list, &a);
     const LoraAdapter ad = ads[max(a, 0)];                  // on its way beside the ids where `a` does not come from them
     if (!count || a < 0 || rc >= ad.rank) return;
     const int64_t k0 = split * k_split, k1 = min(a_ld, k0 + k_split);
@@ -417,19 +459,19 @@ __device__ __forceinline__ void expand_mult(const ExpandWave & e, const W * b_al
     }
 }
 
-template <bool PLAN>
+template <LoraDeal DEAL>
 __global__ __launch_bounds__(256, 5)
 void lora_expand_kernel(const LoraAdapter * __restrict__ ads, int n, const int * __restrict__ ids, const LoraTile * __restrict__ tiles, const int * __restrict__ n_tiles,
                         const int * __restrict__ perm, const float * __restrict__ u, int u_ld, int splits, int64_t T, int64_t n_out,
                         const float * base, int64_t ldb, float * y, int64_t ldy) {
     extern __shared__ __align__(16) float us[];             // [16][r_ld + 4]
-    __shared__ int lists[4][PLAN ? ET : 64];
+    __shared__ int lists[4][DEAL == LORA_FEW ? 64 : ET];
     // neighbouring workgroups take neighbouring columns of the same tokens
     const int n_col = (int) ((n_out + 255) >> 8), at = (int) (blockIdx.x / (unsigned) n_col), col = (int) (blockIdx.x % (unsigned) n_col);
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
     int * list = lists[wave];
     int a = -1;
-    const int all = lora_tokens<PLAN>(tiles, n_tiles, perm, ids, (int) T, n, at, ET, list, &a);
+    const int all = lora_tokens<DEAL>(tiles, n_tiles, perm, ids, (int) T, n, at, ET, list, &a);
     const LoraAdapter ad = ads[max(a, 0)];
     if (!all || (a < 0 && base == y)) return;
     ExpandWave e{list, all, us, 0, 0, n_out, base, ldb, y, ldy};
@@ -675,24 +717,24 @@ static int sdh_lora_create_impl(int64_t n_in, int64_t n_out, const sdh_lora_desc
 
 struct LoraCall { const int * ids; const float * x; int64_t ldx, T; const float * base; int64_t ldb; float * y; int64_t ldy; };
 
-template <bool PLAN>
+template <LoraDeal DEAL>
 static void lora_two_steps(const LoraSet & l, const LoraWs & w, const LoraCall & c, hipStream_t s) {
     const LoraAdapter * ads = (const LoraAdapter *) l.dev;
     const int64_t k_split = ((l.a_ld + w.splits - 1) / w.splits + 31) / 32 * 32;      // the last ones may be empty
     const int n_z = (l.u_ld + LORA_RC - 1) / LORA_RC;
     const auto along = [&](int size, int64_t planned) {                               // workgroups along the tokens, as lora_tokens deals them
-        return !PLAN ? std::min<int64_t>(c.T, l.n + 1) : c.ids ? planned : (c.T + size - 1) / size;
+        return DEAL == LORA_FEW ? std::min<int64_t>(c.T, l.n + 1) : c.ids ? planned : (c.T + size - 1) / size;
     };
     const auto shrink = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned) (along(LT, w.max_tiles) * n_z * w.splits)), dim3(256), 0, s, ads, l.n, c.ids, w.tiles, w.n_tiles, w.perm, c.x, c.ldx, l.n_in, l.a_ld, c.T, w.splits, k_split, n_z, w.u, l.u_ld);
     };
-    shrink(lora_shrink_kernel<PLAN>);
+    shrink(lora_shrink_kernel<DEAL>);
     const unsigned n_col = (unsigned) ((l.n_out + 255) / 256);
     const auto expand = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned) along(ET, w.max_etiles) * n_col), dim3(256), (size_t) (16 * (l.u_ld + 4)) * 4, s,
                            ads, l.n, c.ids, w.etiles, w.n_tiles + 1, w.perm, w.u, l.u_ld, w.splits, c.T, l.n_out, c.base, c.ldb, c.y, c.ldy);
     };
-    expand(lora_expand_kernel<PLAN>);
+    expand(lora_expand_kernel<DEAL>);
 }
 
 static void lora_launch(const LoraSet & l, const LoraWs & w, const LoraCall & c, hipStream_t s) {
@@ -700,10 +742,14 @@ static void lora_launch(const LoraSet & l, const LoraWs & w, const LoraCall & c,
     // 5.5 and 5.7 us (two launches 8.9 and 9.0), 256 KB 9.1 and 11.4 (9.8), 512 KB 20.2 (10.7 and 11.0)
     if (c.T <= 4 && (int64_t) l.u_ld * l.a_ld * (l.any_f32 ? 4 : 2) <= (192 << 10)) {
         hipLaunchKernelGGL(lora_fused_kernel, dim3((unsigned) c.T, (unsigned) ((l.n_out + 511) / 512)), dim3(512), 0, s, (const LoraAdapter *) l.dev, l.n, c.ids, c.x, c.ldx, l.n_in, l.a_ld, l.n_out, c.base, c.ldb, c.y, c.ldy);
-    } else if (c.T <= 64) lora_two_steps<false>(l, w, c, s);
+    } else if (c.T <= 64) lora_two_steps<LORA_FEW>(l, w, c, s);
+    // a wave finds its tokens in a step per adapter and 64 tokens, while these steps take less than the plan's launch: 128 / 256 tokens of 3
+    // adapters in any order 20.5 / 26.6 us against 24.3 / 29.7 (rank 64, 14336 -> 4096), 128 of 15 16.5 against 20.0 (rank 16, 4096 -> 14336),
+    // but 256 of 15 27.0 against 23.7 and 512 of 3 30.4 against 29.3
+    else if (c.ids && c.T <= LORA_SCAN_T && (c.T + 63) / 64 * (l.n + 1) <= 32) lora_two_steps<LORA_SCAN>(l, w, c, s);
     else {
         if (c.ids) hipLaunchKernelGGL(lora_plan_kernel, dim3(1), dim3(1024), (size_t) (l.n + 2) * 12, s, c.ids, c.T, l.n, w.perm, w.tiles, w.etiles, w.n_tiles);
-        lora_two_steps<true>(l, w, c, s);
+        lora_two_steps<LORA_PLAN>(l, w, c, s);
     }
 }
 

@@ -452,6 +452,13 @@ def test_lora_all_none_and_null_ids(hip, T):
     check_lora(ads, None, T)
 
 
+@pytest.mark.parametrize("T", [65, 127, 128, 129, 200, 255, 256, 257, 513])
+@pytest.mark.parametrize("n", [1, 2, 7, 9, 10, 15, 16, 63])
+@pytest.mark.parametrize("order", ["runs", "gaps"])
+def test_lora_some_hundred_tokens(hip, T, n, order):
+    check_lora(make_adapters(40, 70, [1 + 7 * i % 20 for i in range(n)], ["h", "f"] * n, seed=n), some_ids(T, n, order, T), T, base="in place" if T % 2 else None)
+
+
 @pytest.mark.parametrize("T", [66, 96, 511, 2000])
 @pytest.mark.parametrize("base", ["apart", "in place", None])
 def test_lora_one_adapter_for_all_tokens(hip, T, base):
