@@ -158,7 +158,7 @@ void lora_plan_kernel(const int * __restrict__ ids, int64_t T, int n, int * __re
         return;
     }
     for (int64_t t = tid; t < t_end; t += 4096) {
-        const int b[4] = {bin(t), bin(t + 1024), bin(t + 2048), bin(t + 3072)};
+        const int b[4] = {bin(t), bin(t + 1024), bin(t + 2 * 1024), bin(t + 3 * 1024)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int place = count_in(b[i]);
