@@ -333,6 +333,24 @@ def test_dense_many_workgroups_infinite_scales(hip, n_in, n_out, T):
     w.close()
 
 
+@pytest.mark.parametrize("n_in, n_out, T", [(160, 64, 1), (96, 64, 5), (320, 200, 9)] + FORMS[:5])
+@pytest.mark.parametrize("scale", [1e-36, 1e-39])
+def test_dense_scales_below_the_normal_range(hip, n_in, n_out, T, scale):
+    """Products of scales in F32's subnormal range keep its resolution of 2^-149: half a step per block, times the block's integer sum."""
+    W, q, d = dense_case(n_in, n_out, T, 9)
+    d[:] = (np.abs(np.random.default_rng(1).standard_normal(d.shape)) * scale).astype(np.float32)
+    w, qd, dd, y = scan.DenseWeight(W), dev(q), dev(d), Out(T, n_out)
+    sublayer.dense_forward_q8_device(w, sublayer.Q8View(qd.data_ptr(), n_in, dd.data_ptr(), n_in // 32), T, y.ptr, y.ld)
+    got = y.get()
+    want, mag = dense_ref(W, q, d)
+    ones = W.reshape(n_out, -1, 34).copy()
+    ones[:, :, :2] = np.frombuffer(np.float16(1).tobytes(), np.uint8)
+    _, sums = dense_ref(ones.reshape(W.shape), q, np.ones_like(d))
+    nb = n_in // 32
+    assert np.all(np.abs(got.astype(np.float64) - want) <= (nb + 10) * U * mag + 2.0 ** -150 * sums + nb * 2.0 ** -149)
+    w.close()
+
+
 def test_dense_refusals(hip):
     q, d, y = torch.zeros(4, 64, dtype=torch.int8, device="cuda"), torch.zeros(4, 2, device="cuda"), torch.zeros(4, 48, device="cuda")
     w = scan.DenseWeight(make_dense(64, 48, "q8_0"))
