@@ -197,6 +197,29 @@ def test_quantize_ties_go_to_the_even_step(hip):
     assert q.get()[0, :9].tolist() == [127, 0, 2, 2, 0, -2, -2, 126, -126]
 
 
+@pytest.mark.parametrize("n", [2016, 20000])
+def test_quantize_exact_ties_whatever_the_step(hip, n):
+    """A block of maximum 127 k has the step k exactly, and (j + 1/2) k lies exactly between two steps, however 127 / (127 k) rounds:
+    the even one for every k and j. Their neighbours in F32 on either side go to the step that is nearer."""
+    rng = np.random.default_rng(n)
+    T = 40
+    k = rng.integers(1, 2000, (T, n // 32, 1)).astype(np.float32)
+    k[0, :4, 0] = 49, 98, 103, 107                       # 73.5 / 49 = 1.5, where 73.5 * (127 / 6223) is below it
+    k *= np.float32(2.0) ** rng.integers(-20, 20, k.shape).astype(np.float32)
+    j = rng.integers(-127, 127, (T, n // 32, 32)).astype(np.float32)
+    x = (j + np.float32(0.5)) * k                        # exact: 8 + 11 bits
+    side = rng.integers(-1, 2, x.shape).astype(np.float32)
+    x = np.where(side == 0, x, np.nextafter(x, np.copysign(np.float32(np.inf), side)))
+    x[0, :4, 1] = 1.5 * k[0, :4, 0]
+    x[:, :, :1] = 127 * k
+    q, d = Out(T, n, dtype=torch.int8), Out(T, n // 32)
+    xd = dev(x.reshape(T, n))
+    sublayer.q8_quantize_device(xd.data_ptr(), n, n, T, sublayer.Q8View(q.ptr, q.ld, d.ptr, d.ld))
+    assert np.array_equal(d.get(), k[:, :, 0])
+    # x / k in 64 bits is exact at a tie and on the right side of it elsewhere (a neighbour is 2^-24 of it away)
+    assert np.array_equal(q.get(), np.rint(x.astype(np.float64) / k).astype(np.int8).reshape(T, n))
+
+
 # ---- dense ----------------------------------------------------------------------------------------------------------
 def dense_case(n_in, n_out, T, seed=0, extreme=False):
     rng = np.random.default_rng(seed)
