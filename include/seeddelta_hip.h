@@ -318,8 +318,8 @@ typedef struct sdh_q8 {
  * out8 (may be NULL): z in 8 bits, per block of 32: d = max|z| / 127, q = z / d rounded to the nearest integer, ties to even.
  * s is rounded to F32; the mean, z and the division are formed in 64 bits and each output is rounded once: a value next to the
  * border of two 8-bit steps goes to the right one. The bits of an output do not depend on which others are asked for. A block
- * that holds a value that is not finite gets a scale that is not finite and quants of zero (all 32 values stand for NaN); a
- * block of zeros gets d = 0.
+ * that holds a value that is not finite, or whose scale leaves F32, gets a scale that is not finite and quants of zero (all 32
+ * values stand for NaN); a block of zeros gets d = 0.
  * n >= 1; with out8 n % 32 == 0. */
 int sdh_rms_norm(const float * x, int64_t ldx, const float * res, int64_t ldr, const float * weight, float eps,
                  int64_t n, int64_t n_tokens, float * sum, int64_t lds, float * y, int64_t ldy, const sdh_q8 * out8,

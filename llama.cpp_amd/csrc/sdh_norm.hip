@@ -88,7 +88,7 @@ __device__ __forceinline__ void emit4(const NormArgs & a, int64_t t, int i, bool
         m = umax64(m, __shfl_xor(m, 1, 64)); m = umax64(m, __shfl_xor(m, 2, 64)); m = umax64(m, __shfl_xor(m, 4, 64));
         const double amax = __longlong_as_double((long long) m);
         const float d = (float) (m < 0x7ff0000000000000ull ? quotient(amax, 127.0, 1.0 / 127.0) : amax);
-        const bool fine = d > 0.0f && m < 0x7ff0000000000000ull;     // zeros, and blocks that are not finite: quants of 0
+        const bool fine = d > 0.0f && d < INFINITY;          // zeros, and blocks that are not finite (the scale of F32 decides): quants of 0
         unsigned b = 0;
         if (fine) {
             // z / d = 127 z / amax. z times a rounded 127 / amax would not do: a tie (z F32: 127 z is exact) has to come out as itself,

@@ -197,6 +197,19 @@ def test_quantize_ties_go_to_the_even_step(hip):
     assert q.get()[0, :9].tolist() == [127, 0, 2, 2, 0, -2, -2, 126, -126]
 
 
+def test_norm_scale_past_the_range(hip):
+    """A block of z whose scale leaves F32 is not finite: quants of zero, as where a value itself is not finite."""
+    n = 20000
+    x, w = np.zeros((2, n), np.float32), np.full(n, 3.4e38, np.float32)
+    x[:, 40] = 1.0                                        # z = 3.4e38 * sqrt(20000) = 4.8e40, z / 127 = 3.8e38
+    x[1, 41] = 1.0                                        # z = 3.4e40, z / 127 = 2.7e38: still in range
+    q, d, xd, wd = Out(2, n, dtype=torch.int8), Out(2, n // 32), dev(x), dev(w)
+    sublayer.rms_norm_device(xd.data_ptr(), n, n, 2, weight_ptr=wd.data_ptr(), eps=0.0, q8=sublayer.Q8View(q.ptr, q.ld, d.ptr, d.ld))
+    q, d = q.get(), d.get()
+    assert np.isinf(d[0, 1]) and not q[0].any() and not d[0, 2:].any()
+    assert np.isfinite(d[1]).all() and q[1, 40] == q[1, 41] == 127 and np.count_nonzero(q[1]) == 2
+
+
 @pytest.mark.parametrize("n", [2016, 20000])
 def test_quantize_exact_ties_whatever_the_step(hip, n):
     """A block of maximum 127 k has the step k exactly, and (j + 1/2) k lies exactly between two steps, however 127 / (127 k) rounds:
