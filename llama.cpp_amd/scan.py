@@ -30,7 +30,7 @@ from typing import Callable, Dict, Iterable, List, Optional, Sequence, Tuple
 import numpy as np
 
 from . import seeddelta as sd
-from .dense import dense_dims, dense_type
+from .dense import Q8_BYTES, dense_dims, dense_type
 
 KINDS = ("ffn_gate", "ffn_up", "ffn_down")
 KIND_ID = {k: i for i, k in enumerate(KINDS)}
@@ -46,6 +46,8 @@ class DenseWeight:
     def __init__(self, W: np.ndarray):
         lib = sd.load_library()
         W = np.ascontiguousarray(W)
+        if W.ndim != 2 or (W.dtype == np.uint8 and W.shape[1] % Q8_BYTES):
+            raise sd.SeedDeltaError(f"DenseWeight: {W.dtype} of shape {W.shape}: two dimensions, rows of whole blocks of {Q8_BYTES} bytes for Q8_0")
         self.n_in, self.n_out = dense_dims(W)
         t = sd.SdhTensor()
         t.data, t.type, t.n_dims = W.ctypes.data, dense_type(W), 2

@@ -6,8 +6,8 @@ import numpy as np
 import pytest
 import torch
 
+from llama_cpp_amd import scan, sublayer
 from llama_cpp_amd import seeddelta as sd
-from llama_cpp_amd import sublayer
 
 BAD, NO_DEVICE = r"\(-1\)", r"\(-2\)"
 P = 4096                                     # a pointer that is never read: 16-byte aligned
@@ -96,3 +96,17 @@ def test_lora_entry_points_without_a_set():
 
 def test_struct_layouts_match_the_header():
     assert C.sizeof(sd.SdhQ8) == 32 and C.sizeof(sd.SdhLoraDesc) == 2 * C.sizeof(sd.SdhTensor) + 8
+
+
+@pytest.mark.parametrize("W", [np.zeros((3, 100), np.uint8), np.zeros((3, 33), np.uint8), np.zeros(68, np.uint8), np.zeros((2, 3, 34), np.uint8), np.zeros(64, np.float32)])
+def test_dense_weights_of_ragged_rows_are_refused(W, monkeypatch):
+    monkeypatch.setattr(sd, "_inited_device", 0)
+    with pytest.raises(sd.SeedDeltaError, match="DenseWeight"):
+        scan.DenseWeight(W)
+    with pytest.raises(sd.SeedDeltaError, match="DenseWeight|raw Q8_0 rows"):
+        sd.SeedDeltaContext().add_dense("up", W)
+
+
+def test_dense_weights_of_whole_blocks_end_at_the_device():
+    with pytest.raises(sd.SeedDeltaError, match=NO_DEVICE):
+        scan.DenseWeight(np.zeros((3, 68), np.uint8))
