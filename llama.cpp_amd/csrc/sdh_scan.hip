@@ -1474,6 +1474,7 @@ static int sdh_dense_create_impl(const sdh_tensor * W, sdh_dense ** out) {
     d->v.type = W->type; d->v.n_in = n_in; d->v.n_out = n_out;
     const uint8_t * src = (const uint8_t *) W->data;
     auto fail = [&](int rc) { (void) hipFree(d->alloc0); (void) hipFree(d->alloc1); delete d; return rc; };
+    auto sent = [](hipError_t e) { if (e != hipSuccess) set_error("upload of a dense weight failed: %s", hipGetErrorString(e)); return e == hipSuccess; };
     if (W->type == SDH_TYPE_Q8_0) {
         if (n_in % 32) { set_error("Q8_0 needs n_in %% 32 == 0"); return fail(SDH_ERR_INVALID); }
         const int64_t nblk = n_in / 32;
@@ -1493,8 +1494,8 @@ static int sdh_dense_create_impl(const sdh_tensor * W, sdh_dense ** out) {
                     std::memcpy(&q[(size_t) (r * n_in + b * 32)], row + b * 34 + 2, 32);
                 }
             }
-            (void) hipMemcpy((int8_t *) d->alloc0 + r0 * n_in, q.data(), (size_t) (rows * n_in), hipMemcpyHostToDevice);
-            (void) hipMemcpy((uint16_t *) d->alloc1 + r0 * nblk, sc.data(), (size_t) (rows * nblk) * 2, hipMemcpyHostToDevice);
+            if (!sent(hipMemcpy((int8_t *) d->alloc0 + r0 * n_in, q.data(), (size_t) (rows * n_in), hipMemcpyHostToDevice)) ||
+                !sent(hipMemcpy((uint16_t *) d->alloc1 + r0 * nblk, sc.data(), (size_t) (rows * nblk) * 2, hipMemcpyHostToDevice))) return fail(SDH_ERR_HIP);
         }
         d->v.q = (const int8_t *) d->alloc0; d->v.d = (const __half *) d->alloc1;
         d->stored_bytes = n_out * nblk * 34;
@@ -1504,14 +1505,13 @@ static int sdh_dense_create_impl(const sdh_tensor * W, sdh_dense ** out) {
         if (hipMalloc(&d->alloc0, (size_t) (n_out * n_in) * es) != hipSuccess) {
             set_error("hipMalloc failed for a dense weight"); return fail(SDH_ERR_HIP);
         }
-        (void) hipMemcpy2D(d->alloc0, (size_t) n_in * es, src, (size_t) W->nb[1], (size_t) n_in * es, (size_t) n_out, hipMemcpyHostToDevice);
+        if (!sent(hipMemcpy2D(d->alloc0, (size_t) n_in * es, src, (size_t) W->nb[1], (size_t) n_in * es, (size_t) n_out, hipMemcpyHostToDevice))) return fail(SDH_ERR_HIP);
         d->v.data = d->alloc0;
         d->stored_bytes = n_out * n_in * (int64_t) es;
     } else {
         set_error("dense weight type %d not supported (F32, F16, Q8_0)", W->type);
         return fail(SDH_ERR_UNSUPPORTED);
     }
-    if (hipGetLastError() != hipSuccess) { set_error("upload of a dense weight failed"); return fail(SDH_ERR_HIP); }
     *out = (sdh_dense *) d;
     return SDH_OK;
 }

@@ -1,0 +1,64 @@
+"""What the library does when the HIP runtime says no, on the CPU: hip_stub.c takes the runtime's place in a process of its own (kernels do
+not run; a test says which call fails, which device is current, whether a capture is under way)."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+START = """
+import ctypes as C, sys
+import numpy as np
+stub = C.CDLL({stub!r}, C.RTLD_GLOBAL)
+sys.path.insert(0, {root!r})
+import llama_cpp_amd
+from llama_cpp_amd import scan, sublayer, seeddelta as sd
+from llama_cpp_amd.dense import make_dense
+from llama_cpp_amd.payload import make_payload
+def refused(fn, code):
+    try:
+        fn()
+    except sd.SeedDeltaError as e:
+        assert f"({{code}})" in str(e), e
+        return str(e)
+    raise AssertionError("not refused")
+"""
+
+
+@pytest.fixture(scope="module")
+def stub(tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("stub") / "hip_stub.so")
+    subprocess.check_call(["gcc", "-std=c11", "-shared", "-fPIC", "-O1", "-I/opt/rocm/include", "-o", out, os.path.join(HERE, "hip_stub.c")])
+
+    def run(code):
+        p = subprocess.run([sys.executable, "-c", START.format(stub=out, root=os.path.dirname(HERE)) + code + "\nprint('done')"],
+                           capture_output=True, text=True, timeout=240)
+        assert p.returncode == 0 and p.stdout.endswith("done\n"), p.stdout + p.stderr
+    return run
+
+
+def test_dense_upload_that_fails_is_an_error_and_leaves_nothing(stub):
+    """Whichever copy fails, and whether or not the runtime keeps the error of a call that others follow."""
+    stub("""
+sd.init(0)
+before = stub.stub_live()
+for W, copies in ((make_dense(1024, 3000), 6), (make_dense(96, 50), 2), (make_dense(64, 33, "f16"), 1), (make_dense(64, 33, "f32"), 1)):
+    for keep in (0, 1):
+        for n in range(copies):
+            stub.stub_fail_copy(n, keep)
+            assert "failed" in refused(lambda: scan.DenseWeight(W), -3)
+            assert stub.stub_live() == before, (n, keep)
+    stub.stub_fail_copy(-1, 1)
+    w = scan.DenseWeight(W)
+    w.close()
+    assert stub.stub_live() == before
+""")
+
+
+def test_dense_upload_is_not_blamed_for_an_earlier_error(stub):
+    stub("""
+sd.init(0)
+stub.stub_stale_error()
+scan.DenseWeight(make_dense(96, 50)).close()
+""")
