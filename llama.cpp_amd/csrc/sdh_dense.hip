@@ -527,6 +527,7 @@ static int sdh_dense_forward_q8_impl(const sdh_dense * W, const sdh_q8 * x, int6
     if (!aligned(x->q, 16) || x->ldq % 16 || !aligned(x->d, 4) || !aligned(y, 4)) { set_error("%s: x->q needs 16-byte aligned rows, x->d and y 4-byte ones", who); return SDH_ERR_INVALID; }
     const int rc = ready_on_device(who);
     if (rc != SDH_OK) return rc;
+    if (w.device != lib().device) { set_error("%s: the weight was made on device %d, the library is bound to %d", who, w.device, lib().device); return SDH_ERR_INVALID; }
     const DenseArgs a{w.q, (const __half *) w.d, x->q, x->ldq, x->d, x->ldd, (int) w.n_out, (int) (w.n_in / 32), T, y, ldy};
     return launch_dense(a, (hipStream_t) stream);
 }

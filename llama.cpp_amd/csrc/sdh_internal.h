@@ -227,7 +227,7 @@ int64_t stack_bytes(const FfnStack * st);
 // What every one of their entry points checks first: sdh_init() was called and its device is the current one (a launch goes to
 // the current device, whatever device the pointers are on).
 int ready_on_device(const char * who);
-struct DenseQ8 { const int8_t * q; const uint16_t * d; int64_t n_in, n_out; int type; };   // [n_out][n_in], f16 [n_out][n_in/32]
+struct DenseQ8 { const int8_t * q; const uint16_t * d; int64_t n_in, n_out; int type, device; };   // [n_out][n_in], f16 [n_out][n_in/32]
 DenseQ8 dense_q8(const sdh_dense * W);     // sdh_scan.hip (the handle's layout)
 std::vector<float> tensor_f32(const sdh_tensor & t);     // F16 / F32, any strides -> contiguous F32 [ne1][ne0], exact (sdh_api.hip)
 inline bool aligned(const void * p, size_t a) { return ((uintptr_t) p & (a - 1)) == 0; }

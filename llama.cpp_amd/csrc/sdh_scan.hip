@@ -57,6 +57,7 @@ struct DeviceDense {
     DenseView v{};
     void * alloc0 = nullptr, * alloc1 = nullptr;
     int64_t stored_bytes = 0;
+    int device = -1;                    // the one that was current at creation
     uint64_t serial = next_serial();    // identity for caches (an address can be reused by a later tensor)
     static uint64_t next_serial() { static std::atomic<uint64_t> n{0}; return ++n; }
 };
@@ -1440,8 +1441,8 @@ static std::shared_ptr<const FitPlan> plan_fit(std::mt19937 & rng, int64_t n_in,
 }
 
 DenseQ8 dense_q8(const sdh_dense * W) {
-    const DenseView & v = ((const DeviceDense *) W)->v;
-    return DenseQ8{v.q, (const uint16_t *) v.d, v.n_in, v.n_out, v.type};
+    const DeviceDense & d = *(const DeviceDense *) W;
+    return DenseQ8{d.v.q, (const uint16_t *) d.v.d, d.v.n_in, d.v.n_out, d.v.type, d.device};
 }
 
 static DenseView view_or_null(const sdh_dense * d) {
@@ -1474,6 +1475,7 @@ static int sdh_dense_create_impl(const sdh_tensor * W, sdh_dense ** out) {
     d->v.type = W->type; d->v.n_in = n_in; d->v.n_out = n_out;
     const uint8_t * src = (const uint8_t *) W->data;
     auto fail = [&](int rc) { (void) hipFree(d->alloc0); (void) hipFree(d->alloc1); delete d; return rc; };
+    if (hipGetDevice(&d->device) != hipSuccess) { set_error("sdh_dense_create: no current device"); return fail(SDH_ERR_HIP); }
     auto sent = [](hipError_t e) { if (e != hipSuccess) set_error("upload of a dense weight failed: %s", hipGetErrorString(e)); return e == hipSuccess; };
     if (W->type == SDH_TYPE_Q8_0) {
         if (n_in % 32) { set_error("Q8_0 needs n_in %% 32 == 0"); return fail(SDH_ERR_INVALID); }

@@ -78,3 +78,5 @@ hipError_t hipMemcpy2D(void * to, size_t tp, const void * from, size_t fp, size_
 hipError_t hipMemset(void * p, int v, size_t n) { memset(p, v, n); return done(hipSuccess); }
 hipError_t hipMemsetAsync(void * p, int v, size_t n, hipStream_t s) { (void) s; memset(p, v, n); return done(hipSuccess); }
 hipError_t hipLaunchKernel(const void * f, dim3 g, dim3 b, void ** a, size_t l, hipStream_t s) { (void) f; (void) g; (void) b; (void) a; (void) l; (void) s; ++launches; return done(hipSuccess); }
+hipError_t __hipPushCallConfiguration(dim3 g, dim3 b, size_t l, hipStream_t s) { (void) g; (void) b; (void) l; (void) s; return hipSuccess; }
+hipError_t __hipPopCallConfiguration(dim3 * g, dim3 * b, size_t * l, hipStream_t * s) { memset(g, 0, sizeof *g); memset(b, 0, sizeof *b); *l = 0; *s = 0; return hipSuccess; }

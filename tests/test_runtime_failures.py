@@ -62,3 +62,21 @@ sd.init(0)
 stub.stub_stale_error()
 scan.DenseWeight(make_dense(96, 50)).close()
 """)
+
+
+def test_dense_weight_of_another_device_is_refused(stub):
+    """The kernels run on the device that the library is bound to; a handle that was made while another one was current is not theirs to read."""
+    stub("""
+sd.init(0)
+x8 = sublayer.Q8View(4096, 96, 8192, 3)
+here = scan.DenseWeight(make_dense(96, 50))
+stub.stub_set_device(1)
+there = scan.DenseWeight(make_dense(96, 50))
+assert "current device" in refused(lambda: sublayer.dense_forward_q8_device(here, x8, 4, 16384, 50), -1)
+stub.stub_set_device(0)
+n = stub.stub_launches()
+assert "made on device 1" in refused(lambda: sublayer.dense_forward_q8_device(there, x8, 4, 16384, 50), -1)
+assert stub.stub_launches() == n
+sublayer.dense_forward_q8_device(here, x8, 4, 16384, 50)
+assert stub.stub_launches() == n + 1
+""")
