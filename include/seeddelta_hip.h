@@ -137,7 +137,9 @@ typedef enum sdh_op_kind {
 
 /* ---- library / device ----------------------------------------------------------------
  * sdh_init: bind the calling process to HIP device `device` and create the library's
- * stream and scratch. Idempotent per device. Replaces nothing in the reference (its op is
+ * stream and scratch. Idempotent per device. The device becomes the calling thread's current one (HIP keeps one per
+ * thread, device 0 at first): a thread that creates handles or issues calls makes this call too, unless the library
+ * is bound to device 0. Replaces nothing in the reference (its op is
  * CPU-only); a shim calls it lazily from the first custom-op callback. */
 int          sdh_init(int device);
 int          sdh_abi_version(void);

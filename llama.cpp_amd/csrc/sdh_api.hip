@@ -206,7 +206,7 @@ const char * sdh_last_error(void) { return g_last_error.c_str(); }
 int sdh_init(int device) {
     std::lock_guard<std::mutex> lk(g_mu);
     LibState & s = lib();
-    if (s.inited && s.device == device) return SDH_OK;
+    if (s.inited && s.device == device) { SDH_HIP_CHECK(hipSetDevice(device)); return SDH_OK; }      // another thread's first call, perhaps
     int n = 0;
     if (hipGetDeviceCount(&n) != hipSuccess || n <= 0) {
         set_error("no HIP device visible");

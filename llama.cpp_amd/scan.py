@@ -552,7 +552,8 @@ class Evaluator:
         if self._pool is None or self._pool_threads != threads:
             if self._pool is not None:
                 self._pool.shutdown(wait=True)
-            self._pool = ThreadPoolExecutor(max_workers=threads)
+            bound = sd._inited_device               # a new thread's current device is 0
+            self._pool = ThreadPoolExecutor(max_workers=threads, initializer=None if bound is None else lambda: sd.init(bound))
             self._pool_threads = threads
         return self._pool
 

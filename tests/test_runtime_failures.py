@@ -80,3 +80,17 @@ assert stub.stub_launches() == n
 sublayer.dense_forward_q8_device(here, x8, 4, 16384, 50)
 assert stub.stub_launches() == n + 1
 """)
+
+
+def test_worker_threads_of_a_scan_run_on_the_bound_device(stub):
+    """The current device is a thread's own and 0 in a new one: a rank bound to device 1 uploads and evaluates there from its pool too."""
+    stub("""
+sd.init(1)
+ev = scan.Evaluator(lambda layer, kind: make_dense(96, 50), scan.ScanParams())
+assert set(ev._workers(4).map(lambda _: stub.stub_device(), range(32))) == {1}
+W = ev._workers(4).submit(lambda: scan.DenseWeight(make_dense(96, 50))).result()
+sublayer.dense_forward_q8_device(W, sublayer.Q8View(4096, 96, 8192, 3), 4, 16384, 50)
+stub.stub_set_device(0)
+sd.init(1)                                    # once more in a thread: binds the thread
+assert stub.stub_device() == 1
+""")
