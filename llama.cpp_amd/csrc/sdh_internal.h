@@ -31,6 +31,7 @@ void set_error(const char * fmt, ...);
     do {                                                                                     \
         hipError_t e_ = (expr);                                                              \
         if (e_ != hipSuccess) {                                                              \
+            (void) hipGetLastError();       /* reported here: not the next call's error */   \
             sdh::set_error("%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__, __LINE__); \
             return SDH_ERR_HIP;                                                              \
         }                                                                                    \

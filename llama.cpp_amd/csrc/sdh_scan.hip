@@ -1474,7 +1474,7 @@ static int sdh_dense_create_impl(const sdh_tensor * W, sdh_dense ** out) {
     DeviceDense * d = new DeviceDense();
     d->v.type = W->type; d->v.n_in = n_in; d->v.n_out = n_out;
     const uint8_t * src = (const uint8_t *) W->data;
-    auto fail = [&](int rc) { (void) hipFree(d->alloc0); (void) hipFree(d->alloc1); delete d; return rc; };
+    auto fail = [&](int rc) { (void) hipFree(d->alloc0); (void) hipFree(d->alloc1); (void) hipGetLastError(); delete d; return rc; };
     if (hipGetDevice(&d->device) != hipSuccess) { set_error("sdh_dense_create: no current device"); return fail(SDH_ERR_HIP); }
     auto sent = [](hipError_t e) { if (e != hipSuccess) set_error("upload of a dense weight failed: %s", hipGetErrorString(e)); return e == hipSuccess; };
     if (W->type == SDH_TYPE_Q8_0) {

@@ -94,3 +94,21 @@ stub.stub_set_device(0)
 sd.init(1)                                    # once more in a thread: binds the thread
 assert stub.stub_device() == 1
 """)
+
+
+def test_an_error_is_reported_once(stub):
+    """The call that meets an error of the runtime returns it; the next one, which looks at its launch, does not find it again."""
+    stub("""
+sd.init(0)
+norm = lambda: sublayer.rms_norm_device(4096, 64, 64, 2, y_ptr=8192, ldy=64)
+for make in (lambda: scan.DenseWeight(make_dense(96, 50)), lambda: scan.DenseWeight(make_dense(64, 33, "f16")),
+             lambda: sublayer.LoraSet([(np.zeros((4, 32), np.float16), np.zeros((48, 4), np.float16), 1.0)])):
+    stub.stub_fail_copy(0, 1)
+    refused(make, -3)
+    norm()
+    stub.stub_fail_copy(-1, 1)
+    stub.stub_capture(1)                                # an allocation is refused
+    refused(make, -3)
+    stub.stub_capture(0)
+    norm()
+""")
