@@ -176,8 +176,9 @@ int64_t sdh_weight_payload_bytes(const sdh_weight * w);
  * out-of-range perm entries read element 0 (:524-527), scale applied only if != 1 (:645),
  * tall/wide base split on n_out >= n_in (:1073).
  * HIP graphs: with device pointers the call may be made on a capturing stream. Call it once
- * eagerly first (workspaces and the fused decode launch's one-time residency check need the
- * host); a decode launch captured before that records the two-kernel path instead. Captured
+ * eagerly first with as many tokens (workspaces and the fused decode launch's one-time residency check need the
+ * host); a decode launch captured before that records the two-kernel path instead. A later call with more tokens takes a
+ * larger workspace; the one that a graph was recorded with stays valid as long as the handle. Captured
  * and eager calls on one handle may be mixed freely on one stream; calls on one handle from
  * different streams or graph branches must be ordered by the caller (they share the handle's
  * hand-off buffer). The same holds for sdh_ffn_forward / sdh_ffn_gate_up. */

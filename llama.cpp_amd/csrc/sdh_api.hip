@@ -165,18 +165,38 @@ static void free_weight(DeviceWeight * w) {
     (void) hipFree(w->idx); (void) hipFree(w->val); (void) hipFree(w->rs);
     (void) hipFree(w->d1); (void) hipFree(w->d2); (void) hipFree(w->d3); (void) hipFree(w->p1); (void) hipFree(w->p2);
     (void) hipFree(w->pack_dev); (void) hipFree(w->handoff);
-    (void) hipFree(w->G); (void) hipFree(w->inv); (void) hipFree(w->nf_ring); (void) hipFree(w->ws);
+    (void) hipFree(w->G); (void) hipFree(w->inv); (void) hipFree(w->nf_ring); (void) hipFree(w->ws_mem.p);
+    for (float * p : w->ws_mem.aside) (void) hipFree(p);
     fold_free(*w);
     direct_free(*w);
     delete w;
 }
 
-static int ensure_ws(DeviceWeight * w, size_t bytes) {
-    if (w->ws_bytes >= bytes) return SDH_OK;
-    if (w->ws) { SDH_HIP_CHECK(hipFree(w->ws)); w->ws = nullptr; w->ws_bytes = 0; }
-    SDH_HIP_CHECK(hipMalloc((void **) &w->ws, bytes));
-    w->ws_bytes = bytes;
+bool stream_capturing(hipStream_t s) {
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &cs) == hipSuccess) return cs != hipStreamCaptureStatusNone;
+    (void) hipGetLastError();                               // the legacy stream while another one captures
+    return true;
+}
+
+// A workspace of `bytes` for a call on stream s. A graph that calls were recorded into keeps the address that they were given: a workspace
+// of such a call is set aside when a larger one takes its place (and stays as long as its owner), others are freed.
+static int grow_ws(GrowingWs & ws, size_t bytes, hipStream_t s) {
+    const bool capturing = stream_capturing(s);
+    if (ws.bytes < bytes) {
+        if (ws.p && (ws.recorded || capturing)) ws.aside.push_back(ws.p);
+        else if (ws.p) SDH_HIP_CHECK(hipFree(ws.p));
+        ws.p = nullptr; ws.bytes = 0; ws.recorded = false;
+        SDH_HIP_CHECK(hipMalloc((void **) &ws.p, bytes));
+        ws.bytes = bytes;
+    }
+    ws.recorded = ws.recorded || capturing;
     return SDH_OK;
+}
+static int ensure_ws(DeviceWeight * w, size_t bytes, hipStream_t s) {
+    const int rc = grow_ws(w->ws_mem, bytes, s);
+    w->ws = w->ws_mem.p;
+    return rc;
 }
 
 // drain recorded event pairs into the running totals (waits for the last one)
@@ -625,7 +645,7 @@ static int sdh_forward_impl(sdh_weight * h, const float * x, int64_t ldx, int64_
     if (((flags & SDH_FWD_MFMA_FOLD) || fold_default) && has_base && !(flags & SDH_FWD_EXACT_ORDER) && !noalloc &&
         w->w0_closed_form && w->L >= 128 && n_tokens > MAX_FUSED_TOKENS) {
         const int64_t fchunk = std::min<int64_t>(n_tokens, 2048);
-        int rc = ensure_ws(w, w0_fold_ws_bytes(*w, fchunk));
+        int rc = ensure_ws(w, w0_fold_ws_bytes(*w, fchunk), s);
         if (rc != SDH_OK) return rc;
         int pair = -1;
         if (ls.prof_on) {
@@ -698,14 +718,14 @@ static int sdh_forward_impl(sdh_weight * h, const float * x, int64_t ldx, int64_
         }
         if (mfma_tiled) {
             const size_t part_bytes = per_tok * (size_t) chunk;                 // wide: [chunk][B][L] partial products
-            int rc = ensure_ws(w, part_bytes + w0_mfma_x16_bytes(*w, chunk));
+            int rc = ensure_ws(w, part_bytes + w0_mfma_x16_bytes(*w, chunk), s);
             if (rc != SDH_OK) return rc;
             _Float16 * x16 = (_Float16 *) ((unsigned char *) w->ws + part_bytes);
             if (w->tall) { rc = launch_w0_mfma_tiled(*w, xc, dldx, tc, x16, a.y, a.ldy, s); a.v = a.y; a.v_ld = a.ldy; }
             else         { rc = launch_w0_mfma_tiled(*w, xc, dldx, tc, x16, w->ws, (int64_t) w->B * w->L, s); a.v = w->ws; }
             if (rc != SDH_OK) { if (rc == 1) set_error("w0 mfma: payload does not fit the tile scheme"); return rc == 1 ? SDH_ERR_UNSUPPORTED : rc; }
         } else if (has_base) {
-            int rc = noalloc ? SDH_OK : ensure_ws(w, per_tok * (size_t) chunk);
+            int rc = noalloc ? SDH_OK : ensure_ws(w, per_tok * (size_t) chunk, s);
             if (rc != SDH_OK) return rc;
             float * const ws = noalloc ? ext_ws : w->ws;
             rc = 1;
@@ -780,13 +800,9 @@ int sdh_glu(int act, const float * g, const float * u, float * y, int64_t n, voi
 static int ffn_workspace(LibState & ls, hipStream_t s, const size_t * floats, int n, float ** out) {
     size_t total = 0;
     for (int i = 0; i < n; ++i) total += (floats[i] + 3) & ~(size_t) 3;
-    const size_t need = total * sizeof(float) + 64;
-    if (ls.ffn_ws_bytes < need) {
-        if (ls.ffn_ws) { SDH_HIP_CHECK(hipStreamSynchronize(s)); SDH_HIP_CHECK(hipFree(ls.ffn_ws)); }
-        ls.ffn_ws = nullptr; ls.ffn_ws_bytes = 0;
-        SDH_HIP_CHECK(hipMalloc((void **) &ls.ffn_ws, need)); ls.ffn_ws_bytes = need;
-    }
-    float * p = ls.ffn_ws;
+    const int rc = grow_ws(ls.ffn_ws, total * sizeof(float) + 64, s);
+    if (rc != SDH_OK) return rc;
+    float * p = ls.ffn_ws.p;
     for (int i = 0; i < n; ++i) { out[i] = p; p += (floats[i] + 3) & ~(size_t) 3; }
     return SDH_OK;
 }
@@ -851,8 +867,8 @@ static int ffn_gate_up(sdh_weight * hg, sdh_weight * hu, int act, const float * 
     // (SDH_FWD_MFMA_FOLD: both nodes as folded contractions instead, the activation in the up node's epilogue)
     if (T > MAX_FUSED_TOKENS && T <= 1024 && g != u && with_base(g) && with_base(u) && g->tall && u->tall &&
         !(flags & (SDH_FWD_EXACT_ORDER | SDH_FWD_W0_MFMA | SDH_FWD_MFMA_FOLD)) && per_tok * (size_t) T <= ((size_t) 64 << 20)) {
-        if ((rc = ensure_ws(g, per_tok * (size_t) T)) != SDH_OK) return rc;
-        if ((rc = ensure_ws(u, per_tok * (size_t) T)) != SDH_OK) return rc;
+        if ((rc = ensure_ws(g, per_tok * (size_t) T, s)) != SDH_OK) return rc;
+        if ((rc = ensure_ws(u, per_tok * (size_t) T, s)) != SDH_OK) return rc;
         rc = launch_base_apply_pair(*g, *u, dx, dldx, T, g->ws, u->ws, s);
         if (rc < 0) return rc;
         if (rc == SDH_OK) g->base_ready = u->base_ready = true;
@@ -882,8 +898,8 @@ static int ffn_gate_up(sdh_weight * hg, sdh_weight * hu, int act, const float * 
     static const bool no_pair = getenv("SDH_FOLD_NO_PAIR") != nullptr;            // A/B switch
     if ((flags & SDH_FWD_MFMA_FOLD) && T > 256 && g != u && !(flags & SDH_FWD_EXACT_ORDER) && !no_pair) {
         const int64_t fchunk = std::min<int64_t>(T, 2048);
-        if ((rc = ensure_ws(g, w0_fold_ws_bytes(*g, fchunk))) != SDH_OK) return rc;
-        if ((rc = ensure_ws(u, w0_fold_ws_bytes(*u, fchunk))) != SDH_OK) return rc;
+        if ((rc = ensure_ws(g, w0_fold_ws_bytes(*g, fchunk), s)) != SDH_OK) return rc;
+        if ((rc = ensure_ws(u, w0_fold_ws_bytes(*u, fchunk), s)) != SDH_OK) return rc;
         int sg = 0, su = 0;
         if ((rc = nf_slot(g, s, &sg)) != SDH_OK) return rc;
         if ((rc = nf_slot(u, s, &su)) != SDH_OK) return rc;

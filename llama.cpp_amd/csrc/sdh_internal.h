@@ -48,6 +48,16 @@ struct BasePackDesc {
     int wide32 = 0;                   // 1: f32 / i32 parameters, 0: f16 / i16 (as the builder writes them)
 };
 
+// Device memory that grows with the calls that use it (grow_ws in sdh_api.hip)
+struct GrowingWs {
+    float * p = nullptr;
+    size_t  bytes = 0;
+    bool    recorded = false;            // a call that has p was recorded into a graph
+    std::vector<float *> aside;          // smaller ones before it that graphs may still use
+};
+
+bool stream_capturing(hipStream_t s);
+
 // ---- device-resident payload ---------------------------------------------------------------
 // All tensors are repacked contiguous at upload; element types of idx/val are kept as stored
 // in the GGUF (they are the HBM stream), small per-row / per-base-block vectors are widened
@@ -91,10 +101,10 @@ struct DeviceWeight {
     uint64_t seq = 0;            // forwards issued
     hipStream_t last_stream = nullptr;
     // workspace for the base term v[T_chunk][B][L]
-    float * ws = nullptr;
+    float * ws = nullptr;        // == ws_mem.p
+    GrowingWs ws_mem;
     const float * x4_hint = nullptr;  // token-interleaved copy of the next call's x (see DeltaLaunch::x4); set and cleared by the FFN path
     bool    base_ready = false;  // ws already holds the base terms of the next call's tokens (gate|up base launch of the FFN path)
-    size_t  ws_bytes = 0;
     // the residual re-laid out for the folded MFMA contraction (sdh_w0fold.hip), built on first use: entries bucketed by
     // (128-row tile, 64-wide k-slab), fold_off [tiles][fold_ng] = {begin, end} of a bucket in fold_ent
     unsigned * fold_ent = nullptr; int2 * fold_off = nullptr; int fold_ng = 0, fold_spb = 0;
@@ -124,7 +134,7 @@ struct LibState {
     unsigned * census_ctr = nullptr;    // residency census of the fused decode kernel (sdh_decode.hip)
     // gated FFN block (sdh_ffn.hip): f16 GELU table as ggml builds it, intermediate activations
     uint16_t * gelu_tab = nullptr;      // [65536] device
-    float * ffn_ws = nullptr; size_t ffn_ws_bytes = 0;
+    GrowingWs ffn_ws;
     int ffn_last_fused = 0;             // the last gate/up evaluation ran as the single gate|up launch
     int last_decode_kind = 0;           // sdh_debug_last_decode_kind: 1 direct, 2 fused, 3 two kernels
     // measurement hooks (sdh_profile_*): event pairs around the dominant kernel

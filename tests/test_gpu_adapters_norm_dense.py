@@ -671,6 +671,51 @@ def test_context_refuses_adapters_of_another_projection(hip, dims):
     assert torch.all(y == 7.0)
 
 
+@pytest.mark.parametrize("T", [1, 6, 100])
+def test_context_captured_and_replayed(hip, T):
+    """mul_mat_device of a payload and of a dense key, with adapters, recorded after one eager call of as many tokens. Eager calls of more
+    tokens between the replays take larger workspaces of the payload's handle: the graph keeps its own."""
+    n, n_out, most = 1024, 2048, 5 * T + 3
+    ctx, rng = hip.SeedDeltaContext(), np.random.default_rng(T)
+    assert ctx.try_add("up", make_payload(n, n_out, scheme="coo", K=16, base=True, seed=1))
+    ctx.add_dense("gate", make_dense(n, n_out, "q8_0", 2))
+    ads = make_adapters(n, n_out, [8, 20], ["h", "f"])
+    for k in ("up", "gate"):
+        ctx.add_adapters(k, ads)
+
+    def buffers(T):
+        return dict(T=T, x=torch.zeros(T, n, device="cuda"), q=torch.empty(T, n, dtype=torch.int8, device="cuda"), d=torch.empty(T, n // 32, device="cuda"),
+                    ids=torch.zeros(T, dtype=torch.int32, device="cuda"), up=torch.empty(T, n_out, device="cuda"), gate=torch.empty(T, n_out, device="cuda"),
+                    ws=torch.empty(ctx.workspace_bytes("up", T), dtype=torch.uint8, device="cuda"))
+
+    def call(b, st):
+        x8 = sublayer.Q8View(b["q"].data_ptr(), n, b["d"].data_ptr(), n // 32)
+        sublayer.q8_quantize_device(b["x"].data_ptr(), n, n, b["T"], x8, stream=st)
+        for k in ("up", "gate"):
+            assert ctx.mul_mat_device(k, b["x"].data_ptr(), n, b["T"], b[k].data_ptr(), n_out, x8=x8, ids_ptr=b["ids"].data_ptr(), ws_ptr=b["ws"].data_ptr(), ws_bytes=b["ws"].numel(), stream=st)
+
+    cap, eager, more = buffers(T), buffers(T), [buffers(m) for m in (T + 1, 2 * T, most)]
+    call(eager, 0)
+    torch.cuda.synchronize()
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=side):
+        call(cap, torch.cuda.current_stream().cuda_stream)
+    for rep in range(4):
+        x, ids = dev(rng.standard_normal((T, n)).astype(np.float32)), dev(rng.integers(-1, 3, T).astype(np.int32))
+        for b in (cap, eager):
+            b["x"].copy_(x); b["ids"].copy_(ids)
+        for k in ("up", "gate"):
+            cap[k].fill_(-7.0)
+        g.replay()
+        call(eager, 0)
+        torch.cuda.synchronize()
+        for k in ("up", "gate"):
+            assert torch.equal(cap[k], eager[k]), (rep, k)
+        if rep < len(more):
+            call(more[rep], 0)
+            torch.cuda.synchronize()
+
+
 def test_norm_more_rows_than_one_launch(hip):
     """Over 2^21 rows: the launch is cut."""
     T, n = (1 << 21) + 5, 4

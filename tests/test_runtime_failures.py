@@ -112,3 +112,45 @@ for make in (lambda: scan.DenseWeight(make_dense(96, 50)), lambda: scan.DenseWei
     stub.stub_capture(0)
     norm()
 """)
+
+
+def test_workspace_that_a_graph_holds_outlives_a_larger_one(stub):
+    """A call with more tokens than before takes a larger workspace. One whose address a graph has recorded stays until the handle goes."""
+    stub("""
+sd.init(0)
+def grown(recorded):
+    before = stub.stub_live()
+    w = sd.SeedDeltaWeight(make_payload(1024, 2048, scheme="coo", K=16, base=True, seed=1))
+    call = lambda T: w.forward_device(4096, 1024, T, 8192, 2048, sd.FWD_NO_MFMA)
+    call(16)
+    if recorded:
+        stub.stub_capture(1); call(16); stub.stub_capture(0)
+    a = stub.stub_live()
+    call(64)
+    b = stub.stub_live()
+    stub.stub_capture(1)                            # within the new size: nothing is allocated or freed
+    call(64)
+    refused(lambda: call(200), -3)                  # a larger one is (this mode of capture does not allow it)
+    stub.stub_capture(0)
+    call(200)
+    w.close()
+    assert stub.stub_live() == before
+    return b - a
+assert grown(False) == 0 and grown(True) == 1
+""")
+
+
+def test_ffn_workspace_that_a_graph_holds_outlives_a_larger_one(stub):
+    stub("""
+sd.init(0)
+mk = lambda i, o, s: sd.SeedDeltaWeight(make_payload(i, o, scheme="coo", K=16, base=True, seed=s))
+g, u, d = mk(1024, 2048, 1), mk(1024, 2048, 2), mk(2048, 1024, 3)
+call = lambda T: sd.ffn_forward_device(g, u, d, sd.ACT_SILU, 4096, 1024, T, 8192, 1024, sd.FWD_NO_MFMA)
+call(16)
+a = stub.stub_live()
+call(24)
+assert stub.stub_live() == a
+stub.stub_capture(1); call(24); stub.stub_capture(0)
+call(64)
+assert stub.stub_live() == a + 4                   # the three handles' and the block's own
+""")
