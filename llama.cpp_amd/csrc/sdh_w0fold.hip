@@ -284,6 +284,7 @@ int fold_ensure(DeviceWeight & w, hipStream_t s) {
     const int64_t per_row = is_block ? w.nb : w.K;
     const int64_t cap = (int64_t) w.n_out * (is_block ? w.nb * w.block : w.K);
     if (cap <= 0 || cap > 0x7fffffff) return 1;
+    if (stream_capturing(s)) { set_error("the first folded call of a payload builds its layout, which a graph cannot record: call it once eagerly first"); return SDH_ERR_UNSUPPORTED; }
     const size_t off_bytes = (size_t) tiles * (a.n_g + 1) * sizeof(int);
     const size_t ent_words = (size_t) cap + (size_t) 4 * tiles * a.n_g + 4;       // every bucket padded to a multiple of 4
     int * counts = nullptr, * cursor = nullptr; unsigned * ent = nullptr; int2 * bounds = nullptr; _Float16 * gp = nullptr; short * p16 = nullptr;

@@ -154,3 +154,17 @@ stub.stub_capture(1); call(24); stub.stub_capture(0)
 call(64)
 assert stub.stub_live() == a + 4                   # the three handles' and the block's own
 """)
+
+
+def test_folded_layout_is_not_built_under_capture(stub):
+    stub("""
+sd.init(0)
+w = sd.SeedDeltaWeight(make_payload(1024, 2048, scheme="coo", K=16, base=True, seed=1))
+call = lambda T: w.forward_device(4096, 1024, T, 8192, 2048, sd.FWD_MFMA_FOLD)
+w.forward_device(4096, 1024, 2048, 8192, 2048, sd.FWD_NO_MFMA)      # a workspace that is large enough
+live = stub.stub_live()
+stub.stub_capture(1)
+assert "eagerly" in refused(lambda: call(16), -4)
+stub.stub_capture(0)
+assert stub.stub_live() == live
+""")
