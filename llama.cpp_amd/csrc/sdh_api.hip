@@ -529,12 +529,15 @@ static int device_to_host_sync(LibState & L, float * dst, int64_t ld, const floa
 }
 
 // per-call non-finite counter: ring slot, the second half of the ring is re-zeroed while the
-// first half is in use (one small memset every NF_SLOTS/2 calls, none on the other calls)
+// first half is in use (one small launch every NF_SLOTS/2 calls, none on the other calls; no memset, as the call may be recorded
+// into a graph, and memset nodes have given wrong results on replays)
+static __global__ void nf_clear_kernel(int * p) { p[threadIdx.x] = 0; }
 static int nf_slot(DeviceWeight * w, hipStream_t s, int * slot_out) {
     constexpr int NS = DeviceWeight::NF_SLOTS;
     const int slot = (int) (w->seq % NS);
     if (w->seq > 0 && slot % (NS / 2) == 0) {
-        SDH_HIP_CHECK(hipMemsetAsync(w->nf_ring + slot, 0, (NS / 2) * sizeof(int), s));
+        hipLaunchKernelGGL(nf_clear_kernel, dim3(1), dim3(NS / 2), 0, s, w->nf_ring + slot);
+        SDH_HIP_CHECK(hipGetLastError());
     }
     *slot_out = slot;
     return SDH_OK;

@@ -8,7 +8,7 @@
 
 static _Thread_local int device;
 static _Thread_local hipError_t last;
-static int devices = 2, capturing, launches, live, copies, fail_copy = -1, sticky = 1;
+static int devices = 2, capturing, launches, memsets, live, copies, fail_copy = -1, sticky = 1;
 
 static hipError_t done(hipError_t e) {
     if (e != hipSuccess || !sticky) last = e;
@@ -21,6 +21,7 @@ void stub_stale_error(void) { last = hipErrorInvalidValue; }
 void stub_capture(int on) { capturing = on; }
 int stub_live(void) { return live; }
 int stub_launches(void) { return launches; }
+int stub_memsets(void) { return memsets; }          /* asynchronous ones: nodes of a graph under capture */
 int stub_device(void) { return device; }
 void stub_set_device(int d) { device = d; }
 
@@ -76,7 +77,7 @@ hipError_t hipMemcpy2D(void * to, size_t tp, const void * from, size_t fp, size_
     return done(hipSuccess);
 }
 hipError_t hipMemset(void * p, int v, size_t n) { memset(p, v, n); return done(hipSuccess); }
-hipError_t hipMemsetAsync(void * p, int v, size_t n, hipStream_t s) { (void) s; memset(p, v, n); return done(hipSuccess); }
+hipError_t hipMemsetAsync(void * p, int v, size_t n, hipStream_t s) { (void) s; ++memsets; memset(p, v, n); return done(hipSuccess); }
 hipError_t hipLaunchKernel(const void * f, dim3 g, dim3 b, void ** a, size_t l, hipStream_t s) { (void) f; (void) g; (void) b; (void) a; (void) l; (void) s; ++launches; return done(hipSuccess); }
 hipError_t __hipPushCallConfiguration(dim3 g, dim3 b, size_t l, hipStream_t s) { (void) g; (void) b; (void) l; (void) s; return hipSuccess; }
 hipError_t __hipPopCallConfiguration(dim3 * g, dim3 * b, size_t * l, hipStream_t * s) { memset(g, 0, sizeof *g); memset(b, 0, sizeof *b); *l = 0; *s = 0; return hipSuccess; }

@@ -572,3 +572,45 @@ def test_direct_decode_captured_without_a_warm_up_call(hip):
     for i in range(3):
         assert np.array_equal(bits(outs[i]), bits(w.forward_host(xs[i:i + 1])))
         check_fast(p, xs[i:i + 1], outs[i], O.forward(p, xs[i:i + 1], nth=8))
+
+
+def test_nonfinite_counts_past_the_ring_of_counters(hip):
+    """Each call counts into the next of a ring of counters, half of which is cleared when the ring comes round: eagerly, and by the call
+    that happens to be recorded into a graph (replays of it count and clear in order)."""
+    torch = pytest.importorskip("torch")
+    p = make_payload(256, 512, scheme="coo", K=16, base=False, seed=1)
+    w, rng = hip.SeedDeltaWeight(p), np.random.default_rng(0)
+    x, y = torch.zeros((1, 256), device="cuda"), torch.zeros((1, 512), device="cuda")
+    call = lambda st=0: w.forward_device(x.data_ptr(), 256, 1, y.data_ptr(), 512, stream=st)  # noqa: E731
+
+    def fill(bad):
+        v = rng.standard_normal((1, 256)).astype(np.float32)
+        v[0, rng.choice(256, bad, replace=False)] = np.nan
+        x.copy_(torch.from_numpy(v))
+        torch.cuda.synchronize()
+
+    def check():
+        torch.cuda.synchronize()
+        n = int((~torch.isfinite(y)).sum())
+        assert w.nonfinite_count() == n
+        return n
+
+    for i in range(400):                                  # the ring has 256
+        fill(i % 5)
+        call()
+        assert (check() > 0) == (i % 5 > 0)
+    fill(3)
+    for i in range(400, 500):
+        call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        for i in range(500, 540):                         # 512 clears the counters of 512 .. 639
+            call(torch.cuda.current_stream().cuda_stream)
+    for rep in range(3):
+        fill(rep + 1)
+        g.replay()
+        assert check() > 0
+        torch.zeros(8, device="cuda").sum().item()

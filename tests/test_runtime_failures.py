@@ -168,3 +168,16 @@ assert "eagerly" in refused(lambda: call(16), -4)
 stub.stub_capture(0)
 assert stub.stub_live() == live
 """)
+
+
+def test_no_memset_node_is_recorded(stub):
+    """The ring of non-finite counters is cleared by a kernel: a call of any number may be the one that is recorded."""
+    stub("""
+sd.init(0)
+w = sd.SeedDeltaWeight(make_payload(256, 512, scheme="coo", K=16, base=False, seed=1))
+stub.stub_capture(1)
+n = stub.stub_memsets()
+for _ in range(600):
+    w.forward_device(4096, 256, 1, 8192, 512)
+assert stub.stub_memsets() == n and stub.stub_launches() >= 600
+""")
