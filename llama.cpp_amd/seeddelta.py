@@ -513,6 +513,8 @@ class SeedDeltaContext:
         at = w if w is not None else d
         if s is not None and (s.n_in, s.n_out) != (at.n_in, at.n_out):
             raise SeedDeltaError(f"mul_mat_device: {key}: adapters of {s.n_in} -> {s.n_out} beside a weight of {at.n_in} -> {at.n_out}")
+        if T == 0:
+            return True
         from . import sublayer
         if w is not None:
             w.forward_device(x_ptr, ldx, T, y_ptr, ldy, flags, stream)

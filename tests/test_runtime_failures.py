@@ -181,3 +181,21 @@ for _ in range(600):
     w.forward_device(4096, 256, 1, 8192, 512)
 assert stub.stub_memsets() == n and stub.stub_launches() >= 600
 """)
+
+
+def test_no_tokens_are_no_work_for_any_key(stub):
+    """An empty batch has null pointers (an empty tensor's); a payload, a dense weight and adapters take it alike."""
+    stub("""
+sd.init(0)
+ctx = sd.SeedDeltaContext()
+assert ctx.try_add("up", make_payload(256, 512, scheme="coo", K=16, base=True, seed=1))
+ctx.add_dense("gate", make_dense(256, 512))
+for k in ("up", "gate"):
+    ctx.add_adapters(k, [(np.zeros((4, 256), np.float16), np.zeros((512, 4), np.float16), 1.0)])
+n = stub.stub_launches()
+for k in ("up", "gate"):
+    for ids in (0, 4096):
+        assert ctx.mul_mat_device(k, 0, 256, 0, 0, 512, x8=sublayer.Q8View(0, 256, 0, 8), ids_ptr=ids) is True
+assert ctx.mul_mat_device("down", 0, 256, 0, 0, 512) is False
+assert stub.stub_launches() == n
+""")
