@@ -517,6 +517,7 @@ class SeedDeltaContext:
             return True
         from . import sublayer
         if w is not None:
+            sublayer.q8_quantize_device(0, 0, 0, 0, None)       # no tokens: that the current device is the bound one, which sdh_forward does not check
             w.forward_device(x_ptr, ldx, T, y_ptr, ldy, flags, stream)
         else:
             sublayer.dense_forward_q8_device(d, x8, T, y_ptr, ldy, stream)

@@ -199,3 +199,22 @@ for k in ("up", "gate"):
 assert ctx.mul_mat_device("down", 0, 256, 0, 0, 512) is False
 assert stub.stub_launches() == n
 """)
+
+
+def test_mul_mat_device_launches_nothing_on_another_device(stub):
+    stub("""
+sd.init(0)
+ctx = sd.SeedDeltaContext()
+assert ctx.try_add("up", make_payload(256, 512, scheme="coo", K=16, base=True, seed=1))
+ctx.add_dense("gate", make_dense(256, 512))
+call = lambda k: ctx.mul_mat_device(k, 4096, 256, 16, 8192, 512, x8=sublayer.Q8View(4096, 256, 8192, 8))
+n = stub.stub_launches()
+stub.stub_set_device(1)
+for k in ("up", "gate"):
+    assert "current device is 1" in refused(lambda: call(k), -1)
+assert stub.stub_launches() == n
+stub.stub_set_device(0)
+for k in ("up", "gate"):
+    assert call(k)
+assert stub.stub_launches() > n
+""")
