@@ -456,8 +456,8 @@ def llama_seeddelta_mul_mat_base_block(x, w_ref, base_d1, base_d2, base_d3, base
 class SeedDeltaContext:
     """Mirror of ``llama_seeddelta_context`` (src/llama-seeddelta.h:27-38): dense-weight key ->
     device payload, filled with the acceptance rules of ``try_add_seeddelta``
-    (src/llama-context.cpp:145-286; enforced inside sdh_weight_create), and of the rest of ``build_lora_mm``
-    (src/llama-graph.cpp:672-746) on the device: the weights that stay dense and the adapters of either."""
+    (src/llama-context.cpp:145-286; enforced inside sdh_weight_create); beside the payloads the other operands of ``build_lora_mm``
+    (src/llama-graph.cpp:672-746): the weights that stay dense and the adapters of either."""
 
     def __init__(self, enabled: bool = True, gap_tol: float = 0.02):
         self.enabled = enabled
@@ -504,9 +504,15 @@ class SeedDeltaContext:
 
     def mul_mat_device(self, key, x_ptr: int, ldx: int, T: int, y_ptr: int, ldy: int, x8=None, ids_ptr: int = 0,
                        ws_ptr: int = 0, ws_bytes: int = 0, flags: int = 0, stream: int = 0) -> bool:
-        """build_lora_mm whole, on device buffers: the key's payload (from x), else its dense weight (from x8, the same activations in
-        8 bits as sublayer.rms_norm_device writes them beside x), then the adapters of the tokens' `ids` added in place (read from x;
-        none registered, or no ids: none added). False: the key has neither payload nor dense weight, nothing was done."""
+        """build_lora_mm on device buffers, with one adapter per token: the key's payload (from x), else its dense weight (from x8, the
+        same activations in 8 bits as sublayer.rms_norm_device writes them beside x), then scale * B (A x) of the adapter that `ids`
+        (int32 on the device) gives each token, added in place. No ids or no adapters registered: none added. One adapter for all
+        tokens, or several on one token (the reference adds every active one): LoraSet.apply_device after this call, base = y.
+        False: the key has neither payload nor dense weight, nothing was done.
+
+        Graphs and streams: with a dense key the call allocates nothing and may be recorded as its first call; calls that may overlap take a
+        workspace each. With a payload key the rules of sdh_forward hold: one eager call of as many tokens before it is recorded, and
+        calls on one key are ordered by the caller whatever their streams (its handle owns a workspace and a hand-off buffer)."""
         w, d, s = self.find(key) if self.enabled else None, self.dense.get(key), self.adapters.get(key)
         if w is None and d is None:
             return False
