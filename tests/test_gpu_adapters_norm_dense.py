@@ -561,6 +561,160 @@ def test_lora_a_token_does_not_depend_on_the_others(hip, T):
     assert np.array_equal(bits(run_lora(ads, other, T, x=x, base=None)[0][0]), bits(a[0]))
 
 
+# ---- adapters, tokens sorted by the plan ----------------------------------------------------------------------------
+# More than 256 tokens, or more than 64 of more adapters than a wave deals by itself, are sorted by lora_plan_kernel. The workspace begins with
+# its permutation of the tokens, so a test sees that it ran.
+def tokens_in_order(ws, T):
+    """The workspace's first T numbers, if they are a permutation of the tokens; None: nothing was sorted."""
+    perm = ws[:4 * T].cpu().numpy().view(np.int32)
+    return perm if np.array_equal(np.sort(perm), np.arange(T)) else None
+
+
+def run_planned(adapters, ids, x, base=None, pad=0, shift=0):
+    """-> (y, 64-bit y, bound); the plan is checked: tokens of an adapter in a row, adapters in order, those without one last"""
+    T, n_out, n = len(ids), adapters[0][1].shape[0], len(adapters)
+    s, idd = sublayer.LoraSet(adapters), dev(np.asarray(ids, np.int32))
+    xs, y = padded(x, pad, shift), Out(T, n_out, pad, shift)
+    bs = (None, 0, 0) if base is None else padded(base, pad, shift)
+    ws = torch.full((s.workspace_bytes(T) + 64,), 0x5b, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    s.apply_device(idd.data_ptr(), xs[1], xs[2], T, y.ptr, y.ld, base_ptr=bs[1], ldb=bs[2], ws_ptr=ws.data_ptr(), ws_bytes=ws.numel() - 64)
+    got = y.get()
+    assert torch.all(ws[-64:] == 0x5b), "written behind the workspace"
+    perm = tokens_in_order(ws, T)
+    assert perm is not None, "not sorted by the plan: the dispatch rule has changed"
+    bins = np.where((ids >= 0) & (ids < n), ids, n)
+    assert np.all(np.diff(bins[perm]) >= 0)
+    s.close()
+    return got, *lora_ref(adapters, np.asarray(ids), x, base, n_out)
+
+
+@pytest.mark.parametrize("T, n, planned", [(64, 40, False), (65, 15, False), (65, 16, True), (128, 16, True), (256, 7, False), (256, 8, True), (257, 1, True), (300, 0, False)])
+def test_lora_which_calls_sort_tokens(hip, T, n, planned):
+    """n = 0: no ids"""
+    s = sublayer.LoraSet(make_adapters(32, 40, [4] * max(n, 1), ["h"] * max(n, 1)))
+    x, y, ids = torch.randn(T, 32, device="cuda"), torch.empty(T, 40, device="cuda"), dev(some_ids(T, max(n, 1), "each", T).astype(np.int32))
+    ws = torch.full((s.workspace_bytes(T),), 0x5b, dtype=torch.uint8, device="cuda")
+    s.apply_device(ids.data_ptr() if n else 0, x.data_ptr(), 32, T, y.data_ptr(), 40, ws_ptr=ws.data_ptr(), ws_bytes=ws.numel())
+    torch.cuda.synchronize()
+    assert (tokens_in_order(ws, T) is not None) == planned
+    assert planned or torch.all(ws[:4 * T] == 0x5b)
+    s.close()
+
+
+@pytest.mark.parametrize("T", [65, 300, 1024, 4095, 4096, 4097, 9000])
+@pytest.mark.parametrize("n", [16, 40, 1000, 4096])
+@pytest.mark.parametrize("order", ["runs", "gaps"])
+def test_lora_planned_token_and_adapter_counts(hip, T, n, order):
+    rng = np.random.default_rng(T + n)
+    ads = [(rng.standard_normal((1 + i % 5, 20)).astype(np.float16), rng.standard_normal((24, 1 + i % 5)).astype(np.float32 if i % 3 else np.float16), 0.5 + i % 4) for i in range(n)]
+    got, want, bound = run_planned(ads, some_ids(T, n, order, T), rng.standard_normal((T, 20)).astype(np.float32), rng.standard_normal((T, 24)).astype(np.float32))
+    assert np.all(np.abs(got - want) <= bound)
+
+
+@pytest.mark.parametrize("ids", [np.full(300, -1), np.full(300, 2), np.full(5000, 7), np.arange(300) % 3, np.r_[np.zeros(4999, int), 1], np.r_[2, np.full(4999, -5)]])
+def test_lora_planned_lopsided_batches(hip, ids):
+    rng = np.random.default_rng(len(ids))
+    x, base = rng.standard_normal((len(ids), 70)).astype(np.float32), rng.standard_normal((len(ids), 90)).astype(np.float32)
+    got, want, bound = run_planned(make_adapters(70, 90, [16, 3, 40], ["h", "f", "h"]), ids, x, base)
+    assert np.all(np.abs(got - want) <= bound)
+    none = (ids < 0) | (ids >= 3)
+    assert np.array_equal(got[none], base[none])
+
+
+@pytest.mark.parametrize("rank", [1, 8, 9, 16, 33, 64, 65, 100, 130, 512])
+@pytest.mark.parametrize("ty", ["h", "f"])
+def test_lora_planned_ranks(hip, rank, ty):
+    rng = np.random.default_rng(rank)
+    got, want, bound = run_planned(make_adapters(96, 132, [rank, 5], [ty, "h"], seed=rank), some_ids(300, 2, "each", rank), rng.standard_normal((300, 96)).astype(np.float32))
+    assert np.all(np.abs(got - want) <= bound)
+
+
+@pytest.mark.parametrize("n_in, n_out", [(1, 1), (3, 5), (31, 33), (127, 1025), (130, 1028), (544, 2052), (1000, 999)])
+@pytest.mark.parametrize("pad, shift", [(4, 0), (3, 1), (0, 2)])
+def test_lora_planned_shapes_and_strides(hip, n_in, n_out, pad, shift):
+    rng = np.random.default_rng(n_in)
+    x, base = rng.standard_normal((300, n_in)).astype(np.float32), rng.standard_normal((300, n_out)).astype(np.float32)
+    got, want, bound = run_planned(make_adapters(n_in, n_out, [4, 20], ["h", "f"], seed=n_in), some_ids(300, 2, "gaps", 5), x, base, pad=pad, shift=shift)
+    assert np.all(np.abs(got - want) <= bound)
+
+
+@pytest.mark.parametrize("T", [300, 5000])
+@pytest.mark.parametrize("rank", [5, 16, 70])
+def test_lora_planned_values_that_are_not_finite_stay_with_their_token(hip, T, rank):
+    x = np.random.default_rng(1).standard_normal((T, 96)).astype(np.float32)
+    x[T // 2, 11], x[0, 95] = np.inf, np.nan
+    with np.errstate(invalid="ignore"):
+        got, want, bound = run_planned(make_adapters(96, 140, [rank, 9], ["h", "f"]), some_ids(T, 2, "each", 8), x)
+    bad = np.zeros(T, bool)
+    bad[[0, T // 2]] = True
+    assert np.all(~np.isfinite(got[bad]))
+    assert np.all(np.abs(got[~bad] - want[~bad]) <= bound[~bad])
+
+
+@pytest.mark.parametrize("T", [300, 5000])
+def test_lora_planned_token_does_not_depend_on_its_place(hip, T):
+    """The atomics give a token its place in its adapter's run: another order of the tokens, other neighbours and a second run of the same
+    call give every token the same bits."""
+    ads = make_adapters(300, 500, [16, 8, 24], ["h", "f", "h"])
+    rng = np.random.default_rng(0)
+    x, ids, perm = rng.standard_normal((T, 300)).astype(np.float32), some_ids(T, 3, "gaps", 1), rng.permutation(T)
+    a = run_planned(ads, ids, x)[0]
+    assert np.array_equal(bits(run_planned(ads, ids, x)[0]), bits(a))
+    assert np.array_equal(bits(run_planned(ads, ids[perm], x[perm])[0]), bits(a[perm]))
+    other = ids.copy()
+    other[1::2] = -1
+    assert np.array_equal(bits(run_planned(ads, other, x)[0][::2]), bits(a[::2]))
+
+
+@pytest.mark.parametrize("T", [300, 5000])
+def test_lora_planned_captured_and_replayed(hip, T):
+    """Recorded as the set's first call; every replay sorts the ids that it finds, with eager calls on the same set in between."""
+    n_in, n_out, rng = 160, 264, np.random.default_rng(T)
+    s = sublayer.LoraSet(make_adapters(n_in, n_out, [16, 4, 33], ["h", "f", "h"]))
+    mk = lambda: dict(x=torch.empty(T, n_in, device="cuda"), y=torch.empty(T, n_out, device="cuda"), ids=torch.zeros(T, dtype=torch.int32, device="cuda"),  # noqa: E731
+                      ws=torch.full((s.workspace_bytes(T),), 0x5b, dtype=torch.uint8, device="cuda"))
+    call = lambda b, st: s.apply_device(b["ids"].data_ptr(), b["x"].data_ptr(), n_in, T, b["y"].data_ptr(), n_out, base_ptr=b["y"].data_ptr(), ldb=n_out, ws_ptr=b["ws"].data_ptr(), ws_bytes=b["ws"].numel(), stream=st)  # noqa: E731
+    cap, eager, side = mk(), mk(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        call(cap, torch.cuda.current_stream().cuda_stream)
+    for rep in range(4):
+        x, y, ids = rng.standard_normal((T, n_in)).astype(np.float32), rng.standard_normal((T, n_out)).astype(np.float32), some_ids(T, 3, ("each", "runs", "gaps", "gaps")[rep], rep)
+        for b in (cap, eager):
+            b["x"].copy_(dev(x)); b["y"].copy_(dev(y)); b["ids"].copy_(dev(ids.astype(np.int32)))
+        g.replay()
+        call(eager, 0)
+        torch.cuda.synchronize()
+        assert torch.equal(cap["y"], eager["y"]), rep
+        assert tokens_in_order(cap["ws"], T) is not None
+        want, bound = lora_ref(make_adapters(n_in, n_out, [16, 4, 33], ["h", "f", "h"]), ids, x, y, n_out)
+        assert np.all(np.abs(cap["y"].cpu().numpy() - want) <= bound)
+    s.close()
+
+
+def test_lora_planned_on_two_streams_at_once(hip):
+    T, n_in, n_out = 600, 512, 1024
+    s = sublayer.LoraSet(make_adapters(n_in, n_out, [16, 8], ["h", "f"]))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    xs = [torch.randn(T, n_in, generator=g, device="cuda") for _ in range(2)]
+    ids = [torch.randint(-1, 2, (T,), generator=g, device="cuda", dtype=torch.int32) for _ in range(2)]
+    ws = [torch.empty(s.workspace_bytes(T), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    run = lambda k, y, st: s.apply_device(ids[k].data_ptr(), xs[k].data_ptr(), n_in, T, y.data_ptr(), n_out, ws_ptr=ws[k].data_ptr(), ws_bytes=ws[k].numel(), stream=st)  # noqa: E731
+    lone, both, streams = [torch.empty(T, n_out, device="cuda") for _ in range(2)], [torch.empty(T, n_out, device="cuda") for _ in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    for k in range(2):
+        run(k, lone[k], 0)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for k in range(2):
+            run(k, both[k], streams[k].cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(lone[0], both[0]) and torch.equal(lone[1], both[1])
+    assert all(tokens_in_order(w, T) is not None for w in ws)
+    s.close()
+
+
 def test_lora_strided_host_views(hip):
     rng = np.random.default_rng(0)
     big_a, big_b = rng.standard_normal((40, 200)).astype(np.float16), rng.standard_normal((12, 300)).astype(np.float16)
