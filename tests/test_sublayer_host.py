@@ -1,6 +1,8 @@
 """What the operators around the projections refuse, without a GPU: every check of arguments comes before the first use of the
 device, so a bad call is an SDH_ERR_INVALID here and a good one ends at the missing device."""
 import ctypes as C
+import re
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -110,3 +112,13 @@ def test_dense_weights_of_ragged_rows_are_refused(W, monkeypatch):
 def test_dense_weights_of_whole_blocks_end_at_the_device():
     with pytest.raises(sd.SeedDeltaError, match=NO_DEVICE):
         scan.DenseWeight(np.zeros((3, 68), np.uint8))
+
+
+def test_device_code_is_compiled_without_packed_fp32():
+    """Every line that compiles HIP code, the measurement helpers' included, switches the packed instructions off."""
+    root, lines = Path(__file__).resolve().parent.parent, []
+    for f in [root / "llama.cpp_amd/csrc/Makefile", *root.glob("tools/*.sh"), *root.glob("tools/*.hip"), *root.glob("tools/gpu/*")]:
+        text = f.read_text()
+        lines += [(f.name, line) for line in text.splitlines() if re.search(r"hipcc\b.*\.hip\b|^CFLAGS", line) and " -shared " not in line]
+    assert len(lines) >= 9
+    assert [x for x in lines if "-Xclang -target-feature -Xclang -packed-fp32-ops" not in x[1]] == []

@@ -1,6 +1,6 @@
 // base_diag.hip — diagnostic build of the library with in-kernel time stamps in the base-term
 // kernel (development tool). Prints where a cold base_apply launch spends its time.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Iinclude -o tools/bin/base_diag tools/base_diag.hip
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -Iinclude -o tools/bin/base_diag tools/base_diag.hip
 #define SDH_DIAG_STAMPS 1
 #include "../llama.cpp_amd/csrc/sdh_api.hip"
 #include "../llama.cpp_amd/csrc/sdh_base.hip"

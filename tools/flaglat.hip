@@ -1,6 +1,6 @@
 // flaglat.hip — dev tool: how long from an agent-scope 8-byte store in one workgroup until a polling
 // agent-scope load in another workgroup sees it, same XCD vs different XCD (s_memrealtime, 10 ns ticks).
-//   hipcc --offload-arch=gfx950 -O3 -o tools/bin/flaglat tools/flaglat.hip
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/bin/flaglat tools/flaglat.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

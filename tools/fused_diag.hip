@@ -1,7 +1,7 @@
 // fused_diag.hip — diagnostic build of the fused decode kernel with in-kernel time stamps
 // (development tool): when do the base workgroups finish, when do the residual waves finish their
 // own work, and how long do they wait for the base term.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Iinclude -o tools/bin/fused_diag tools/fused_diag.hip
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -Iinclude -o tools/bin/fused_diag tools/fused_diag.hip
 #ifndef SDH_DIAG_NO_STAMPS
 #define SDH_DIAG_STAMPS 1
 #endif

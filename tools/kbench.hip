@@ -6,7 +6,7 @@
 // launches rotating over NPAY distinct buffers (> 256 MB in total, so the Infinity Cache does not
 // serve them).
 //
-//   hipcc --offload-arch=gfx950 -O3 -o kbench tools/kbench.hip -Iinclude -Lllama.cpp_amd/csrc -lseeddelta_hip
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o kbench tools/kbench.hip -Iinclude -Lllama.cpp_amd/csrc -lseeddelta_hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -1,6 +1,6 @@
 // placement.hip — dev tool: where does the dispatcher put the workgroups of one launch?
 // Every workgroup records its (XCC, SE, CU) and stays resident for ~20 us; prints workgroups per CU.
-//   hipcc --offload-arch=gfx950 -O3 -o tools/bin/placement tools/placement.hip
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/bin/placement tools/placement.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <map>
