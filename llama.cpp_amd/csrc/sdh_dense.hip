@@ -154,7 +154,7 @@ __global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) dxs[wave][2 * h + i][m] = bs + 2 * h + i >= b0 ? dx[i] : 0.0f;
         load(b0 + 4 * NW);                                       // past the end: in bounds and not used
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int at = m * 8 + ((2 * k + h) ^ key);
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(512, 4) void dense_mid_kernel(const DenseArgs a) {
                 acc[4 * q + 3] = fmaf((float) z[4 * q + 3], d.w * dc[k], acc[4 * q + 3]);
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
     }
     __syncthreads();
     float * part = reinterpret_cast<float *>(turn);              // [NW][32][33]
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(512, TT * RR == 1 ? 8 : TT + RR <= 4 ? 4 : 2) void 
 #pragma unroll
         for (int i = 0; i < TT; ++i) dxs[wave][dxb + i][dxt] = bs + dxb + i >= b0 ? dx[i] : 0.0f;
         load(b0 + 4 * NW);                                       // past the end: in bounds and not used
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int at = 2 * (m * 8 + ((2 * k + (g >> 1)) ^ key)) + (g & 1);         // 8 bytes
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(512, TT * RR == 1 ? 8 : TT + RR <= 4 ? 4 : 2) void 
                 }
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
     }
     __syncthreads();
     float * part = reinterpret_cast<float *>(turn);              // [NW][16 TT][16 RR + 1]

@@ -241,6 +241,12 @@ int ready_on_device(const char * who);
 struct DenseQ8 { const int8_t * q; const uint16_t * d; int64_t n_in, n_out; int type, device; };   // [n_out][n_in], f16 [n_out][n_in/32]
 DenseQ8 dense_q8(const sdh_dense * W);     // sdh_scan.hip (the handle's layout)
 std::vector<float> tensor_f32(const sdh_tensor & t);     // F16 / F32, any strides -> contiguous F32 [ne1][ne0], exact (sdh_api.hip)
+// Between a wave's stores to LDS and its other lanes' loads of them. LDS works in order within a wave, so nothing has to wait; the fence keeps
+// the compiler from moving either past it (the barrier by itself orders lanes, not memory).
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+}
 inline bool aligned(const void * p, size_t a) { return ((uintptr_t) p & (a - 1)) == 0; }
 
 int launch_w0_tile(const DeviceWeight & w, int64_t o0, int64_t o1, int64_t i0, int64_t i1,

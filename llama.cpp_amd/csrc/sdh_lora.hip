@@ -310,7 +310,7 @@ __device__ __forceinline__ void shrink_steps(const float * const (&xr)[4], const
             for (int j = 0; j < NJ; ++j) ac[u][j] = an[u][j];
         }
         if (k + 128 * U < k_end) load(k + 128 * U);
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (u && k + 128 * u >= k_end) break;
@@ -328,7 +328,7 @@ __device__ __forceinline__ void shrink_steps(const float * const (&xr)[4], const
 #pragma unroll
                         for (int i = 0; i < NS; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[i][h][q], ac[u][j].get(h, q), acc[i][j], 0, 0, 0);
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
     }
 }
 
@@ -394,6 +394,7 @@ void lora_shrink_kernel(const LoraAdapter * __restrict__ ads, int n, const int *
     const int split = (int) (blockIdx.x % (unsigned) splits), rest = (int) (blockIdx.x / (unsigned) splits), rc = rest % n_z * LORA_RC;
     int a = -1;
     const int count = lora_tokens<DEAL>(tiles, n_tiles, perm, ids, (int) T, n, rest / n_z, LT, list, &a);
+    wave_lds_order();                                       // the list
     const LoraAdapter ad = ads[max(a, 0)];                  // on its way beside the ids where `a` does not come from them
     if (!count || a < 0 || rc >= ad.rank) return;
     const int64_t k0 = split * k_split, k1 = min(a_ld, k0 + k_split);
@@ -472,6 +473,7 @@ void lora_expand_kernel(const LoraAdapter * __restrict__ ads, int n, const int *
     int * list = lists[wave];
     int a = -1;
     const int all = lora_tokens<DEAL>(tiles, n_tiles, perm, ids, (int) T, n, at, ET, list, &a);
+    wave_lds_order();                                       // the list
     const LoraAdapter ad = ads[max(a, 0)];
     if (!all || (a < 0 && base == y)) return;
     ExpandWave e{list, all, us, 0, 0, n_out, base, ldb, y, ldy};
