@@ -387,7 +387,7 @@ int64_t sdh_dense_bytes(const sdh_dense * W);      /* bytes as stored (the scan'
 /* sdh_dense_forward_q8 — a dense Q8_0 weight times 8-bit activations, for the projections of a layer that have no payload:
  *   y[o,t] = sum_b d_w[b,o] * d[b,t] * sum_{i in block b} q_w[i,o] * q[i,t]
  * the arithmetic of ggml's Q8_0 mul_mat (ggml_vec_dot_q8_0_q8_0, ggml/src/ggml-cpu/quants.c): integer sums inside a block
- * of 32, F32 across blocks. x: [n_in, n_tokens] as sdh_rms_norm / sdh_q8_quantize write it, x->q 16-byte aligned with ldq a
+ * of 32, F32 across blocks (as is the product of a block's two scales: past F32's range it is infinite). x: [n_in, n_tokens] as sdh_rms_norm / sdh_q8_quantize write it, x->q 16-byte aligned with ldq a
  * multiple of 16. y: F32 [n_out, n_tokens] with column stride ldy. Same rules as the calls around the projections above.
  * F16 / F32 weights: SDH_ERR_UNSUPPORTED. */
 int     sdh_dense_forward_q8(const sdh_dense * W, const sdh_q8 * x, int64_t n_tokens, float * y, int64_t ldy, void * stream);

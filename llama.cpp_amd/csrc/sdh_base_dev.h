@@ -84,9 +84,9 @@ __device__ __forceinline__ void base_stages(float (&y)[Ly::E]) {
     constexpr int E = Ly::E, LOG_E = Ly::LOG_E;
     constexpr int b0 = JJ * LOG_E;
     constexpr int b1 = (b0 + LOG_E < Ly::N) ? b0 + LOG_E : Ly::N;
-    // Two butterflies per v_pk_add_f32: the same IEEE additions (u - w == u + (-w) exactly), half the VALU
-    // instructions of the stages. The transform of one block runs on one CU and is VALU-issue bound there
-    // (8 waves on 4 SIMDs); hipcc packs only about half of the scalar form by itself. cfg3: 8.06 -> 7.81 us.
+    // Two butterflies as one sum of pairs: the same IEEE additions (u - w == u + (-w) exactly). The transform of one block
+    // runs on one CU and is VALU-issue bound there (8 waves on 4 SIMDs). The pairs compile to two additions each: the library is
+    // built without packed FP32 instructions, some forms of which have given wrong results on this hardware.
     static_assert(E % 2 == 0, "E is a power of two >= 2");
     typedef float f32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
@@ -195,8 +195,8 @@ __device__ __forceinline__ float base_lane_xor(float v) {
 }
 
 // One stage on lane bit K: y = partner + sgn * y with sgn = +1 (bit clear) / -1 (bit set): partner - y is the fused
-// multiply-add partner + (-1 * y), exact product, ONE rounding — the butterfly's own addition. Two elements per
-// v_pk_fma_f32.
+// multiply-add partner + (-1 * y), exact product, ONE rounding — the butterfly's own addition. In pairs (two
+// instructions, packed FP32 being off).
 template <class Ly, int K>
 __device__ __forceinline__ void base_lane_stage(float (&y)[Ly::E], int lane) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));

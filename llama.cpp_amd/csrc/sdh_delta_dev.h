@@ -123,7 +123,7 @@ __device__ __forceinline__ float mul_then_add(float acc, float v, float x) {
     const float prod = v * x;
     return acc + prod;
 }
-// two tokens per instruction (v_pk_mul_f32, v_pk_add_f32): each component rounds as the scalar forms do
+// two tokens as a pair: each component rounds as the scalar form does (and is an instruction of its own, packed FP32 being off)
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2_t mul_then_add2(f32x2_t acc, float v, f32x2_t x) {
 #pragma clang fp contract(off)

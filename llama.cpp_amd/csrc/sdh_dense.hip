@@ -7,7 +7,7 @@
 //   dense_thin_kernel, dense_mid_kernel
 //                      a batch: 16 to 64 rows of v_mfma_i32_16x16x32_i8 or 32 x 32 tiles of v_mfma_i32_32x32x32_i8, whose K is exactly
 //                      one block, straight from memory.
-//   dense_mfma_kernel  a prompt: tiles of 64 x 64 to 128 x 128 through LDS, bound by the vector pipe (integers to F32).
+//   dense_mfma_kernel  a prompt: tiles of 64 x 64 to 128 x 128 through LDS; most of its time is the vector pipe's (integers to F32).
 #include "sdh_internal.h"
 
 #include <algorithm>
@@ -298,9 +298,10 @@ static void launch_thin(const DenseArgs & a, hipStream_t s) {
 // Many tokens: BM tokens x BN rows per workgroup, both operands through LDS in steps of SB blocks, two stages. A wave owns 32 tokens x
 // 32 NN rows; with KS = 2 two waves share them, each with every other block, joined at the end.
 //
-// What bounds it is the vector pipe, to whose time that of the matrix pipe adds (562,000 + 229,000 of 743,000 busy cycles per SIMD for
-// 2048 tokens x 4096 -> 14336: 356 us, 675 TOP/s): a 32x32x32 MFMA takes 32 cycles and leaves 16 integers per lane, each of which costs
-// a conversion and a fused multiply-add (packed F32 being off). The products of the scales come from v_mfma_f32_32x32x1_2b_f32, two
+// 2048 tokens x 4096 -> 14336 take 357 us, 674 TOP/s. Of 741,000 busy cycles per SIMD the vector pipe works 562,000 (76 %) and the matrix pipe
+// 229,000 (31 %): two pipes that can run at once, so neither alone is the bound yet. A wave waits for its MFMAs and converts then, and a
+// barrier per step keeps its neighbours in phase. The vector pipe alone would be about 270 us: a 32x32x32 MFMA takes 32 cycles and leaves
+// 16 integers per lane, each of which costs a conversion and a fused multiply-add (packed F32 being off). The products of the scales come from v_mfma_f32_32x32x1_2b_f32, two
 // tiles in 64 cycles (32 vector instructions of 4 cycles otherwise); a step's addresses are one operation each, and the operands' way
 // through registers is left out (loads to LDS), so two tiles take 128 cycles of the matrix pipe and 72 vector instructions, 288 cycles
 // (products by vector instructions and operands through registers: 424 us).
@@ -459,7 +460,7 @@ static void launch_mid(const DenseArgs & a, hipStream_t s) {
 // The forms from 2 tokens on: tile of tokens x rows, and its time in us per 128 bytes of K: per round in which the workgroups fill the CUs
 // (workgroups per CU, rounded up), plus `add`, `least` at least. `blocks`: the fewest blocks of a row; before that the start and the end
 // of a large tile count for more than its rounds (48 tokens x 1152 -> 6912: 32 x 64 8.9 us, 32 x 32 6.6). Fitted to nine shapes between 1152 and 28672 at 2 to 2048 tokens (a
-// call's time less 2 us). What the choice is worth, us:
+// call's time less 2 us); between these shapes nothing says how far the choice is from the best form. What the choice is worth, us:
 //   14336 -> 4096    11 tokens  16 x 16 11.7, 16 x 48 23, 16 x 64 29, 32 x 32 22.5;    32 tokens  32 x 16 17, 32 x 32 23, 32 x 64 39;
 //                    64 / 256 / 512 / 2048 tokens  32 x 32 23 / 79 / 156 / 642, 64 x 64 65 / 66 / 103 / 447, 64 x 128 120 / 114 / 116 / 425,
 //                    128 x 128 189 / 205 / 205 / 340
@@ -500,7 +501,8 @@ static int launch_dense(const DenseArgs & all, hipStream_t s) {
         DenseArgs a = all;
         a.T = std::min(chunk, all.T - t0);
         a.xq += t0 * a.ldq; a.xd += t0 * a.ldd; a.y += t0 * a.ldy;
-        // one token: 4096 -> 14336 11.6 us (16 x 64 tiles 12.7), 14336 -> 4096 13.3 (16 x 16 11.5), 6912 -> 1152 5.1 (6.3)
+        // one token takes the stream of rows whatever the shape: 4096 -> 14336 11.6 us (16 x 64 tiles 12.7), 6912 -> 1152 5.1 (6.3). Of the
+        // shapes measured 14336 -> 4096 loses by it: 13.3 us, 11.5 with 16 x 16 tiles; the costs above do not have this form yet
         if (all.T == 1)       { if (a.nblk >= 96) launch_few<1, 2, 4>(a, s); else launch_few<1, 2, 2>(a, s); }
         else if (form)        form->launch(a, s);
         else                  launch_few<2, 2, 4>(a, s);

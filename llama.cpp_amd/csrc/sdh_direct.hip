@@ -156,7 +156,7 @@ __device__ __forceinline__ float direct_row_dot(const DeltaParams & p, const flo
     return acc;
 }
 
-// 16-point Walsh-Hadamard transform in registers, two butterflies per packed add
+// 16-point Walsh-Hadamard transform in registers, butterflies in pairs
 __device__ __forceinline__ void wht16(float (&z)[16]) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll

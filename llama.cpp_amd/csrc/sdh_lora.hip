@@ -9,9 +9,10 @@
 // One to four tokens of small adapters take one launch (lora_fused_kernel) in which every workgroup forms u for itself.
 //
 // Kernel times (plan + shrink + expand), and what bounds them: 1 token, rank 16, 4096 -> 14336: 6.3 us (one launch and its chain of
-// loads: id, record, A, B). 48 tokens, 32 adapters of rank 32 and less: 5.9 + 11.1 us (the same chains; 22 MB). 512 tokens, rank 64 in
-// F32, 14336 -> 4096: 4.9 + 20 + 13 us (the products alone are 2 x 6 us at the rate of a large F32 product; x comes from the caches
-// twice, once per 32 ranks). 4096 tokens, rank 16, 4096 -> 14336: 7.6 + 23 + 96 us; the last one is 470 MB of base and y, 4.9 TB/s.
+// loads: id, record, A, B). 48 tokens, 32 adapters of rank 32 and less: 5.8 + 11.1 us (the same chains, made again by each of 33 x 56
+// workgroups; 22 MB). 512 tokens, rank 64 in F32, 14336 -> 4096: 4.7 + 19.4 + 13 us (the products alone are 6.1 and 1.8 us at the rate of a
+// large F32 product; one step of loads in flight per wave; x comes from the caches twice, once per 32 ranks). 4096 tokens, rank 16,
+// 4096 -> 14336: 7.4 + 22.7 + 93.6 us; the last one is 470 MB of base and y, 5.0 TB/s.
 //
 // Everything is F32: v_mfma_f32_16x16x4_f32 does 2048 operations in 32 cycles, and both steps move far more bytes than that costs
 // (8 bytes of y per 2 * rank operations, 4 of x per 2 * rank). Which k an MFMA takes is free as long as both operands agree: lane

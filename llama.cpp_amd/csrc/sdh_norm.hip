@@ -3,7 +3,8 @@
 //   s = x + res,  z = s * w / sqrt(mean(s^2) + eps),  per 32 values d = max|z| / 127, q = rint(z / d).
 //
 // One workgroup per token, the row in registers between the sum of squares and the outputs: every input is read once and the memory
-// bounds it. 8192 rows of 4096 with residual and 8-bit output: 78.1 us, 5.6 TB/s (torch's copy of a large tensor: 4.95). A lane holds 4 consecutive
+// bounds it. 8192 rows of 4096 with residual and 8-bit output: 76.7 us, 5.7 TB/s (torch's copy of a large tensor: 4.95); the conversion
+// alone of 2048 rows of 14336: 33.8 us, 4.5 TB/s, of one row 4.4 us. A lane holds 4 consecutive
 // values per step, so eight neighbouring lanes hold a block of 32 and its maximum is three lane exchanges.
 //
 // Arithmetic: s is rounded to F32 (the next layer reads it); from there on everything is in double and rounded once per output.
@@ -29,7 +30,7 @@ struct NormArgs {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 
-// NT: past the caches (rows that are more than the L2 holds together): 78.1 us against 92.8 for the prompt above
+// NT: past the caches (rows that are more than the L2 holds together): 76.7 us against 87.5 for the prompt above
 template <bool VEC, bool NT = false>
 __device__ __forceinline__ float4 load4(const float * p, int i, int n) {
     if constexpr (VEC && NT) { const v4f v = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(p + i)); return make_float4(v.x, v.y, v.z, v.w); }
@@ -66,8 +67,8 @@ __device__ __forceinline__ double block_sum(double v, double * red) {
 }
 
 // n / d, given 1 / d within 2^-40: one Newton step on the quotient. The remainder of the first one is exact (or rounds past its 50th bit), so
-// what is left is rounded once, to n / d itself where that is a double. (Two divisions a lane and three operations a value more than these
-// took 36.9 us instead of 34.7 for 2048 x 14336.)
+// what is left is rounded once, to n / d itself where that is a double. 2048 x 14336 in 8 bits 33.7 us; with the compiler's divisions for the scale
+// and the reciprocal 36.9.
 __device__ __forceinline__ double quotient(double n, double d, double inv) {
     const double p = n * inv;
     return fma(fma(-p, d, n), inv, p);
@@ -185,7 +186,7 @@ static int launch_norm(const NormArgs & all, int64_t T, hipStream_t s) {
     const bool vec = all.n % 4 == 0 && ok(all.x, all.ldx) && ok(all.res, all.ldr) && ok(all.sum, all.lds) && ok(all.y, all.ldy) && ok(all.w, 0);
     const int q4 = (all.n + 3) / 4;
     // few rows: as many threads as there are groups of four values (one row of 4096: 4.8 us); many: four groups a thread, four
-    // workgroups of 256 for one of 1024 (8192 rows of 4096: 78.1 us against 90.4)
+    // workgroups of 256 for one of 1024 (8192 rows of 4096: 76.7 us against 88.6)
     const int nv = q4 > 4096 ? 0 : q4 > 2048 || (T > 2 * lib().num_cu && q4 >= 1024) ? 4 : q4 > 1024 ? 2 : 1;
     const bool nt = (int64_t) 4 * all.n * T > (32 << 20);
     constexpr int64_t CHUNK = 1 << 21;                      // a launch has fewer than 2^32 threads

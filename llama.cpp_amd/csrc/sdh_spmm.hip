@@ -151,8 +151,8 @@ void delta_spmm4_kernel(const DeltaParams p, int64_t T, int rows_per_wg) {
                 else for (int b = 0; b < p.B; ++b) y[u] += vt[(size_t) b * p.L + o];
             }
         }
-        // two tokens per instruction: v_pk_mul_f32 / v_pk_add_f32 round each component as the scalar forms do
-        // (contraction is off), so the sums keep the CPU op's bits at half the multiply and add instructions
+        // tokens in pairs: each component rounds as the scalar form does (contraction is off), so the sums keep the CPU op's bits
+        // (two instructions a pair, packed FP32 being off)
         float2v y01 = {y[0], y[1]}, y23 = {y[2], y[3]};
         auto mac = [&](float v, const xvec x) {
             const float2v vv = {v, v}, x01 = {x[0], x[1]};
