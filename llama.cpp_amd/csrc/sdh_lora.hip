@@ -42,6 +42,7 @@ struct LoraSet {
     int64_t n_in = 0, n_out = 0, a_ld = 0;
     int n = 0, u_ld = 0;                   // adapters; row pitch of u: the largest r_ld
     bool any_f32 = false;
+    int device = -1;
     uint8_t * dev = nullptr;               // the LoraAdapter table, then the matrices
     int64_t stored_bytes = 0;
 };
@@ -682,6 +683,7 @@ static int lora_create(int64_t n_in, int64_t n_out, const sdh_lora_desc * d, int
         l.any_f32 |= a.f32 != 0;
     }
     if (const int rc = ready_on_device("sdh_lora_create")) return rc;
+    l.device = lib().device;
     SDH_HIP_CHECK(hipMalloc((void **) &l.dev, total));
     struct Guard { uint8_t * p; ~Guard() { if (p) (void) hipFree(p); } } guard{l.dev};
     std::vector<uint8_t> buf, keep;
@@ -777,6 +779,7 @@ static int sdh_lora_apply_impl(const sdh_lora * h, const int32_t * ids, const fl
     if (!aligned(ids, 4) || !aligned(x, 4) || !aligned(base, 4) || !aligned(y, 4) || !aligned(ws, 16)) { set_error("%s: pointers need 4-byte alignment, the workspace 16", who); return SDH_ERR_INVALID; }
     const int rc = ready_on_device(who);
     if (rc != SDH_OK) return rc;
+    if (l.device != lib().device) { set_error("%s: the set was made on device %d, the library is bound to %d", who, l.device, lib().device); return SDH_ERR_INVALID; }
     const int64_t need = sdh_lora_workspace_bytes(h, T);
     if (ws_bytes < need) { set_error("%s: the workspace holds %lld bytes, %lld are needed", who, (long long) ws_bytes, (long long) need); return SDH_ERR_INVALID; }
     const int64_t chunk = lora_chunk(l);

@@ -218,3 +218,20 @@ for k in ("up", "gate"):
     assert call(k)
 assert stub.stub_launches() > n
 """)
+
+
+def test_adapters_of_another_device_are_refused(stub):
+    """A set that was made before the library was bound to another device is in the first one's memory."""
+    stub("""
+sd.init(0)
+s = sublayer.LoraSet([(np.zeros((4, 32), np.float16), np.zeros((48, 4), np.float16), 1.0)])
+call = lambda: s.apply_device(0, 4096, 32, 8, 8192, 48, ws_ptr=16384, ws_bytes=1 << 20)
+call()
+sd.init(1)
+n = stub.stub_launches()
+assert "made on device 0" in refused(call, -1)
+assert stub.stub_launches() == n
+sd.init(0)
+call()
+assert stub.stub_launches() > n
+""")
