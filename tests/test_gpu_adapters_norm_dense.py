@@ -936,6 +936,55 @@ def test_two_streams_at_once(hip):
     s.close()
 
 
+# ---- rows far apart -------------------------------------------------------------------------------------------------
+def far(T, n, dtype, align=4):
+    """(T, n) rows whose last one begins past 2^32 elements of a buffer -> (buffer, view, stride)"""
+    ld = (2 ** 32 // (T - 1) + n + align) // align * align
+    buf = torch.empty((T - 1) * ld + n, dtype=dtype, device="cuda")
+    return buf, buf.as_strided((T, n), (ld, 1)), ld
+
+
+@pytest.mark.parametrize("T", [3, 40, 700])
+def test_rows_past_32_bits_norm_and_dense(hip, T):
+    n, n_out = 256, 320
+    rng = np.random.default_rng(T)
+    x = rng.standard_normal((T, n)).astype(np.float32)
+    W = make_dense(n, n_out, "q8_0", 3)
+    keep, xv, ldx = far(T, n, torch.float32)
+    xv.copy_(dev(x))
+    kq, qv, ldq = far(T, n, torch.int8, 16)
+    d, y = torch.empty(T, n // 32, device="cuda"), torch.empty(T, n, device="cuda")
+    sublayer.rms_norm_device(xv.data_ptr(), ldx, n, T, eps=EPS, sum_ptr=xv.data_ptr(), lds=ldx, y_ptr=y.data_ptr(), ldy=n, q8=sublayer.Q8View(qv.data_ptr(), ldq, d.data_ptr(), n // 32))
+    torch.cuda.synchronize()
+    s, z = norm_ref(x, None, None)
+    assert np.array_equal(bits(xv.contiguous().cpu().numpy()), bits(s)) and np.all(np.abs(y.cpu().numpy() - z) <= (U + 1e-12) * np.abs(z))
+    q, dh = qv.contiguous().cpu().numpy(), d.cpu().numpy()
+    check_q8(q, dh, z)
+    del keep, xv
+    ko, ov, ldo = far(T, n_out, torch.float32)
+    w = scan.DenseWeight(W)
+    sublayer.dense_forward_q8_device(w, sublayer.Q8View(qv.data_ptr(), ldq, d.data_ptr(), n // 32), T, ov.data_ptr(), ldo)
+    want, mag = dense_ref(W, q, dh)
+    assert np.all(np.abs(ov.contiguous().cpu().numpy() - want) <= (n // 32 + 10) * U * mag)
+    w.close()
+
+
+@pytest.mark.parametrize("T", [3, 40, 130, 700])
+def test_rows_past_32_bits_adapters(hip, T):
+    n_in, n_out = 160, 300
+    ads, ids, rng = make_adapters(n_in, n_out, [8, 20, 33], ["h", "f", "h"]), some_ids(T, 3, "gaps", T), np.random.default_rng(T)
+    ids[-1] = 1
+    x, base = rng.standard_normal((T, n_in)).astype(np.float32), rng.standard_normal((T, n_out)).astype(np.float32)
+    (kx, xv, ldx), (ky, yv, ldy) = far(T, n_in, torch.float32), far(T, n_out, torch.float32)
+    xv.copy_(dev(x)); yv.copy_(dev(base))
+    s, idd = sublayer.LoraSet(ads), dev(ids.astype(np.int32))
+    ws = torch.empty(s.workspace_bytes(T), dtype=torch.uint8, device="cuda")
+    s.apply_device(idd.data_ptr(), xv.data_ptr(), ldx, T, yv.data_ptr(), ldy, base_ptr=yv.data_ptr(), ldb=ldy, ws_ptr=ws.data_ptr(), ws_bytes=ws.numel())
+    want, bound = lora_ref(ads, ids, x, base, n_out)
+    assert np.all(np.abs(yv.contiguous().cpu().numpy() - want) <= bound)
+    s.close()
+
+
 # ---- a run of them together -----------------------------------------------------------------------------------------
 @pytest.mark.parametrize("T", [1, 3, 40])
 def test_ffn_sublayer_with_a_dense_gate_and_adapters(hip, T):
